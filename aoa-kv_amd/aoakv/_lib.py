@@ -65,6 +65,16 @@ SIGNATURES = {
     "aoakv_rms_norm_forward": [_p, _p, _p, _u32, _u32, _f32, _p],
     "aoakv_rope_append_kv_cache_prefill": [_p, _p, _p, _u32, _u32, _p, _p, _u32, _u32, _p, _p,
                                            _p, _p, _u32, _u32, _u32, _u32, _f32, _f32, _p],
+    "aoakv_chunk_attn_workspace_size": [_u32, _u32],
+    "aoakv_chunk_attn": [_p, _p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
+                         _u32, _u32, _u32, _u32, _u32, _f32, _p, _sz, _p, _p],
+    "aoakv_attn_weights_workspace_size": [_u32],
+    "aoakv_attn_weights": [_p, _p, _p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32,
+                           _u32, _u32, _u32, _u32, _u32, _u32, _f32, _p, _sz, _p, _p],
+    "aoakv_keep_tokens": [_p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
+                          _p, _p],
+    "aoakv_compact_kv_cache": [_p, _u32, _u32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                               _u32, _u32, _u32, _u32, _u32, _u32, _p, _p],
     "aoakv_rope_append_kv_cache_decode": [_p, _p, _p, _u32, _u32, _p, _p, _p, _p, _p, _p, _p,
                                           _p, _p, _u32, _u32, _u32, _u32, _f32, _f32, _p],
 }
@@ -74,6 +84,8 @@ _RESTYPES = {
     "aoakv_decode_workspace_size": _sz,
     "aoakv_layer_workspace_size": _sz,
     "aoakv_prefill_workspace_size": _sz,
+    "aoakv_chunk_attn_workspace_size": _sz,
+    "aoakv_attn_weights_workspace_size": _sz,
 }
 
 

@@ -3,7 +3,7 @@
 Each function checks dtypes, devices and shapes, then calls the C ABI with
 raw device pointers on torch's current HIP stream.  Tensors are never
 copied or converted here: a wrong dtype / layout is an error, not a cast.
-The calls of the append, decode and prefill paths do this in C++ (aoakv._host,
+The calls of the append, decode, prefill and eviction paths do this in C++ (aoakv._host,
 csrc/host.cpp), where a call's checks cost more than a short kernel.
 """
 from __future__ import annotations
@@ -288,3 +288,66 @@ def prefill_with_paged_kv_cache(q, kv_data, kv_indices, num_kv_pages: int, kv_la
     pool has none the call runs without it, slower."""
     return _host.prefill_with_paged_kv_cache(q, o, kv_data, kv_indices, num_kv_pages,
                                              kv_last_page_len, layout, int(causal))
+
+
+def chunk_attn(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages: int,
+               layout: int, causal: bool = True, window: int = 0, soft_cap: float = 0.0,
+               slopes=None, prefix_len=None, o=None, return_lse: bool = False, workspace=None):
+    """Attention of the new tokens of every sequence of a batch (aoakv_chunk_attn).
+
+    q [T, Hq, D] fp16 holds the sequences' new tokens one after the other, rows
+    q_indptr[b] .. q_indptr[b + 1] - 1 (int32, device) those of sequence b, the
+    last of its cached ones (the page table counts them).  A score is
+    q . k / sqrt(D), then soft_cap * tanh(score / soft_cap) (``soft_cap`` > 0),
+    then less slopes[h] * distance (``slopes`` fp32 [Hq]).  A token sees itself
+    and what is before it (all, without ``causal``), no further back than
+    ``window`` tokens with itself (> 0), and the first prefix_len[b] tokens
+    (int32 [B]) in any case.  Returns o [T, Hq, D], with ``return_lse`` also
+    the fp32 [T, Hq] log of each row's sum of exponentials (0 and -inf for a row
+    that sees nothing).  Rows of no sequence are left as ``o`` held them.
+    ``workspace``: a decode workspace whose error word receives
+    WS_ERR_TRUNCATED when a page table is longer than ``max_pages``."""
+    return _host.chunk_attn(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+                            max_pages, layout, int(causal), window, float(soft_cap), slopes,
+                            prefix_len, o, int(return_lse), workspace)
+
+
+def attn_weights(q, lse, q_indptr, weights, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+                 max_pages: int, layout: int, causal: bool = True, window: int = 0,
+                 soft_cap: float = 0.0, slopes=None, prefix_len=None, start=None,
+                 workspace=None):
+    """Adds up the attention weight that each cached token receives from the
+    rows of q (aoakv_attn_weights): weights [max_pages, Hkv, S] fp32, by physical
+    page, gains the sum over a sequence's rows and a kv head's query heads of
+    exp(score - lse), with lse as ``chunk_attn`` returned it and its options.
+    Positions from start[b] on (int32 [B]; None: the rows' own tokens) start
+    from 0.  For the last rows of a prompt alone pass those of q and lse."""
+    _host.attn_weights(q, lse, q_indptr, weights, kv_data, kv_indptr, kv_indices,
+                       kv_last_page_len, max_pages, layout, int(causal), window, float(soft_cap),
+                       slopes, prefix_len, start, workspace)
+
+
+def keep_tokens(weights, kv_indptr, kv_indices, kv_last_page_len, keep: int, kept,
+                max_pages: int, sink: int = 0, recent: int = 0, workspace=None):
+    """Which ``keep`` tokens each kv head keeps (aoakv_keep_tokens): the first
+    ``sink``, the last ``recent`` and those of the others with the largest weight
+    (ties to the earlier token), in ascending order into kept [B, Hkv, >= keep]
+    int32.  A shorter sequence keeps every token; the rest of its row is left."""
+    _host.keep_tokens(weights, kv_indptr, kv_indices, kv_last_page_len, keep, kept, max_pages,
+                      sink, recent, workspace)
+
+
+def compact_kv_cache(kept, keep: int, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+                     new_indptr, new_indices, metadata_data, metadata_indptr, metadata_indices,
+                     v_log_norm, v_mean, max_pages: int, layout: int, weights=None,
+                     workspace=None):
+    """Packs the cache down to the kept tokens (aoakv_compact_kv_cache): slot i
+    of a head's new pages gets its token kept[b, h, i], with the page statistics
+    of a bulk append and, if given, the ``weights`` moved along.  ``new_indptr``
+    and ``new_indices`` None: in place, into the first pages of the old lists;
+    else into pages that no sequence of the call holds.  The metadata tables are
+    the new lists'."""
+    _host.compact_kv_cache(kept, keep, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+                           new_indptr, new_indices, metadata_data, metadata_indptr,
+                           metadata_indices, v_log_norm, v_mean, max_pages, layout, weights,
+                           workspace)

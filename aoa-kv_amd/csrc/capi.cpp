@@ -1028,4 +1028,205 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
                     "prefill_with_paged_kv_cache");
 }
 
+// The arguments that chunk_attn and attn_weights share.
+static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indptr,
+                      uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
+                      const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                      const int32_t* prefix_len, const float* slopes, uint32_t batch_size,
+                      uint32_t max_pages, uint32_t num_qo_heads, uint32_t num_kv_heads,
+                      uint32_t head_dim, uint32_t page_size, uint32_t layout, uint32_t causal,
+                      uint32_t window, float soft_cap, const void* workspace,
+                      size_t workspace_bytes, size_t need, uint32_t* error_word, const char* fn) {
+  if (int e = check_shape(head_dim, page_size, layout, num_qo_heads)) return e;
+  REQUIRE(num_kv_heads != 0u && num_qo_heads % num_kv_heads == 0u,
+          "%s: num_qo_heads %u not a multiple of num_kv_heads %u", fn, num_qo_heads, num_kv_heads);
+  REQUIRE(q_indptr && kv_data && kv_indptr && kv_indices && kv_last_page_len,
+          "%s: null pointer argument", fn);
+  REQUIRE(num_q_tokens == 0u || q, "%s: null pointer argument", fn);
+  REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
+  REQUIRE(num_q_tokens < (1u << 31), "%s: too many rows", fn);
+  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size < (1ull << 31),
+          "%s: max_pages %u out of range", fn, max_pages);
+  REQUIRE(window < (1u << 31), "%s: window %u out of range", fn, window);
+  REQUIRE(soft_cap >= 0.f && std::isfinite(soft_cap), "%s: soft_cap %g must be >= 0", fn,
+          (double)soft_cap);
+  REQUIRE(need == 0u || workspace, "%s: null workspace", fn);
+  REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16u == 0u,
+          "%s: workspace not aligned to 16 bytes", fn);
+  REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes < %zu needed", fn, workspace_bytes,
+          need);
+  a.q = static_cast<const aoakv::f16*>(q);
+  a.q_indptr = q_indptr;
+  a.kv = static_cast<const aoakv::f16*>(kv_data);
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.prefix_len = prefix_len;
+  a.slopes = slopes;
+  a.T = num_q_tokens;
+  a.B = batch_size;
+  a.max_pages = max_pages;
+  a.Hq = num_qo_heads;
+  a.H = num_kv_heads;
+  a.S = page_size;
+  a.causal = causal ? 1u : 0u;
+  a.window = window;
+  a.sm_scale = 1.0f / std::sqrt((float)head_dim);
+  a.soft_cap = soft_cap;
+  a.g = aoakv::make_geom(layout, num_kv_heads, page_size, head_dim);
+  a.error = error_word;
+  return AOAKV_OK;
+}
+
+size_t aoakv_chunk_attn_workspace_size(uint32_t num_qo_heads, uint32_t head_dim) {
+  (void)num_qo_heads;
+  (void)head_dim;
+  return 0;
+}
+
+int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
+                     uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
+                     const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                     const int32_t* prefix_len, const float* slopes, uint32_t batch_size,
+                     uint32_t max_pages, uint32_t num_qo_heads, uint32_t num_kv_heads,
+                     uint32_t head_dim, uint32_t page_size, uint32_t layout, uint32_t causal,
+                     uint32_t window, float soft_cap, void* workspace, size_t workspace_bytes,
+                     uint32_t* error_word, void* stream) {
+  aoakv::ChunkArgs a{};
+  if (int e = fill_chunk(a, q, q_indptr, num_q_tokens, kv_data, kv_indptr, kv_indices,
+                         kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
+                         num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
+                         soft_cap, workspace, workspace_bytes,
+                         aoakv_chunk_attn_workspace_size(num_qo_heads, head_dim), error_word,
+                         "chunk_attn"))
+    return e;
+  if (num_q_tokens == 0u) return ok();
+  REQUIRE(o, "chunk_attn: null pointer argument");
+  a.o = static_cast<aoakv::f16*>(o);
+  a.lse = lse;
+  return hip_status(aoakv::launch_chunk_attn(a, head_dim, static_cast<hipStream_t>(stream)),
+                    "chunk_attn");
+}
+
+size_t aoakv_attn_weights_workspace_size(uint32_t num_kv_heads) {
+  (void)num_kv_heads;
+  return 0;
+}
+
+int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
+                       const int32_t* start, float* weights, uint32_t num_q_tokens,
+                       const void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,
+                       const int32_t* kv_last_page_len, const int32_t* prefix_len,
+                       const float* slopes, uint32_t batch_size, uint32_t max_pages,
+                       uint32_t num_qo_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                       uint32_t page_size, uint32_t layout, uint32_t causal, uint32_t window,
+                       float soft_cap, void* workspace, size_t workspace_bytes,
+                       uint32_t* error_word, void* stream) {
+  aoakv::ChunkArgs a{};
+  if (int e = fill_chunk(a, q, q_indptr, num_q_tokens, kv_data, kv_indptr, kv_indices,
+                         kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
+                         num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
+                         soft_cap, workspace, workspace_bytes,
+                         aoakv_attn_weights_workspace_size(num_kv_heads), error_word,
+                         "attn_weights"))
+    return e;
+  REQUIRE((num_q_tokens == 0u || lse) && weights, "attn_weights: null pointer argument");
+  a.lse = const_cast<float*>(lse);  // (only read by the weights)
+  a.weights = weights;
+  a.start = start;
+  return hip_status(aoakv::launch_attn_weights(a, head_dim, static_cast<hipStream_t>(stream)),
+                    "attn_weights");
+}
+
+// The sizes of an eviction call.
+static int check_evict(uint32_t keep, uint32_t kept_stride, uint32_t batch_size,
+                       uint32_t max_pages, uint32_t num_heads, uint32_t page_size,
+                       const char* fn) {
+  REQUIRE(page_size >= 1u && page_size <= aoakv::kMaxPageSize, "%s: page_size %u unsupported (1..%u)",
+          fn, page_size, aoakv::kMaxPageSize);
+  REQUIRE(num_heads >= 1u && num_heads <= 256u, "%s: num_heads %u out of range [1, 256]", fn,
+          num_heads);
+  REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
+  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size < (1ull << 31),
+          "%s: max_pages %u out of range", fn, max_pages);
+  REQUIRE(keep >= 1u && keep <= kept_stride, "%s: keep %u not in [1, kept_stride %u]", fn, keep,
+          kept_stride);
+  return AOAKV_OK;
+}
+
+int aoakv_keep_tokens(const float* weights, const int32_t* kv_indptr, const int32_t* kv_indices,
+                      const int32_t* kv_last_page_len, int32_t* kept, uint32_t kept_stride,
+                      uint32_t keep, uint32_t sink, uint32_t recent, uint32_t batch_size,
+                      uint32_t max_pages, uint32_t num_kv_heads, uint32_t page_size,
+                      uint32_t* error_word, void* stream) {
+  if (int e = check_evict(keep, kept_stride, batch_size, max_pages, num_kv_heads, page_size,
+                          "keep_tokens"))
+    return e;
+  REQUIRE(weights && kv_indptr && kv_indices && kv_last_page_len && kept,
+          "keep_tokens: null pointer argument");
+  REQUIRE((uint64_t)sink + recent <= keep, "keep_tokens: sink %u + recent %u > keep %u", sink,
+          recent, keep);
+  aoakv::KeepArgs a{};
+  a.weights = weights;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.kept = kept;
+  a.stride = kept_stride;
+  a.keep = keep;
+  a.sink = sink;
+  a.recent = recent;
+  a.max_pages = max_pages;
+  a.H = num_kv_heads;
+  a.S = page_size;
+  a.error = error_word;
+  return hip_status(aoakv::launch_keep(a, batch_size, static_cast<hipStream_t>(stream)),
+                    "keep_tokens");
+}
+
+int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t keep,
+                           void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,
+                           const int32_t* kv_last_page_len, const int32_t* new_indptr,
+                           const int32_t* new_indices, void* metadata_data,
+                           const int32_t* metadata_indptr, const int32_t* metadata_indices,
+                           void* v_log_norm, void* v_mean, float* weights, uint32_t batch_size,
+                           uint32_t max_pages, uint32_t num_heads, uint32_t head_dim,
+                           uint32_t page_size, uint32_t layout, uint32_t* error_word,
+                           void* stream) {
+  if (int e = check_shape(head_dim, page_size, layout, num_heads)) return e;
+  if (int e = check_evict(keep, kept_stride, batch_size, max_pages, num_heads, page_size,
+                          "compact_kv_cache"))
+    return e;
+  REQUIRE(kept && kv_data && kv_indptr && kv_indices && kv_last_page_len && metadata_data &&
+              metadata_indptr && metadata_indices && v_log_norm && v_mean,
+          "compact_kv_cache: null pointer argument");
+  REQUIRE((new_indptr == nullptr) == (new_indices == nullptr),
+          "compact_kv_cache: new_indptr and new_indices are both given or both NULL");
+  aoakv::CompactArgs a{};
+  a.kept = kept;
+  a.stride = kept_stride;
+  a.keep = keep;
+  a.kv = static_cast<aoakv::f16*>(kv_data);
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.in_place = new_indptr == nullptr ? 1u : 0u;
+  a.new_indptr = a.in_place ? kv_indptr : new_indptr;
+  a.new_indices = a.in_place ? kv_indices : new_indices;
+  a.meta = static_cast<aoakv::f16*>(metadata_data);
+  a.meta_indptr = metadata_indptr;
+  a.meta_indices = metadata_indices;
+  a.v_log_norm = static_cast<aoakv::f16*>(v_log_norm);
+  a.v_mean = static_cast<aoakv::f16*>(v_mean);
+  a.weights = weights;
+  a.max_pages = max_pages;
+  a.H = num_heads;
+  a.S = page_size;
+  a.g = aoakv::make_geom(layout, num_heads, page_size, head_dim);
+  a.error = error_word;
+  return hip_status(
+      aoakv::launch_compact(a, batch_size, head_dim, static_cast<hipStream_t>(stream)),
+      "compact_kv_cache");
+}
+
 }  // extern "C"

@@ -35,7 +35,9 @@ struct PyErr {};
   X(append_kv_cache_prefill) X(append_kv_cache_decode) X(rope_append_kv_cache_decode)  \
   X(rope_append_kv_cache_prefill) X(rms_norm_forward) X(estimate_attn_score)           \
   X(topk_filtering) X(decode_sparse_attn) X(sparse_decode_layer)                       \
-  X(prefill_workspace_size) X(prefill_with_workspace) X(last_error)
+  X(prefill_workspace_size) X(prefill_with_workspace) X(chunk_attn_workspace_size)     \
+  X(chunk_attn) X(attn_weights_workspace_size) X(attn_weights) X(keep_tokens)          \
+  X(compact_kv_cache) X(last_error)
 
 struct Lib {
 #define X(n) decltype(&aoakv_##n) n = nullptr;
@@ -451,6 +453,217 @@ void rms_norm_forward(PyObject* const* a) {
   });
 }
 
+// ---- ragged chunks and eviction
+// A tensor as `need` takes it, on the device that the call runs on.
+const Tensor& here(PyObject* o, const char* name, at::ScalarType dtype) {
+  const Tensor& t = need(o, name, dtype);
+  if (t.get_device() != c10::hip::current_device())
+    raise(PyExc_ValueError, std::string(name) + " must be on the current device");
+  return t;
+}
+const Tensor* here_or_null(PyObject* o, const char* name, at::ScalarType dtype) {
+  return o == Py_None ? nullptr : &here(o, name, dtype);
+}
+template <class T>
+T* data_or_null(const Tensor* t) {
+  return t == nullptr ? nullptr : static_cast<T*>(t->data_ptr());
+}
+// a size below 2^31, compared whole
+uint32_t size31(PyObject* o, const char* name) {
+  return u32_at_most(o, 0x7FFFFFFF, (std::string(name) + " must be in [0, 2^31)").c_str());
+}
+// the error word of a decode workspace, or none
+uint32_t* error_word(PyObject* o) {
+  if (o == Py_None) return nullptr;
+  const Tensor& ws = here(o, "workspace", at::kByte);
+  if (ws.numel() < 12) raise(PyExc_ValueError, "workspace too small to hold the error word");
+  return static_cast<uint32_t*>(ptr(ws)) + AOAKV_WS_ERR_WORD;
+}
+// kv_indptr, kv_indices, kv_last_page_len of a batch of B sequences
+struct PageTable {
+  const int32_t *indptr, *indices, *last;
+  int64_t B;
+};
+PageTable page_table(PyObject* const* t) {
+  const Tensor &ip = here(t[0], "kv_indptr", at::kInt), &ix = here(t[1], "kv_indices", at::kInt),
+               &last = here(t[2], "kv_last_page_len", at::kInt);
+  const int64_t B = last.numel();
+  if (ip.numel() != B + 1)
+    raise(PyExc_ValueError, "indptr / last_page_len sizes do not match the batch");
+  return PageTable{static_cast<const int32_t*>(ptr(ip)), static_cast<const int32_t*>(ptr(ix)),
+                   static_cast<const int32_t*>(ptr(last)), B};
+}
+const int32_t* per_sequence(PyObject* o, const char* name, int64_t n) {
+  const Tensor* t = here_or_null(o, name, at::kInt);
+  if (t != nullptr && t->numel() != n)
+    raise(PyExc_ValueError, std::string(name) + " does not match the batch");
+  return data_or_null<const int32_t>(t);
+}
+const Tensor& paged_weights(PyObject* o, int64_t H, int64_t S) {
+  const Tensor& w = here(o, "weights", at::kFloat);
+  if (w.dim() != 3 || (H >= 0 && (w.size(1) != H || w.size(2) != S)))
+    raise(PyExc_ValueError, "weights must be [max_pages, num_kv_heads, page_size], got " +
+                                shape_str(w));
+  return w;
+}
+// scratch memory of a call, from torch's pool on this stream
+Tensor scratch(size_t bytes, const Tensor& like) {
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+// What chunk_attn and attn_weights have alike: q, the cache, the tables and
+// (causal, window, soft_cap, slopes, prefix_len) from t[5].
+struct Chunks {
+  const Tensor &q, &kv;
+  Dims d;
+  PageTable t;
+  const int32_t *q_indptr, *prefix;
+  const float* slopes;
+  uint32_t T, Hq, max_pages, causal, window;
+  float cap;
+};
+// q, q_indptr; t: kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages,
+// layout, causal, window, soft_cap, slopes, prefix_len
+Chunks chunk_args(PyObject* q_, PyObject* q_indptr, PyObject* const* t) {
+  const Tensor &q = here(q_, "q", at::kHalf), &kv = here(t[0], "kv_data", at::kHalf);
+  const Dims d = cache_dims(kv, t[5]);
+  if (q.dim() != 3 || q.size(2) != d.D)
+    raise(PyExc_ValueError, "q must be [T, Hq, " + std::to_string(d.D) + "], got " + shape_str(q));
+  const PageTable table = page_table(t + 1);
+  const Tensor& ip = here(q_indptr, "q_indptr", at::kInt);
+  if (ip.numel() != table.B + 1)
+    raise(PyExc_ValueError, "q_indptr does not match the batch");
+  const Tensor* slopes = here_or_null(t[9], "slopes", at::kFloat);
+  if (slopes != nullptr && slopes->numel() != q.size(1))
+    raise(PyExc_ValueError, "slopes must be [" + std::to_string(q.size(1)) + "]");
+  if (q.size(0) > 0x7FFFFFFF) raise(PyExc_ValueError, "q has too many rows");
+  return Chunks{q, kv, d, table, static_cast<const int32_t*>(ptr(ip)),
+                per_sequence(t[10], "prefix_len", table.B), data_or_null<const float>(slopes),
+                (uint32_t)q.size(0), (uint32_t)q.size(1), size31(t[4], "max_pages"),
+                u32(t[6]), size31(t[7], "window"), f32(t[8])};
+}
+
+// (q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages,
+//  layout, causal, window, soft_cap, slopes, prefix_len, o or None, return_lse,
+//  workspace) -> o or (o, lse)
+PyObject* chunk_attn(PyObject* const* a) {
+  const Chunks c = chunk_args(a[0], a[1], a + 2);
+  const Tensor* given = here_or_null(a[13], "o", at::kHalf);
+  if (given != nullptr && given->sizes() != c.q.sizes())
+    raise(PyExc_ValueError, "o must have q's shape");
+  const bool want = u32(a[14]) != 0u;
+  uint32_t* err = error_word(a[15]);
+  const Tensor o = given != nullptr ? *given : at::empty_like(c.q);
+  Tensor lse;
+  if (want) lse = at::empty({c.q.size(0), c.q.size(1)}, c.q.options().dtype(at::kFloat));
+  const size_t n = g_lib.chunk_attn_workspace_size(c.Hq, c.d.D);
+  const Tensor ws = scratch(n, c.q);
+  void* s = stream();
+  call("aoakv_chunk_attn", [&] {
+    return g_lib.chunk_attn(ptr(c.q), ptr(o), want ? static_cast<float*>(ptr(lse)) : nullptr,
+                            c.q_indptr, c.T, ptr(c.kv), c.t.indptr, c.t.indices, c.t.last,
+                            c.prefix, c.slopes, (uint32_t)c.t.B, c.max_pages, c.Hq, c.d.H, c.d.D,
+                            c.d.S, c.d.layout, c.causal, c.window, c.cap, ptr(ws), n, err, s);
+  });
+  if (!want) return THPVariable_Wrap(o);
+  PyObject *x = THPVariable_Wrap(o), *y = THPVariable_Wrap(lse);
+  PyObject* both = x != nullptr && y != nullptr ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return both;
+}
+
+// (q, lse, q_indptr, weights, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+//  max_pages, layout, causal, window, soft_cap, slopes, prefix_len, start,
+//  workspace)
+void attn_weights(PyObject* const* a) {
+  const Chunks c = chunk_args(a[0], a[2], a + 4);
+  const Tensor &lse = here(a[1], "lse", at::kFloat), &w = paged_weights(a[3], c.d.H, c.d.S);
+  if (lse.dim() != 2 || lse.size(0) != c.q.size(0) || lse.size(1) != c.q.size(1))
+    raise(PyExc_ValueError, "lse must be [T, Hq], got " + shape_str(lse));
+  if (w.size(0) != c.kv.size(0))
+    raise(PyExc_ValueError, "weights and kv_data have different page counts");
+  const int32_t* start = per_sequence(a[15], "start", c.t.B);
+  uint32_t* err = error_word(a[16]);
+  const size_t n = g_lib.attn_weights_workspace_size(c.d.H);
+  const Tensor ws = scratch(n, c.q);
+  void* s = stream();
+  call("aoakv_attn_weights", [&] {
+    return g_lib.attn_weights(ptr(c.q), static_cast<const float*>(ptr(lse)), c.q_indptr, start,
+                              static_cast<float*>(ptr(w)), c.T, ptr(c.kv), c.t.indptr,
+                              c.t.indices, c.t.last, c.prefix, c.slopes, (uint32_t)c.t.B,
+                              c.max_pages, c.Hq, c.d.H, c.d.D, c.d.S, c.d.layout, c.causal,
+                              c.window, c.cap, ptr(ws), n, err, s);
+  });
+}
+
+const Tensor& kept_rows(PyObject* o, int64_t B, int64_t H) {
+  const Tensor& k = here(o, "kept", at::kInt);
+  if (k.dim() != 3 || k.size(0) != B || k.size(1) != H)
+    raise(PyExc_ValueError, "kept must be [" + std::to_string(B) + ", " + std::to_string(H) +
+                                ", >= keep], got " + shape_str(k));
+  return k;
+}
+
+// (weights, kv_indptr, kv_indices, kv_last_page_len, keep, kept, max_pages,
+//  sink, recent, workspace)
+void keep_tokens(PyObject* const* a) {
+  const Tensor& w = paged_weights(a[0], -1, 0);
+  const PageTable t = page_table(a + 1);
+  const Tensor& kept = kept_rows(a[5], t.B, w.size(1));
+  const uint32_t keep = size31(a[4], "keep"), pages = size31(a[6], "max_pages"),
+                 sink = size31(a[7], "sink"), recent = size31(a[8], "recent");
+  uint32_t* err = error_word(a[9]);
+  void* s = stream();
+  call("aoakv_keep_tokens", [&] {
+    return g_lib.keep_tokens(static_cast<const float*>(ptr(w)), t.indptr, t.indices, t.last,
+                             static_cast<int32_t*>(ptr(kept)), (uint32_t)kept.size(2), keep, sink,
+                             recent, (uint32_t)t.B, pages, (uint32_t)w.size(1),
+                             (uint32_t)w.size(2), err, s);
+  });
+}
+
+// (kept, keep, kv_data, kv_indptr, kv_indices, kv_last_page_len, new_indptr,
+//  new_indices, metadata_data, metadata_indptr, metadata_indices, v_log_norm,
+//  v_mean, max_pages, layout, weights, workspace)
+void compact_kv_cache(PyObject* const* a) {
+  const Tensor &kv = here(a[2], "kv_data", at::kHalf), &meta = here(a[8], "metadata_data", at::kHalf),
+               &log_norm = here(a[11], "v_log_norm", at::kHalf),
+               &mean = here(a[12], "v_mean", at::kHalf);
+  const Dims d = cache_dims(kv, a[14]), md = cache_dims(meta, a[14]);
+  if (md.S != d.S || md.H != d.H || md.D != d.D)
+    raise(PyExc_ValueError, "metadata_data's pages must be as kv_data's");
+  const PageTable t = page_table(a + 3);
+  const Tensor& kept = kept_rows(a[0], t.B, d.H);
+  if (log_norm.numel() != kv.size(0) * d.H || mean.numel() != kv.size(0) * d.H * d.D)
+    raise(PyExc_ValueError, "v_log_norm must be [max_pages, H] and v_mean [max_pages, H, D]");
+  if ((a[6] == Py_None) != (a[7] == Py_None))
+    raise(PyExc_ValueError, "new_indptr and new_indices are both given or both None");
+  const int32_t* new_ip = per_sequence(a[6], "new_indptr", t.B + 1);
+  const Tensor* new_ix = here_or_null(a[7], "new_indices", at::kInt);
+  const int32_t* mip = static_cast<const int32_t*>(ptr(here(a[9], "metadata_indptr", at::kInt)));
+  if (THPVariable_Unpack(a[9]).numel() != t.B + 1)
+    raise(PyExc_ValueError, "metadata_indptr does not match the batch");
+  const int32_t* mix = static_cast<const int32_t*>(ptr(here(a[10], "metadata_indices", at::kInt)));
+  float* w = nullptr;
+  if (a[15] != Py_None) {
+    const Tensor& x = paged_weights(a[15], d.H, d.S);
+    if (x.size(0) != kv.size(0))
+      raise(PyExc_ValueError, "weights and kv_data have different page counts");
+    w = static_cast<float*>(ptr(x));
+  }
+  const uint32_t keep = size31(a[1], "keep"), pages = size31(a[13], "max_pages");
+  uint32_t* err = error_word(a[16]);
+  void* s = stream();
+  call("aoakv_compact_kv_cache", [&] {
+    return g_lib.compact_kv_cache(static_cast<const int32_t*>(ptr(kept)), (uint32_t)kept.size(2),
+                                  keep, ptr(kv), t.indptr, t.indices, t.last, new_ip,
+                                  data_or_null<const int32_t>(new_ix), ptr(meta), mip, mix,
+                                  ptr(log_norm), ptr(mean), w, (uint32_t)t.B, pages, d.H, d.D,
+                                  d.S, d.layout, err, s);
+  });
+}
+
 // No C++ exception leaves a call: torch's become RuntimeError.
 template <auto F, Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -510,6 +723,10 @@ PyMethodDef g_methods[] = {
     ENTRY(sparse_decode_layer, 18),
     ENTRY(prefill_with_paged_kv_cache, 8),
     ENTRY(rms_norm_forward, 4),
+    ENTRY(chunk_attn, 16),
+    ENTRY(attn_weights, 17),
+    ENTRY(keep_tokens, 10),
+    ENTRY(compact_kv_cache, 17),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

@@ -274,4 +274,64 @@ hipError_t launch_gen_estimate(const EstimateArgs& a, uint32_t batch, uint32_t m
                                uint32_t head_dim, hipStream_t s);
 hipError_t launch_gen_prefill(const PrefillArgs& a, uint32_t head_dim, hipStream_t s);
 
+// Attention of a ragged batch of chunks over the paged cache and the weights
+// its keys received (chunk.hip).  Sequence b's queries are the rows q_indptr[b]
+// .. q_indptr[b + 1] of q, the last of its cached tokens.
+struct ChunkArgs {
+  const f16* q;   // [T, Hq, D]
+  f16* o;         // [T, Hq, D]
+  float* lse;     // [T, Hq], or nullptr (attention); read by the weights
+  float* weights; // [pages, H, S] (weights only)
+  const int32_t* start;  // [B] first position whose weight starts from 0, or nullptr
+  const int32_t* q_indptr;
+  const f16* kv;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  const int32_t* prefix_len;  // [B] or nullptr
+  const float* slopes;        // [Hq] or nullptr
+  uint32_t T, B, max_pages, Hq, H, S;
+  uint32_t causal, window;    // window 0: none
+  float sm_scale, soft_cap;   // soft_cap 0: none
+  PageGeom g;
+  uint32_t* error;            // receives kErrTruncated, or nullptr
+};
+hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
+hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
+
+// Eviction (evict.hip): the tokens a kv head keeps, and the cache packed down
+// to them.
+struct KeepArgs {
+  const float* weights;  // [pages, H, S]
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  int32_t* kept;         // [B, H, stride]
+  uint32_t stride, keep, sink, recent, max_pages, H, S;
+  uint32_t* error;
+};
+hipError_t launch_keep(const KeepArgs& a, uint32_t batch, hipStream_t s);
+
+struct CompactArgs {
+  const int32_t* kept;   // [B, H, stride]
+  uint32_t stride, keep;
+  f16* kv;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  const int32_t* new_indptr;   // the old table in place
+  const int32_t* new_indices;
+  uint32_t in_place;
+  f16* meta;
+  const int32_t* meta_indptr;
+  const int32_t* meta_indices;
+  f16* v_log_norm;
+  f16* v_mean;
+  float* weights;        // or nullptr
+  uint32_t max_pages, H, S;
+  PageGeom g;
+  uint32_t* error;
+};
+hipError_t launch_compact(const CompactArgs& a, uint32_t batch, uint32_t head_dim, hipStream_t s);
+
 }  // namespace aoakv

@@ -19,7 +19,9 @@
  *
  * plus fused entry points: aoakv_sparse_decode_layer (estimate + top-k +
  * sparse decode for one layer), aoakv_estimate_topk, and
- * aoakv_rope_append_kv_cache_decode (RoPE + decode append).
+ * aoakv_rope_append_kv_cache_decode (RoPE + decode append); and, beyond the
+ * reference, aoakv_chunk_attn (attention of a ragged batch of chunks),
+ * aoakv_attn_weights, aoakv_keep_tokens and aoakv_compact_kv_cache (eviction).
  *
  * Conventions
  *   - All tensor arguments are device pointers (plain pointers, no torch
@@ -462,6 +464,109 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
                                  uint32_t num_qo_heads, uint32_t num_kv_heads,
                                  uint32_t head_dim, uint32_t page_size, uint32_t layout,
                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of new tokens of EVERY sequence of a batch over the paged cache, in
+ * one call: chunks of prompts, drafted tokens to check, single tokens, mixed.
+ * No counterpart in the reference (its prefill takes one sequence and its
+ * decode one token each); the plain case is that of
+ * aoakv_prefill_with_paged_kv_cache.
+ *
+ * q, o: [num_q_tokens, num_qo_heads, head_dim] fp16; sequence b's rows are
+ * q_indptr[b] .. q_indptr[b + 1] - 1 (int32, device, ascending; none is
+ * allowed), the last of its L_b cached tokens, which the page table already
+ * counts (an empty table row: no tokens).  Rows outside q_indptr[0] ..
+ * q_indptr[B] - 1 are not touched.  Row i of n_b is at position pos = L_b - n_b
+ * + i; for the key at position j, with dot products and softmax in fp32,
+ *   t = q . k / sqrt(head_dim)
+ *   t = soft_cap * tanh(t / soft_cap)      if soft_cap > 0
+ *   t = t - slopes[h] * |pos - j|          if slopes ([num_qo_heads] fp32)
+ * counts where j <= pos (if causal) and pos - j < window (if window > 0), and
+ * for j < prefix_len[b] (int32 [B], or NULL) whatever these say: a prefix that
+ * all queries see, or the first tokens kept beside a window.
+ * o = softmax(t) v; lse (fp32 [num_q_tokens, num_qo_heads], or NULL) = log of
+ * the sum of exp(t).  A row that sees no key: o = 0, lse = -inf.  What keys and
+ * values hold where a row does not see them changes nothing, NaN and inf too.
+ *
+ * num_qo_heads is any multiple of num_kv_heads.  max_pages >= every sequence's
+ * page count: a longer table is cut to it and AOAKV_WS_ERR_TRUNCATED set in
+ * *error_word (NULL: not reported), as in aoakv_topk_filtering.  workspace:
+ * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
+ * initialisation and is free again when the call's work on `stream` is done.
+ */
+size_t aoakv_chunk_attn_workspace_size(uint32_t num_qo_heads, uint32_t head_dim);
+int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
+                     uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
+                     const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                     const int32_t* prefix_len, const float* slopes, uint32_t batch_size,
+                     uint32_t max_pages, uint32_t num_qo_heads, uint32_t num_kv_heads,
+                     uint32_t head_dim, uint32_t page_size, uint32_t layout, uint32_t causal,
+                     uint32_t window, float soft_cap, void* workspace, size_t workspace_bytes,
+                     uint32_t* error_word, void* stream);
+
+/*
+ * The attention weight that every cached token received from the chunks:
+ *   weights[page, kv head, slot] = (j < start[b] ? weights[...] : 0)
+ *                                  + sum over the sequence's rows and the kv
+ *                                    head's query heads of exp(t - lse)
+ * for the token at position j of sequence b, t and what a row sees as in
+ * aoakv_chunk_attn (same arguments), lse as it wrote it.  weights: fp32
+ * [max_pages, num_kv_heads, page_size], by PHYSICAL page as v_log_norm.
+ * start: int32 [B], or NULL: L_b - n_b, so the chunk's own tokens start from 0
+ * (their slots may hold an earlier owner's sums) and the others' sums go on.
+ * To weigh a prompt by its last rows alone, pass those rows of q and lse (and
+ * start 0).  The sum's order is fixed by the lengths: equal calls give equal
+ * bits.  A batch whose sequences share a page is not allowed.  Slots behind a
+ * sequence's last token are not touched.
+ */
+size_t aoakv_attn_weights_workspace_size(uint32_t num_kv_heads);
+int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
+                       const int32_t* start, float* weights, uint32_t num_q_tokens,
+                       const void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,
+                       const int32_t* kv_last_page_len, const int32_t* prefix_len,
+                       const float* slopes, uint32_t batch_size, uint32_t max_pages,
+                       uint32_t num_qo_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                       uint32_t page_size, uint32_t layout, uint32_t causal, uint32_t window,
+                       float soft_cap, void* workspace, size_t workspace_bytes,
+                       uint32_t* error_word, void* stream);
+
+/*
+ * The tokens that each kv head of each sequence keeps: its first `sink`, its
+ * last `recent`, and of the others those with the largest weight (ties to the
+ * lower position, NaN as the smallest), `keep` in all; every token where there
+ * are no more than `keep`.  weights as aoakv_attn_weights leaves them.
+ * kept: int32 [B, num_kv_heads, kept_stride], positions in ascending order;
+ * entries from min(keep, L_b) on are not touched.
+ * 1 <= keep <= kept_stride, sink + recent <= keep.
+ */
+int aoakv_keep_tokens(const float* weights, const int32_t* kv_indptr, const int32_t* kv_indices,
+                      const int32_t* kv_last_page_len, int32_t* kept, uint32_t kept_stride,
+                      uint32_t keep, uint32_t sink, uint32_t recent, uint32_t batch_size,
+                      uint32_t max_pages, uint32_t num_kv_heads, uint32_t page_size,
+                      uint32_t* error_word, void* stream);
+
+/*
+ * Packs every sequence's cache down to the kept tokens: slot i of a kv head's
+ * new page list gets the K, V (and weight, if weights is not NULL) of the
+ * head's token kept[b, h, i], i < min(keep, L_b), in the first ceil(min(keep,
+ * L_b) / page_size) pages of new_indptr / new_indices.  Page statistics (Kmax /
+ * Kmin, V̄, log-norm) are written for these pages as
+ * aoakv_append_kv_cache_prefill into empty pages writes them; metadata_indptr /
+ * metadata_indices list the metadata pages of the new page list.
+ * new_indptr and new_indices NULL: in place, into the first pages of the
+ * sequence's own list.  Otherwise no new page may be a page of kv_indices.
+ * kept: ascending positions, as aoakv_keep_tokens writes them (one past the
+ * sequence's end reads its last token).  The caller then shortens its table.
+ */
+int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t keep,
+                           void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,
+                           const int32_t* kv_last_page_len, const int32_t* new_indptr,
+                           const int32_t* new_indices, void* metadata_data,
+                           const int32_t* metadata_indptr, const int32_t* metadata_indices,
+                           void* v_log_norm, void* v_mean, float* weights, uint32_t batch_size,
+                           uint32_t max_pages, uint32_t num_heads, uint32_t head_dim,
+                           uint32_t page_size, uint32_t layout, uint32_t* error_word,
+                           void* stream);
 
 #ifdef __cplusplus
 }
