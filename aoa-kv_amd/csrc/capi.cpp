@@ -1044,9 +1044,11 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
           "%s: null pointer argument", fn);
   REQUIRE(num_q_tokens == 0u || q, "%s: null pointer argument", fn);
   REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
-  REQUIRE(num_q_tokens < (1u << 31), "%s: too many rows", fn);
-  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size < (1ull << 31),
-          "%s: max_pages %u out of range", fn, max_pages);
+  REQUIRE((uint64_t)num_q_tokens * (num_qo_heads / num_kv_heads) < (1ull << 30),
+          "%s: too many rows (%u x %u query heads per kv head)", fn, num_q_tokens,
+          num_qo_heads / num_kv_heads);
+  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size <= aoakv::kMaxChunkTokens,
+          "%s: max_pages %u of %u tokens not in [1, 2^27 tokens]", fn, max_pages, page_size);
   REQUIRE(window < (1u << 31), "%s: window %u out of range", fn, window);
   REQUIRE(soft_cap >= 0.f && std::isfinite(soft_cap), "%s: soft_cap %g must be >= 0", fn,
           (double)soft_cap);
@@ -1070,7 +1072,7 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   a.H = num_kv_heads;
   a.S = page_size;
   a.causal = causal ? 1u : 0u;
-  a.window = window;
+  a.window = window < aoakv::kMaxChunkTokens ? window : 0u;  // (no two positions are further apart)
   a.sm_scale = 1.0f / std::sqrt((float)head_dim);
   a.soft_cap = soft_cap;
   a.g = aoakv::make_geom(layout, num_kv_heads, page_size, head_dim);
@@ -1078,10 +1080,10 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   return AOAKV_OK;
 }
 
-size_t aoakv_chunk_attn_workspace_size(uint32_t num_qo_heads, uint32_t head_dim) {
-  (void)num_qo_heads;
-  (void)head_dim;
-  return 0;
+size_t aoakv_chunk_attn_workspace_size(uint32_t head_dim) {
+  return head_dim == 64u || head_dim == 128u || head_dim == 256u
+             ? aoakv::chunk_attn_workspace(head_dim)
+             : 0u;
 }
 
 int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
@@ -1097,21 +1099,19 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
                          kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
                          num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
                          soft_cap, workspace, workspace_bytes,
-                         aoakv_chunk_attn_workspace_size(num_qo_heads, head_dim), error_word,
+                         aoakv_chunk_attn_workspace_size(head_dim), error_word,
                          "chunk_attn"))
     return e;
   if (num_q_tokens == 0u) return ok();
   REQUIRE(o, "chunk_attn: null pointer argument");
   a.o = static_cast<aoakv::f16*>(o);
   a.lse = lse;
+  a.parts = static_cast<float*>(workspace);
   return hip_status(aoakv::launch_chunk_attn(a, head_dim, static_cast<hipStream_t>(stream)),
                     "chunk_attn");
 }
 
-size_t aoakv_attn_weights_workspace_size(uint32_t num_kv_heads) {
-  (void)num_kv_heads;
-  return 0;
-}
+size_t aoakv_attn_weights_workspace_size(void) { return aoakv::attn_weights_workspace(); }
 
 int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
                        const int32_t* start, float* weights, uint32_t num_q_tokens,
@@ -1127,13 +1127,14 @@ int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
                          kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
                          num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
                          soft_cap, workspace, workspace_bytes,
-                         aoakv_attn_weights_workspace_size(num_kv_heads), error_word,
+                         aoakv_attn_weights_workspace_size(), error_word,
                          "attn_weights"))
     return e;
   REQUIRE((num_q_tokens == 0u || lse) && weights, "attn_weights: null pointer argument");
   a.lse = const_cast<float*>(lse);  // (only read by the weights)
   a.weights = weights;
   a.start = start;
+  a.parts = static_cast<float*>(workspace);
   return hip_status(aoakv::launch_attn_weights(a, head_dim, static_cast<hipStream_t>(stream)),
                     "attn_weights");
 }
@@ -1147,8 +1148,8 @@ static int check_evict(uint32_t keep, uint32_t kept_stride, uint32_t batch_size,
   REQUIRE(num_heads >= 1u && num_heads <= 256u, "%s: num_heads %u out of range [1, 256]", fn,
           num_heads);
   REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
-  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size < (1ull << 31),
-          "%s: max_pages %u out of range", fn, max_pages);
+  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size <= aoakv::kMaxChunkTokens,
+          "%s: max_pages %u of %u tokens not in [1, 2^27 tokens]", fn, max_pages, page_size);
   REQUIRE(keep >= 1u && keep <= kept_stride, "%s: keep %u not in [1, kept_stride %u]", fn, keep,
           kept_stride);
   return AOAKV_OK;

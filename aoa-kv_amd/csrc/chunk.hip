@@ -9,26 +9,51 @@
 // prefix_len[b] whatever these say.  lse = log sum_j exp(t), o = sum_j exp(t -
 // lse) v_j; a query that sees no key has o = 0 and lse = -inf.  The weight of
 // key j in a kv head is the sum of exp(t - lse) over the queries of its group.
+//
+// Rows.  A kv head's queries of one sequence are packed token by token, the
+// group's heads of a token side by side: row r is token r / G, head r % G.  A
+// tile of K/V in LDS then serves the whole group, and a few tokens fill a tile
+// of rows better.
+//
+// Work.  An item is 128 rows (attention) or 128 keys (weights) of one kv head
+// and sequence, and walks tiles of 64 keys (or rows) that any of its rows sees
+// (or that see any of its keys).  Lengths are known on the device alone, so
+// every workgroup adds up the tiles of all items (kItemUnits more per item, for
+// its start and end) and takes an equal, contiguous share of them, whatever
+// items that cuts: a long sequence beside many short ones, few rows over a long
+// context and a long prompt all end at the same time.  An item that lies in one
+// share is finished there; the parts of one that does not go to the workspace,
+// two slots per workgroup (the part that its share begins with, and the one it
+// ends with), and a second launch joins them in order.  Nothing depends on
+// timing: equal calls give equal bits.
 #include "kernels.hpp"
+#include "mfma_tile.hpp"
 
 namespace aoakv {
 namespace {
 
 constexpr uint32_t kChThreads = 256;
+constexpr int32_t kChRows = 128;  // rows (attention) or keys (weights) of an item
+constexpr int32_t kChTile = 64;   // keys (attention) or rows (weights) of a tile
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kItemUnits = 1u;
 
-// What the device tables say of sequence b, held to the sizes of the call.
+// What the device tables say of a sequence, held to the sizes of the call.
 struct Seq {
-  int32_t q0, n, L, off, prefix;  // first row, new tokens, cached tokens, L - n
+  int32_t q0, n, L, off, prefix;  // first row of q, new tokens, cached tokens, L - n
   uint32_t page0;                 // first entry of kv_indices
 };
 __device__ inline Seq load_seq(const ChunkArgs& a, uint32_t b) {
   Seq s;
   const int32_t T = (int32_t)a.T;
-  s.q0 = min(max(a.q_indptr[b], 0), T);
-  s.n = max(min(a.q_indptr[b + 1], T) - s.q0, 0);
-  const int32_t p0 = a.kv_indptr[b];
-  int32_t P = max(a.kv_indptr[b + 1] - p0, 0);
-  int32_t last = min(max(a.kv_last_page_len[b], 1), (int32_t)a.S);
+  const int32_t r0 = a.q_indptr[b], r1 = a.q_indptr[b + 1], p0 = a.kv_indptr[b],
+                p1 = a.kv_indptr[b + 1];
+  int32_t last = a.kv_last_page_len[b];
+  s.prefix = a.prefix_len != nullptr ? a.prefix_len[b] : 0;
+  s.q0 = min(max(r0, 0), T);
+  s.n = max(min(r1, T) - s.q0, 0);
+  last = min(max(last, 1), (int32_t)a.S);
+  int32_t P = max(p1 - p0, 0);
   if (P > (int32_t)a.max_pages) {
     flag_error(a.error, kErrTruncated);
     P = (int32_t)a.max_pages;
@@ -37,143 +62,1009 @@ __device__ inline Seq load_seq(const ChunkArgs& a, uint32_t b) {
   s.page0 = (uint32_t)p0;
   s.L = P > 0 ? (P - 1) * (int32_t)a.S + last : 0;
   s.off = s.L - s.n;
-  s.prefix = a.prefix_len != nullptr ? a.prefix_len[b] : 0;
+  s.prefix = min(max(s.prefix, 0), s.L);
   return s;
 }
 
-__device__ inline bool sees(const ChunkArgs& a, const Seq& s, int32_t pos, int32_t j) {
-  return j < s.L && (j < s.prefix || ((!a.causal || j <= pos) &&
-                                      (a.window == 0u || pos - j < (int32_t)a.window)));
-}
+// An item's tiles: tile i of its list is tile i < cut ? i : i - cut + first.
+struct Item {
+  int32_t cut, first, count;
+  __device__ int32_t tile(int32_t i) const { return i < cut ? i : i - cut + first; }
+};
 
-__device__ inline float score(const ChunkArgs& a, float dot, uint32_t h, int32_t pos, int32_t j) {
-  float t = dot * a.sm_scale;
-  if (a.soft_cap > 0.f) t = a.soft_cap * tanhf(t / a.soft_cap);
-  if (a.slopes != nullptr) t -= a.slopes[h] * (float)abs(pos - j);
-  return t;
-}
+__device__ inline int32_t group(const ChunkArgs& a) { return (int32_t)(a.Hq / a.H); }
+__device__ inline int32_t div_up(int32_t x, int32_t y) { return (x + y - 1) / y; }
 
-// the sequence that row t belongs to (B: none)
-__device__ inline uint32_t seq_of(const ChunkArgs& a, int32_t t) {
-  uint32_t lo = 0u, hi = a.B;
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) / 2u;
-    if (a.q_indptr[mid + 1u] <= t) lo = mid + 1u;
-    else hi = mid;
+// Items of 128 rows, tiles of 64 keys.
+struct ByRows {
+  static __device__ int32_t items(const ChunkArgs& a, const Seq& s) {
+    return div_up(s.n * group(a), kChRows);
   }
-  return lo;
-}
+  static __device__ Item item(const ChunkArgs& a, const Seq& s, int32_t x) {
+    const int32_t G = group(a), i0 = x * kChRows / G,
+                  i1 = min(s.n - 1, (x * kChRows + kChRows - 1) / G);
+    const int32_t hi = a.causal ? min(max(s.off + i1 + 1, 0), s.L) : s.L;
+    const int32_t lo = a.window != 0u ? max(s.off + i0 - (int32_t)a.window + 1, 0) : 0;
+    const int32_t he = div_up(hi, kChTile), pe = div_up(s.prefix, kChTile), lt = lo / kChTile;
+    if (pe >= lt) return Item{0, 0, max(pe, he)};
+    return Item{pe, lt, pe + max(he - lt, 0)};
+  }
+};
+// Items of 128 keys, tiles of 64 rows.
+struct ByKeys {
+  static __device__ int32_t items(const ChunkArgs& a, const Seq& s) { return div_up(s.L, kChRows); }
+  static __device__ Item item(const ChunkArgs& a, const Seq& s, int32_t x) {
+    const int32_t k0 = x * kChRows;
+    int32_t i0 = 0, i1 = s.n;
+    if (k0 >= s.prefix) {
+      if (a.causal) i0 = min(max(k0 - s.off, 0), s.n);
+      if (a.window != 0u) i1 = min(max((int32_t)a.window + k0 + kChRows - 1 - s.off, 0), s.n);
+    }
+    const int32_t G = group(a), t0 = i0 * G / kChTile, t1 = div_up(i1 * G, kChTile);
+    return Item{0, t0, i1 > i0 ? t1 - t0 : 0};
+  }
+};
 
-__device__ inline float wave_max(float x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
-}
-__device__ inline float wave_sum(float x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
-  return x;
-}
+// ---------------------------------------------------------------- shares
+struct PlanLds {
+  Seq seq[kChThreads];           // of the sequences base .. base + 255
+  uint64_t start[kChThreads];    // units before each of them
+  uint64_t wave[kChThreads / kWave];
+  uint64_t off;
+  uint32_t pick;
+};
 
-// One wave per (row, query head): 64 keys at a time, a key per lane for the
-// scores, D / 64 dims per lane for the values.
-template <int D>
-__global__ __launch_bounds__(kChThreads) void chunk_attn_kernel(ChunkArgs a) {
+// the sum of x over the threads before this one, and over all
+__device__ inline uint64_t scan_units(uint64_t x, PlanLds& l, uint64_t& total) {
   const uint32_t lane = __lane_id(), wave = threadIdx.x / kWave;
-  const uint64_t item = (uint64_t)blockIdx.x * (kChThreads / kWave) + wave;
-  if (item >= (uint64_t)a.T * a.Hq) return;
-  const uint32_t t = (uint32_t)(item / a.Hq), h = (uint32_t)(item % a.Hq), hk = h / (a.Hq / a.H);
-  if ((int32_t)t < a.q_indptr[0]) return;
-  const uint32_t b = seq_of(a, (int32_t)t);
-  if (b >= a.B) return;
-  const Seq s = load_seq(a, b);
-  const int32_t pos = s.off + (int32_t)t - s.q0;
-  const f16* q = a.q + ((size_t)t * a.Hq + h) * D;
-  constexpr int kN = D / kWave;
-  float acc[kN] = {}, m = -INFINITY, l = 0.f;
-  for (int32_t j0 = 0; j0 < s.L; j0 += kWave) {
-    const int32_t j = j0 + (int32_t)lane;
-    const bool ok = sees(a, s, pos, j);
-    uint64_t live = __ballot(ok);
-    if (live == 0u) continue;
-    uint32_t page = 0u, slot = 0u;
-    float x = -INFINITY;
-    if (ok) {
-      page = (uint32_t)a.kv_indices[s.page0 + (uint32_t)j / a.S];
-      slot = (uint32_t)j % a.S;
-      const f16* k = a.kv + elem_off(a.g, page, 0, hk, slot);
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot += (float)q[d] * (float)k[d];
-      x = score(a, dot, h, pos, j);
-    }
-    const float top = fmaxf(m, wave_max(x));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float p = ok ? expf(x - base) : 0.f, w = expf(m - base);
-    l = l * w + wave_sum(p);
-    for (int i = 0; i < kN; ++i) acc[i] *= w;
-    m = top;
-    for (; live != 0u; live &= live - 1u) {
-      const int src = __ffsll((unsigned long long)live) - 1;
-      const float pj = __shfl(p, src);
-      const f16* v = a.kv + elem_off(a.g, __shfl(page, src), 1, hk, __shfl(slot, src));
-      for (int i = 0; i < kN; ++i) acc[i] += pj * (float)v[lane * kN + i];
-    }
+  uint64_t y = x;
+#pragma unroll
+  for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
+    const uint64_t z = __shfl_up((unsigned long long)y, d);
+    if (lane >= d) y += z;
   }
-  f16* o = a.o + ((size_t)t * a.Hq + h) * D;
-  for (int i = 0; i < kN; ++i) o[lane * kN + i] = r16(l > 0.f ? acc[i] / l : l == 0.f ? 0.f : l);
-  if (a.lse != nullptr && lane == 0u) a.lse[(size_t)t * a.Hq + h] = l == 0.f ? -INFINITY : m + logf(l);
+  __syncthreads();
+  if (lane == kWave - 1u) l.wave[wave] = y;
+  __syncthreads();
+  uint64_t before = 0u;
+  total = 0u;
+#pragma unroll
+  for (uint32_t w = 0; w < kChThreads / kWave; ++w) {
+    if (w < wave) before += l.wave[w];
+    total += l.wave[w];
+  }
+  return before + y - x;
 }
 
-// One thread per (sequence, kv head, key): the sum over the queries in order.
-template <int D>
-__global__ __launch_bounds__(kChThreads) void attn_weights_kernel(ChunkArgs a) {
-  const uint32_t b = blockIdx.z, hk = blockIdx.y, G = a.Hq / a.H;
-  const Seq s = load_seq(a, b);
-  for (int32_t j = (int32_t)(blockIdx.x * kChThreads + threadIdx.x); j < s.L;
-       j += (int32_t)(gridDim.x * kChThreads)) {
-    const uint32_t page = (uint32_t)a.kv_indices[s.page0 + (uint32_t)j / a.S];
-    const uint32_t slot = (uint32_t)j % a.S;
-    const f16* k = a.kv + elem_off(a.g, page, 0, hk, slot);
-    float sum = 0.f;
-    for (int32_t i = 0; i < s.n; ++i) {
-      const int32_t pos = s.off + i;
-      if (!sees(a, s, pos, j)) continue;
-      for (uint32_t gi = 0; gi < G; ++gi) {
-        const uint32_t h = hk * G + gi;
-        const size_t row = (size_t)(s.q0 + i) * a.Hq + h;
-        float dot = 0.f;
-        for (int d = 0; d < D; ++d) dot += (float)a.q[row * D + d] * (float)k[d];
-        const float lse = a.lse[row];
-        sum += lse == -INFINITY ? 0.f : expf(score(a, dot, h, pos, j) - lse);
+// A place in the list of all items' units: head by head, in it sequence by
+// sequence, in it item by item.
+template <class By>
+struct Walk {
+  const ChunkArgs& a;
+  PlanLds& l;
+  uint32_t base;    // first sequence in l.seq
+  uint64_t before;  // units of the sequences before it
+  uint64_t inside;  // ... and of those in l.seq
+  uint32_t h, b;
+  int32_t x;        // item of sequence b
+  uint32_t at;      // unit of the item
+
+  __device__ Walk(const ChunkArgs& args, PlanLds& lds) : a(args), l(lds), base(0u), before(0u),
+                                                         inside(0u), h(0u), b(0u), x(0), at(0u) {}
+  __device__ const Seq& seq() const { return l.seq[b - base]; }
+  __device__ void load(uint32_t first) {
+    __syncthreads();
+    if (first + threadIdx.x < a.B) l.seq[threadIdx.x] = load_seq(a, first + threadIdx.x);
+    __syncthreads();
+    base = first;
+  }
+  // loads the sequences from `first` on and counts their units (several
+  // threads share a sequence's items where the batch is small)
+  __device__ void count(uint32_t first, uint64_t units_before) {
+    load(first);
+    const uint32_t nb = min(a.B - first, kChThreads);
+    const uint32_t per = kChThreads >> (nb > 1u ? 32 - __clz(nb - 1u) : 0);
+    const uint32_t sb = threadIdx.x / per, k = threadIdx.x % per;
+    uint64_t u = 0u;
+    if (sb < nb) {
+      const Seq s = l.seq[sb];
+      const int32_t n = By::items(a, s);
+      for (int32_t i = (int32_t)k; i < n; i += (int32_t)per)
+        u += (uint32_t)By::item(a, s, i).count + kItemUnits;
+    }
+    before = units_before;
+    const uint64_t p = scan_units(u, l, inside);
+    if (sb < nb && k == 0u) l.start[sb] = before + p;
+    __syncthreads();
+  }
+  // units of one head
+  __device__ uint64_t total() {
+    uint64_t t = 0u;
+    for (uint32_t first = 0u; first < a.B; first += kChThreads) {
+      count(first, t);
+      t += inside;
+    }
+    return t;
+  }
+  // goes to unit u of all heads, total() units each (u < H * total); total()
+  // was called before
+  __device__ void seek(uint64_t u, uint64_t per_head) {
+    h = (uint32_t)(u / per_head);
+    const uint64_t y = u % per_head;
+    if (a.B > kChThreads) {
+      uint64_t t = 0u;
+      for (uint32_t first = 0u;; first += kChThreads) {
+        count(first, t);
+        t += inside;
+        if (y < t) break;
       }
     }
-    float* w = a.weights + ((size_t)page * a.H + hk) * a.S + slot;
-    const int32_t start = a.start != nullptr ? a.start[b] : s.off;
-    *w = (j < start ? *w : 0.f) + sum;
+    const uint32_t nb = min(a.B - base, kChThreads), i = threadIdx.x;
+    if (i < nb) {
+      const uint64_t s = l.start[i], e = i + 1u < nb ? l.start[i + 1u] : before + inside;
+      if (s <= y && y < e) l.pick = i;
+    }
+    __syncthreads();
+    b = base + l.pick;
+    uint64_t rest = y - l.start[b - base];
+    const Seq s = seq();
+    const int32_t n = By::items(a, s);
+    __syncthreads();
+    for (int32_t first = 0;; first += (int32_t)kChThreads) {
+      const int32_t j = first + (int32_t)i;
+      const uint64_t v = j < n ? (uint32_t)By::item(a, s, j).count + kItemUnits : 0u;
+      uint64_t sum;
+      const uint64_t p = scan_units(v, l, sum);
+      if (rest < sum) {
+        if (p <= rest && rest < p + v) {
+          l.pick = (uint32_t)j;
+          l.off = rest - p;
+        }
+        __syncthreads();
+        break;
+      }
+      rest -= sum;
+    }
+    x = (int32_t)l.pick;
+    at = (uint32_t)l.off;
+    __syncthreads();
   }
+  // the next item (there is one)
+  __device__ void next() {
+    at = 0u;
+    ++x;
+    while (x >= By::items(a, seq())) {
+      x = 0;
+      if (++b == a.B) {
+        b = 0u;
+        ++h;
+      }
+      if (b / kChThreads * kChThreads != base) load(b / kChThreads * kChThreads);
+    }
+  }
+};
+
+// The share of workgroup w: units [w * share, (w + 1) * share) of them.
+__device__ inline uint64_t share_of(uint64_t units, uint32_t workgroups, uint32_t least) {
+  const uint64_t s = (units + workgroups - 1u) / workgroups;
+  return s > least ? s : least;
+}
+
+// Workgroup b runs on XCD b % 8: neighbours in the list share an XCD (and its L2).
+__device__ inline uint32_t list_place() {
+  return blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+}
+
+// x / S for x * S < 2^32 (rcp = floor(2^32 / S) + 1, or 0 for S = 1)
+__device__ inline uint32_t div_page(uint32_t x, uint32_t rcp) {
+  return rcp == 0u ? x : __umulhi(x, rcp);
+}
+
+// ---------------------------------------------------------------- attention
+constexpr int kCap = 1, kBias = 2;  // MOD bits
+
+// floats of a part: O [D / 4][128 rows][4], m [128], l [128]
+__host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kChRows * (D + 2); }
+// workgroups per CU (LDS: two buffers of K and V tiles; see prefill.hip)
+template <int D>
+constexpr uint32_t attn_per_cu() { return D == 256 ? 1u : 2u; }
+constexpr uint32_t kCus = 256u;
+constexpr uint32_t kAttnLeast = 4u;  // units of a share at least
+
+// Row r of a sequence's packed rows.
+struct Row {
+  int32_t tok;  // token of the chunk
+  uint32_t h;   // query head
+};
+__device__ inline Row row_of(const ChunkArgs& a, uint32_t hk, int32_t r) {
+  const int32_t G = group(a), tok = r / G;
+  return Row{tok, hk * (uint32_t)G + (uint32_t)(r - tok * G)};
+}
+
+// o and lse of a row: O dims 32 t + crow(i, g) of the lane's row
+template <int D>
+__device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r, int g, float m2,
+                                 float l, const floatx16 (&acc)[PfShape<D>::kDB]) {
+  const size_t row = (size_t)(s.q0 + r.tok) * a.Hq + r.h;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  f16* o = a.o + row * D;
+#pragma unroll
+  for (int t = 0; t < PfShape<D>::kDB; ++t)
+#pragma unroll
+    for (int i0 = 0; i0 < 16; i0 += 4) {
+      half4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (f16)(acc[t][i0 + e] * inv);
+      *reinterpret_cast<half4*>(o + t * 32 + crow(i0, g)) = v;
+    }
+  if (a.lse != nullptr && g == 0)
+    a.lse[row] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// One workgroup's share.  The tile loop is that of prefill.hip (S^T = K Q^T,
+// lane l holds row l % 32 of its wave's 32); scores are kept in units of log 2.
+template <int D, int MOD, bool S16>
+__global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kernel(ChunkArgs a) {
+  using Sh = PfShape<D>;
+  __shared__ __attribute__((aligned(16))) char s_buf0[2 * Sh::kTileBytes];
+  __shared__ __attribute__((aligned(16))) char s_buf1[2 * Sh::kTileBytes];
+  __shared__ PlanLds s_plan;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+
+  Walk<ByRows> w(a, s_plan);
+  const uint64_t per_head = w.total(), units = per_head * a.H;
+  const uint64_t share = share_of(units, gridDim.x, kAttnLeast);
+  uint64_t u = list_place() * share;
+  const uint64_t u1 = min(u + share, units);
+  if (u >= u1) return;
+  w.seek(u, per_head);
+
+  const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
+  // cap: c tanh(x / c) = c - 2 c / (1 + e^(2 x / c))
+  const float cap2 = a.soft_cap * kLog2e;
+  const float cap_in = MOD & kCap ? 2.f * kLog2e * a.sm_scale / a.soft_cap : 0.f;
+  const int32_t window = a.window != 0u ? (int32_t)a.window : 1 << 30;
+
+  for (;;) {
+    // (the offsets below are made anew for each item: kept over the loop, their
+    // registers would be missing at an item's end)
+    int lane = (int)__lane_id();
+    asm volatile("" : "+v"(lane));
+    const int g = lane / 32, c = lane % 32;
+    constexpr int kNI = 16 / Sh::kRPI;  // load instructions per wave and tile
+    constexpr int kRow16 = 16 * Sh::kRowBytes;
+    const int lrow = lane / Sh::kCh, lslot = lane % Sh::kCh;
+    // lane-constant offsets into a tile (see prefill.hip)
+    const int vm = (lane % 16) / 4, va4 = lane % 4, vG = lane / 16;
+    auto v_off = [&](int t, int key0) {
+      const int row = key0 + vm;
+      const int dim = 32 * t + 16 * (vG % 2) + 4 * va4;
+      return row * Sh::kRowBytes + 16 * ((dim / 8) ^ v_swz<Sh::kCh>(row)) + 2 * (dim % 8);
+    };
+    int k_off[Sh::kKS], v_lo[Sh::kDB], v_hi[Sh::kDB];
+#pragma unroll
+    for (int s8 = 0; s8 < Sh::kKS; ++s8) k_off[s8] = tile_off<D>(c, 2 * s8 + g);
+#pragma unroll
+    for (int t = 0; t < Sh::kDB; ++t) {
+      v_lo[t] = v_off(t, 4 * g);
+      v_hi[t] = v_off(t, 4 * g + 8);
+    }
+
+    const Seq s = w.seq();
+    const Item item = ByRows::item(a, s, w.x);
+    const uint32_t hk = w.h;
+    const uint32_t ue = (uint32_t)item.count + kItemUnits;
+    const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
+    const int32_t t0 = max((int32_t)(ua - kItemUnits), 0), t1 = max((int32_t)(ub - kItemUnits), 0);
+
+    // ---- this lane's row
+    const int32_t R = s.n * group(a);
+    const int32_t r0 = w.x * kChRows + wave * 32;  // the wave's first row
+    const int32_t r = r0 + c;
+    const bool live = r < R;
+    const Row row = row_of(a, hk, live ? r : R - 1);
+    const int32_t pos = s.off + row.tok;
+    half8 qreg[Sh::kKS];
+    {
+      const f16* q = a.q + ((size_t)(s.q0 + row.tok) * a.Hq + row.h) * D + 8 * g;
+#pragma unroll
+      for (int s8 = 0; s8 < Sh::kKS; ++s8) qreg[s8] = *reinterpret_cast<const half8*>(q + 16 * s8);
+    }
+    const float slope = MOD & kBias ? a.slopes[row.h] * kLog2e : 0.f;
+    // keys the row sees: below s.prefix, and [lo, hi)
+    const int32_t hi = a.causal ? min(pos + 1, s.L) : s.L, lo = pos - window + 1;
+    // first and last position of the wave's rows and of the item's
+    const int32_t G = group(a);
+    const int32_t wp0 = s.off + min(r0, R - 1) / G, wp1 = s.off + min(r0 + 31, R - 1) / G;
+    const int32_t ip0 = s.off + w.x * kChRows / G,
+                  ip1 = s.off + min(w.x * kChRows + kChRows - 1, R - 1) / G;
+    // whether rows at positions p0 .. p1 all see the 64 keys from k0 on
+    auto all_see = [&](int32_t k0, int32_t p0, int32_t p1) {
+      return k0 + kChTile <= s.prefix ||
+             (k0 + kChTile <= s.L && (!a.causal || k0 + kChTile - 1 <= p0) && p1 - k0 < window);
+    };
+    // ... or any of the wave's sees one
+    auto any_sees = [&](int32_t k0) {
+      return r0 < R && (k0 < s.prefix || ((!a.causal || k0 <= wp1) &&
+                                          wp0 - (k0 + kChTile - 1) < window));
+    };
+
+    // ---- tile loads: wave w fills rows 16 w .. 16 w + 15 of K and V
+    struct PageIds {
+      uint32_t id[kNI], slot[kNI];
+    };
+    const uint32_t npages = div_page((uint32_t)s.L + a.S - 1u, a.page_rcp);
+    const __attribute__((address_space(4))) int32_t* kv_idx =
+        (const __attribute__((address_space(4))) int32_t*)(a.kv_indices + s.page0);
+    auto page_of = [&](int32_t tile) {
+      const uint32_t key0 = (uint32_t)(tile * kChTile + 16 * wave);
+      PageIds ph;
+      if constexpr (S16) {  // the wave's 16 rows lie in one page
+        uint32_t p = div_page(key0, a.page_rcp);
+        p = p < npages ? p : npages - 1u;
+        ph.id[0] = (uint32_t)kv_idx[p];
+        ph.slot[0] = a.S == 32u ? key0 & 16u : 0u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kNI; ++i) {
+          const uint32_t key = key0 + (uint32_t)(Sh::kRPI * i + lrow);
+          uint32_t p = div_page(key, a.page_rcp);
+          ph.slot[i] = key - p * a.S;
+          p = p < npages ? p : npages - 1u;
+          ph.id[i] = (uint32_t)a.kv_indices[s.page0 + p];
+        }
+      }
+      return ph;
+    };
+    auto load_tile = [&](char* buf, const PageIds& ph) {
+#pragma unroll
+      for (int i = 0; i < kNI; ++i) {
+        const int tr = 16 * wave + Sh::kRPI * i + lrow;
+        const uint32_t slot = S16 ? ph.slot[0] + (uint32_t)(tr & 15) : ph.slot[i];
+        const size_t e = elem_off(a.g, ph.id[S16 ? 0 : i], 0, hk, slot);
+        load_lds16(a.kv + e + 8 * (lslot ^ k_swz<Sh::kCh>(tr)),
+                   buf + (16 * wave + Sh::kRPI * i) * Sh::kRowBytes);
+        load_lds16(a.kv + e + a.g.kv + 8 * (lslot ^ v_swz<Sh::kCh>(tr)),
+                   buf + Sh::kTileBytes + (16 * wave + Sh::kRPI * i) * Sh::kRowBytes);
+      }
+    };
+
+    floatx16 acc_o[Sh::kDB];
+#pragma unroll
+    for (int t = 0; t < Sh::kDB; ++t) acc_o[t] = floatx16{};
+    float m_run = kPfNoMax, l_run = 0.f;
+    // O elements that a value of +inf / -inf / NaN (both) reaches, bit 16 t + i
+    constexpr int kFlags = D == 256 ? 2 : 1;
+    uint64_t inf_pos[kFlags] = {}, inf_neg[kFlags] = {};
+
+    auto vfrag = [&](const lds_char* sV, int t, int kk) {
+      const int rows = kk * kRow16;
+      const half4 x = __builtin_bit_cast(
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + v_lo[t] + rows)));
+      const half4 y = __builtin_bit_cast(
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + v_hi[t] + rows)));
+      return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+
+    // A tile that not every row sees whole.  A probability of 0 times a value of
+    // inf or NaN would be NaN in the product, so the values of keys that are
+    // none (unwritten slots) become 0; and where another value is not finite
+    // (rare), the O elements that it reaches are noted, and the product gets 0.
+    // Called by the whole workgroup.
+    auto clean_values = [&](char* vbuf, int32_t k0) {
+      constexpr int kN = Sh::kTileBytes / 16 / (int)kChThreads;
+      uint4* chunks = reinterpret_cast<uint4*>(vbuf);
+      uint32_t bad = 0u;
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        const int at = tid + (int)kChThreads * j;
+        if (k0 + at / Sh::kCh >= s.L) {
+          chunks[at] = uint4{0u, 0u, 0u, 0u};
+        } else {
+          const uint4 x = chunks[at];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t y = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+            // (exponent bits all set: adding 1 to them carries)
+            bad |= ((y & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+          }
+        }
+      }
+      if (!__syncthreads_or((int)(bad != 0u))) return;
+      // every wave looks through the tile for its own rows
+#pragma nounroll
+      for (int j = 0; j < Sh::kTileBytes / 16; j += kWave) {
+        const int at = j + lane;
+        const H8 x = __builtin_bit_cast(H8, chunks[at]);
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd |= !__builtin_isfinite((float)x.v[e]);
+#pragma nounroll
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(odd); left != 0u; left &= left - 1u) {
+          const int src = __builtin_ctzll(left);
+          const int tr = (j + src) / Sh::kCh;
+          const int d0 = 8 * (((j + src) % Sh::kCh) ^ v_swz<Sh::kCh>(tr));
+          const int32_t key = k0 + tr;
+          const bool seen = key < s.prefix || (key < hi && key >= lo);
+#pragma nounroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t y = reinterpret_cast<const uint16_t*>(chunks + j + src)[e];
+            if ((y & 0x7C00u) != 0x7C00u) continue;
+            // dim d0 + e is element 16 t + i of lane group dd / 4 % 2
+            const int dd = (d0 + e) % 32, bit = 16 * ((d0 + e) / 32) + 4 * (dd / 8) + dd % 4;
+            const uint64_t mask = seen && dd / 4 % 2 == g ? 1ull << (bit % 64) : 0u;
+            const bool nan = (y & 0x3FFu) != 0u;
+#pragma unroll
+            for (int f = 0; f < kFlags; ++f) {
+              if (bit / 64 != f) continue;
+              if (nan || y == 0x7C00u) inf_pos[f] |= mask;
+              if (nan || y == 0xFC00u) inf_neg[f] |= mask;
+            }
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        H8 x = __builtin_bit_cast(H8, chunks[tid + (int)kChThreads * j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!__builtin_isfinite((float)x.v[e])) x.v[e] = (f16)0.f;
+        chunks[tid + (int)kChThreads * j] = __builtin_bit_cast(uint4, x);
+      }
+      __syncthreads();
+    };
+
+    auto tile = [&](const lds_char* sK, const lds_char* sV, int32_t k0) {
+      floatx16 acc_s[2];
+      if constexpr (Sh::kKS <= 8) {
+        half8 kf0[Sh::kKS], kf1[Sh::kKS];
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8)
+          kf0[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(sK + k_off[s8]);
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8)
+          kf1[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+              sK + k_off[s8] + 2 * kRow16);
+        __builtin_amdgcn_sched_barrier(0);
+        acc_s[0] = floatx16{};
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[0] = mfma32(kf0[s8], qreg[s8], acc_s[0]);
+        acc_s[1] = floatx16{};
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[1] = mfma32(kf1[s8], qreg[s8], acc_s[1]);
+      } else {
+        constexpr int kB = 8, kNB = 2 * Sh::kKS / kB;  // batches of 8 fragments
+        auto kread = [&](int bt, half8 (&kf)[kB]) {
+#pragma unroll
+          for (int j = 0; j < kB; ++j)
+            kf[j] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+                sK + k_off[(bt % (kNB / 2)) * kB + j] + (bt / (kNB / 2)) * 2 * kRow16);
+        };
+        half8 kfa[kB], kfb[kB];
+        acc_s[0] = floatx16{};
+        acc_s[1] = floatx16{};
+        kread(0, kfa);
+#pragma unroll
+        for (int bt = 0; bt < kNB; bt += 2) {
+          kread(bt + 1, kfb);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < kB; ++j)
+            acc_s[bt / (kNB / 2)] =
+                mfma32(kfa[j], qreg[(bt % (kNB / 2)) * kB + j], acc_s[bt / (kNB / 2)]);
+          if (bt + 2 < kNB) kread(bt + 2, kfa);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < kB; ++j)
+            acc_s[(bt + 1) / (kNB / 2)] =
+                mfma32(kfb[j], qreg[((bt + 1) % (kNB / 2)) * kB + j], acc_s[(bt + 1) / (kNB / 2)]);
+        }
+      }
+      if constexpr (MOD != 0) {
+        const float d0 = (float)(pos - k0 - 4 * g);  // crow(i, g) = crow(i, 0) + 4 g
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float t = acc_s[ks][i];
+            if constexpr (MOD & kCap)
+              t = __builtin_fmaf(-2.f * cap2,
+                                 __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * cap_in)),
+                                 cap2);
+            else
+              t *= a.sm_scale * kLog2e;
+            if constexpr (MOD & kBias)
+              t = __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(ks * 32 + crow(i, 0))), t);
+            acc_s[ks][i] = t;
+          }
+      }
+      if (!all_see(k0, wp0, wp1)) {
+        const int32_t first = k0 + 4 * g, pre = s.prefix - first, end = hi - first,
+                      begin = lo - first;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int32_t key = ks * 32 + crow(i, 0);
+            acc_s[ks][i] = key < pre || (key < end && key >= begin) ? acc_s[ks][i] : -INFINITY;
+          }
+      }
+      float mt = acc_s[0][0];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mt = fmaxf(mt, acc_s[ks][i]);
+      mt = pair_max(mt);
+      // lazy rescaling (see prefill.hip): a row's running max moves only where a
+      // probability would pass 2^8 (each row by itself: what other rows of the
+      // wave see does not touch its bits)
+      const bool up = (mt - m_run) * scale > 8.f;
+      const bool move = __builtin_amdgcn_ballot_w64(up) != 0;
+      const float m_new = up ? mt : m_run;
+      const float neg_m = -m_new * scale;
+      float lt = 0.f;
+      half8 pb[2][2];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc_s[ks][i], scale, neg_m));
+          lt += p;
+          // (fp16: half a step of 2^-11 per probability, as the values' own; the
+          // sum l has them unrounded)
+          pb[ks][i / 8][i % 8] = (f16)p;
+        }
+      lt = pair_sum(lt);
+      if (move) {
+        const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * scale);
+        l_run = l_run * alpha;
+#pragma unroll
+        for (int t = 0; t < Sh::kDB; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc_o[t][i] *= alpha;
+      }
+      l_run = l_run + lt;
+      m_run = m_new;
+      half8 vfa[4], vfb[4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) vfa[kk] = vfrag(sV, 0, kk);
+#pragma unroll
+      for (int t = 0; t < Sh::kDB; t += 2) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) vfb[kk] = vfrag(sV, t + 1, kk);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) acc_o[t] = mfma32(vfa[kk], pb[kk / 2][kk % 2], acc_o[t]);
+        if (t + 2 < Sh::kDB) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) vfa[kk] = vfrag(sV, t + 2, kk);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          acc_o[t + 1] = mfma32(vfb[kk], pb[kk / 2][kk % 2], acc_o[t + 1]);
+      }
+    };
+
+    // ---- the tiles of this part
+    __syncthreads();  // the item before is done with the buffers
+    PageIds ids{};
+    if (t0 < t1) {
+      load_tile(s_buf0, page_of(item.tile(t0)));
+      if (t0 + 1 < t1) ids = page_of(item.tile(t0 + 1));
+    }
+    for (int32_t it = t0; it < t1; it += 2) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int32_t i = it + v;
+        if (i >= t1) break;  // uniform
+        char* buf = v == 0 ? s_buf0 : s_buf1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (i + 1 < t1) {
+          load_tile(v == 0 ? s_buf1 : s_buf0, ids);
+          if (i + 2 < t1) ids = page_of(item.tile(i + 2));
+        }
+        const int32_t k0 = item.tile(i) * kChTile;
+        if (!all_see(k0, ip0, ip1)) clean_values(buf + Sh::kTileBytes, k0);  // uniform
+        if (any_sees(k0)) tile((const lds_char*)buf, (const lds_char*)(buf + Sh::kTileBytes), k0);
+      }
+    }
+
+#pragma unroll
+    for (int t = 0; t < Sh::kDB; ++t)
+      if (inf_pos[t / 4] != 0u || inf_neg[t / 4] != 0u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int bit = (16 * t + i) % 64;
+          if (inf_pos[t / 4] >> bit & 1u) acc_o[t][i] += INFINITY;
+          if (inf_neg[t / 4] >> bit & 1u) acc_o[t][i] -= INFINITY;
+        }
+      }
+    if (ua == 0u && ub == ue) {
+      if (live) store_row<D>(a, s, row, g, m_run * scale, l_run, acc_o);
+    } else if (live) {  // a part: m in units of log 2
+      float* part = a.parts + (2u * (size_t)list_place() + (ua == 0u ? 1u : 0u)) * part_floats(D);
+      float4* po = reinterpret_cast<float4*>(part) + wave * 32 + c;
+#pragma unroll
+      for (int j = 0; j < Sh::kDB * 4; ++j) {
+        const floatx16& x = acc_o[j / 4];
+        const int i0 = 4 * (j % 4);
+        po[(8 * (j / 4) + 2 * (j % 4) + g) * kChRows] =
+            float4{x[i0], x[i0 + 1], x[i0 + 2], x[i0 + 3]};
+      }
+      if (g == 0) {
+        float* pm = part + kChRows * D + wave * 32 + c;
+        pm[0] = m_run * scale;
+        pm[kChRows] = l_run;
+      }
+    }
+    u += ub - ua;
+    if (u >= u1) return;
+    w.next();
+  }
+}
+
+// Where the item that the border before workgroup w's share cuts begins and
+// ends: its parts are slot 1 of workgroup `first` and slot 0 of first + 1 ..
+// last.  False if the border cuts none, or it is not the item's first cut.
+template <class By>
+__device__ inline bool seek_cut(Walk<By>& w, uint32_t place, uint32_t workgroups, uint32_t least,
+                                uint32_t& last) {
+  const uint64_t per_head = w.total(), units = per_head * w.a.H;
+  const uint64_t share = share_of(units, workgroups, least);
+  const uint64_t u = place * share;
+  if (u >= units) return false;
+  w.seek(u, per_head);
+  if (w.at == 0u || w.at > share) return false;  // (at == share: begins where the share before does)
+  const Item item = By::item(w.a, w.seq(), w.x);
+  last = (uint32_t)((u - w.at + (uint32_t)item.count + kItemUnits - 1u) / share);
+  return true;
+}
+
+// Joins an item's parts: workgroup (w, sub) takes 32 of its rows, a thread one
+// row and D / 8 dims.
+template <int D>
+__global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a, uint32_t workgroups) {
+  __shared__ PlanLds s_plan;
+  Walk<ByRows> w(a, s_plan);
+  const uint32_t place = blockIdx.x / 4u + 1u, sub = blockIdx.x % 4u;
+  uint32_t last = 0u;
+  if (!seek_cut(w, place, workgroups, kAttnLeast, last)) return;
+  const Seq s = w.seq();
+  const int32_t r = (int32_t)(sub * 32u + threadIdx.x % 32u);
+  if (w.x * kChRows + r >= s.n * group(a)) return;
+  const Row row = row_of(a, w.h, w.x * kChRows + r);
+  const uint32_t j0 = threadIdx.x / 32u;
+  const uint32_t n = last - place + 2u;
+  auto part = [&](uint32_t i) {
+    return a.parts + (2u * (size_t)(place - 1u + i) + (i == 0u ? 1u : 0u)) * part_floats(D);
+  };
+  float m = kPfNoMax, l = 0.f;
+  for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, part(i)[kChRows * D + r]);
+  constexpr int kV = D / 32;
+  float4 acc[kV] = {};
+  for (uint32_t i = 0; i < n; ++i) {
+    const float* p = part(i);
+    const float f = __builtin_amdgcn_exp2f(p[kChRows * D + r] - m);
+    l += p[kChRows * (D + 1) + r] * f;
+#pragma unroll
+    for (int v = 0; v < kV; ++v) {
+      const float4 y = reinterpret_cast<const float4*>(p)[(kV * j0 + v) * kChRows + r];
+      acc[v].x += y.x * f;
+      acc[v].y += y.y * f;
+      acc[v].z += y.z * f;
+      acc[v].w += y.w * f;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const size_t at = (size_t)(s.q0 + row.tok) * a.Hq + row.h;
+  f16* o = a.o + at * D + 4 * kV * j0;
+#pragma unroll
+  for (int v = 0; v < kV; ++v)
+    *reinterpret_cast<half4*>(o + 4 * v) = half4{(f16)(acc[v].x * inv), (f16)(acc[v].y * inv),
+                                                 (f16)(acc[v].z * inv), (f16)(acc[v].w * inv)};
+  if (a.lse != nullptr && j0 == 0u)
+    a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------- weights
+constexpr uint32_t kSumsPerCu = 2u;
+constexpr uint32_t kSumsLeast = 4u;
+
+// tanh(y): near 0, where 1 - 2 / (e^2y + 1) has no relative precision left, the
+// odd series to y^9 (its next term is 0.0089 y^10 of the result: 1.5e-8 at y =
+// 0.27)
+__device__ inline float tanh_f32(float y) {
+  const float y2 = y * y;
+  float s = __builtin_fmaf(y2, 62.f / 2835.f, -17.f / 315.f);
+  s = __builtin_fmaf(y2, s, 2.f / 15.f);
+  s = __builtin_fmaf(y2, s, -1.f / 3.f);
+  s = __builtin_fmaf(y * y2, s, y);
+  const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
+  const float f = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e);
+  return __builtin_fabsf(y) < 0.27f ? s : f;
+}
+
+__device__ inline void store_weight(const ChunkArgs& a, const Seq& s, uint32_t b, uint32_t hk,
+                                    int32_t j, float sum) {
+  if (j >= s.L) return;
+  const uint32_t p = div_page((uint32_t)j, a.page_rcp);
+  const uint32_t page = (uint32_t)a.kv_indices[s.page0 + p];
+  float* w = a.weights + ((size_t)page * a.H + hk) * a.S + ((uint32_t)j - p * a.S);
+  const int32_t start = a.start != nullptr ? a.start[b] : s.off;
+  *w = (j < start ? *w : 0.f) + sum;
+}
+
+// One workgroup's share of the items of 128 keys.  Scores are S = Q K^T: a wave
+// holds 32 keys as B operands in registers (lane l: key l % 32) and reads 64
+// query rows at a time from LDS, so a key's sum is a sum over a lane's own
+// registers.  Each 32 rows are added up by themselves first: one chain of
+// single additions over 16384 rows was 2e-6 off.
+template <int D, int MOD>
+__global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(ChunkArgs a) {
+  using Sh = PfShape<D>;
+  __shared__ __attribute__((aligned(16))) char s_q0[Sh::kTileBytes];
+  __shared__ __attribute__((aligned(16))) char s_q1[Sh::kTileBytes];
+  // of a tile's rows: -lse in units of log 2 (-inf: the row counts nothing),
+  // position, slope
+  __shared__ __attribute__((aligned(16))) float s_neg[2][kChTile];
+  __shared__ __attribute__((aligned(16))) int32_t s_pos[2][kChTile];
+  __shared__ __attribute__((aligned(16))) float s_slope[2][kChTile];
+  __shared__ PlanLds s_plan;
+  const int tid = threadIdx.x;
+  const int lane = (int)__lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int g = lane / 32, c = lane % 32;
+
+  Walk<ByKeys> w(a, s_plan);
+  const uint64_t per_head = w.total(), units = per_head * a.H;
+  const uint64_t share = share_of(units, gridDim.x, kSumsLeast);
+  uint64_t u = list_place() * share;
+  const uint64_t u1 = min(u + share, units);
+  if (u >= u1) return;
+  w.seek(u, per_head);
+
+  constexpr int kNI = 16 / Sh::kRPI;
+  constexpr int kRow32 = 32 * Sh::kRowBytes;
+  const int lrow = lane / Sh::kCh, lslot = lane % Sh::kCh;
+  int q_off[Sh::kKS];
+#pragma unroll
+  for (int s8 = 0; s8 < Sh::kKS; ++s8) q_off[s8] = tile_off<D>(c, 2 * s8 + g);
+  const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
+  const float cap2 = a.soft_cap * kLog2e;
+  const float cap_in = MOD & kCap ? a.sm_scale / a.soft_cap : 0.f;
+  const int32_t window = a.window != 0u ? (int32_t)a.window : 1 << 30;
+
+  for (;;) {
+    const Seq s = w.seq();
+    const Item item = ByKeys::item(a, s, w.x);
+    const uint32_t hk = w.h;
+    const uint32_t ue = (uint32_t)item.count + kItemUnits;
+    const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
+    const int32_t t0 = max((int32_t)(ua - kItemUnits), 0), t1 = max((int32_t)(ub - kItemUnits), 0);
+    const int32_t R = s.n * group(a);
+    const int32_t k0 = w.x * kChRows + wave * 32;  // the wave's first key
+    const int32_t key = k0 + c;
+
+    half8 kf[Sh::kKS];
+    {
+      const uint32_t j = (uint32_t)min(key, s.L - 1), p = div_page(j, a.page_rcp);
+      const uint32_t page = (uint32_t)a.kv_indices[s.page0 + p];
+      const f16* k = a.kv + elem_off(a.g, page, 0, hk, j - p * a.S) + 8 * g;
+#pragma unroll
+      for (int s8 = 0; s8 < Sh::kKS; ++s8) kf[s8] = *reinterpret_cast<const half8*>(k + 16 * s8);
+    }
+
+    auto load_tile = [&](char* buf, int32_t tile) {
+#pragma unroll
+      for (int i = 0; i < kNI; ++i) {
+        const int tr = 16 * wave + Sh::kRPI * i + lrow;
+        const Row row = row_of(a, hk, min(tile * kChTile + tr, R - 1));
+        const f16* q = a.q + ((size_t)(s.q0 + row.tok) * a.Hq + row.h) * D;
+        load_lds16(q + 8 * (lslot ^ k_swz<Sh::kCh>(tr)),
+                   buf + (16 * wave + Sh::kRPI * i) * Sh::kRowBytes);
+      }
+    };
+    auto load_rows = [&](int v, int32_t tile) {
+      if (tid < kChTile) {
+        const int32_t r = tile * kChTile + tid;
+        const Row row = row_of(a, hk, min(r, R - 1));
+        const float lse = a.lse[(size_t)(s.q0 + row.tok) * a.Hq + row.h];
+        s_neg[v][tid] = r < R && lse != -INFINITY ? -lse * kLog2e : -INFINITY;
+        s_pos[v][tid] = s.off + row.tok;
+        if constexpr (MOD & kBias) s_slope[v][tid] = a.slopes[row.h] * kLog2e;
+      }
+    };
+
+    float sum = 0.f;
+    __syncthreads();  // the item before is done with the buffers
+    if (t0 < t1) {
+      load_tile(s_q0, item.tile(t0));
+      load_rows(0, item.tile(t0));
+    }
+    for (int32_t it = t0; it < t1; it += 2) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int32_t i = it + v;
+        if (i >= t1) break;  // uniform
+        const lds_char* sQ = (const lds_char*)(v == 0 ? s_q0 : s_q1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (i + 1 < t1) {
+          load_tile(v == 0 ? s_q1 : s_q0, item.tile(i + 1));
+          load_rows(v ^ 1, item.tile(i + 1));
+        }
+        const int32_t r0 = item.tile(i) * kChTile;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int32_t rh = r0 + 32 * half;
+          const int32_t p0 = s.off + min(rh, R - 1) / group(a),
+                        p1 = s.off + min(rh + 31, R - 1) / group(a);
+          // none of the wave's keys is seen, or all by all rows
+          if (rh >= R || (k0 >= s.prefix && ((a.causal && k0 > p1) || p0 - (k0 + 31) >= window)))
+            continue;
+          const bool all = rh + 32 <= R && k0 + 32 <= s.L &&
+                           (k0 + 32 <= s.prefix ||
+                            ((!a.causal || k0 + 31 <= p0) && p1 - k0 < window));
+          floatx16 acc = floatx16{};
+          half8 qf[Sh::kKS];
+#pragma unroll
+          for (int s8 = 0; s8 < Sh::kKS; ++s8)
+            qf[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+                sQ + q_off[s8] + half * kRow32);
+#pragma unroll
+          for (int s8 = 0; s8 < Sh::kKS; ++s8) acc = mfma32(qf[s8], kf[s8], acc);
+          float part = 0.f;
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const int at = 32 * half + 8 * q4 + 4 * g;  // rows crow(4 q4, g) ..
+            const float4 neg = *reinterpret_cast<const float4*>(&s_neg[v][at]);
+            const float ng[4] = {neg.x, neg.y, neg.z, neg.w};
+            int32_t ps[4] = {};
+            if (MOD & kBias || !all) {
+              const int4 x = *reinterpret_cast<const int4*>(&s_pos[v][at]);
+              ps[0] = x.x, ps[1] = x.y, ps[2] = x.z, ps[3] = x.w;
+            }
+            float sl[4] = {};
+            if constexpr (MOD & kBias) {
+              const float4 x = *reinterpret_cast<const float4*>(&s_slope[v][at]);
+              sl[0] = x.x, sl[1] = x.y, sl[2] = x.z, sl[3] = x.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float t = acc[4 * q4 + e];
+              if constexpr (MOD & kCap) t = cap2 * tanh_f32(t * cap_in);
+              else if constexpr (MOD != 0) t *= a.sm_scale * kLog2e;
+              if constexpr (MOD & kBias)
+                t = __builtin_fmaf(-sl[e], __builtin_fabsf((float)(ps[e] - key)), t);
+              float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t, scale, ng[e]));
+              if (!all) {
+                const bool see =
+                    key < s.L && ng[e] != -INFINITY &&
+                    (key < s.prefix || ((!a.causal || key <= ps[e]) && ps[e] - key < window));
+                p = see ? p : 0.f;
+              }
+              part += p;
+            }
+          }
+          sum += part;
+        }
+      }
+    }
+    sum = pair_sum(sum);
+    if (ua == 0u && ub == ue) {
+      if (g == 0) store_weight(a, s, w.b, hk, key, sum);
+    } else if (g == 0) {
+      a.parts[(2u * (size_t)list_place() + (ua == 0u ? 1u : 0u)) * kChRows + wave * 32 + c] = sum;
+    }
+    u += ub - ua;
+    if (u >= u1) return;
+    w.next();
+  }
+}
+
+// Joins an item's parts: a thread per key.
+__global__ __launch_bounds__(kChThreads) void weights_join_kernel(ChunkArgs a, uint32_t workgroups) {
+  __shared__ PlanLds s_plan;
+  Walk<ByKeys> w(a, s_plan);
+  const uint32_t place = blockIdx.x + 1u;
+  uint32_t last = 0u;
+  if (!seek_cut(w, place, workgroups, kSumsLeast, last)) return;
+  if (threadIdx.x >= (uint32_t)kChRows) return;
+  float sum = a.parts[(2u * (size_t)(place - 1u) + 1u) * kChRows + threadIdx.x];
+  for (uint32_t i = place; i <= last; ++i) sum += a.parts[2u * (size_t)i * kChRows + threadIdx.x];
+  store_weight(a, w.seq(), w.b, w.h, w.x * kChRows + (int32_t)threadIdx.x, sum);
+}
+
+// Workgroups of a call: those that fit on the chip at once, fewer where the
+// call's bounds say that shares of `least` units need no more.
+uint32_t workgroups(const ChunkArgs& a, uint64_t items, uint64_t tiles, uint32_t fit,
+                    uint32_t least) {
+  const uint64_t units = items * (tiles + kItemUnits) * a.H;
+  const uint64_t n = (units + least - 1u) / least;
+  const uint64_t m = n < fit ? n : fit;
+  return (uint32_t)((m + kXcds - 1u) / kXcds * kXcds);
+}
+
+template <int D, int MOD>
+hipError_t launch_attn(const ChunkArgs& a, uint32_t n, hipStream_t s) {
+  if (a.S % 16u == 0u)
+    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, true>), dim3(n), dim3(kChThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, false>), dim3(n), dim3(kChThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_attn(const ChunkArgs& a, hipStream_t s) {
+  const uint64_t G = a.Hq / a.H;
+  const uint32_t n = workgroups(a, (a.T * G) / kChRows + a.B,
+                                ((uint64_t)a.max_pages * a.S) / kChTile + 2u,
+                                kCus * attn_per_cu<D>(), kAttnLeast);
+  hipError_t e = hipSuccess;
+  switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
+    case 0: e = launch_attn<D, 0>(a, n, s); break;
+    case kCap: e = launch_attn<D, kCap>(a, n, s); break;
+    case kBias: e = launch_attn<D, kBias>(a, n, s); break;
+    default: e = launch_attn<D, kCap | kBias>(a, n, s); break;
+  }
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a, n);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
+  const uint64_t G = a.Hq / a.H;
+  const uint32_t n = workgroups(a, (uint64_t)a.B * (((uint64_t)a.max_pages * a.S) / kChRows + 1u),
+                                (a.T * G) / kChTile + 2u, kCus * kSumsPerCu, kSumsLeast);
+  const dim3 grid(n), block(kChThreads);
+  switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
+    case 0: hipLaunchKernelGGL((attn_weights_kernel<D, 0>), grid, block, 0, s, a); break;
+    case kCap: hipLaunchKernelGGL((attn_weights_kernel<D, kCap>), grid, block, 0, s, a); break;
+    case kBias: hipLaunchKernelGGL((attn_weights_kernel<D, kBias>), grid, block, 0, s, a); break;
+    default:
+      hipLaunchKernelGGL((attn_weights_kernel<D, (kCap | kBias)>), grid, block, 0, s, a);
+      break;
+  }
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  hipLaunchKernelGGL(weights_join_kernel, dim3(n - 1u), block, 0, s, a, n);
+  return hipGetLastError();
+}
+
+ChunkArgs with_rcp(const ChunkArgs& args) {
+  ChunkArgs a = args;
+  a.page_rcp = a.S == 1u ? 0u : (uint32_t)((1ull << 32) / a.S) + 1u;
+  return a;
 }
 
 }  // namespace
 
-hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s) {
-  const dim3 grid((uint32_t)(((uint64_t)a.T * a.Hq + 3u) / 4u)), block(kChThreads);
+size_t chunk_attn_workspace(uint32_t head_dim) {
+  const size_t per_cu = head_dim == 256u ? attn_per_cu<256>() : attn_per_cu<128>();
+  return 2u * kCus * per_cu * part_floats((int)head_dim) * sizeof(float);
+}
+size_t attn_weights_workspace() { return 2u * kCus * kSumsPerCu * kChRows * sizeof(float); }
+
+hipError_t launch_chunk_attn(const ChunkArgs& args, uint32_t head_dim, hipStream_t s) {
+  const ChunkArgs a = with_rcp(args);
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL(chunk_attn_kernel<64>, grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL(chunk_attn_kernel<128>, grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL(chunk_attn_kernel<256>, grid, block, 0, s, a); break;
+    case 64: return launch_attn<64>(a, s);
+    case 128: return launch_attn<128>(a, s);
+    default: return launch_attn<256>(a, s);
   }
-  return hipGetLastError();
 }
 
-hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s) {
-  const uint64_t blocks = ((uint64_t)a.max_pages * a.S + kChThreads - 1u) / kChThreads;
-  const dim3 grid((uint32_t)(blocks < 1024u ? blocks : 1024u), a.H, a.B), block(kChThreads);
+hipError_t launch_attn_weights(const ChunkArgs& args, uint32_t head_dim, hipStream_t s) {
+  const ChunkArgs a = with_rcp(args);
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL(attn_weights_kernel<64>, grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL(attn_weights_kernel<128>, grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL(attn_weights_kernel<256>, grid, block, 0, s, a); break;
+    case 64: return launch_sums<64>(a, s);
+    case 128: return launch_sums<128>(a, s);
+    default: return launch_sums<256>(a, s);
   }
-  return hipGetLastError();
 }
 
 }  // namespace aoakv

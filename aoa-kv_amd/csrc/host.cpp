@@ -556,7 +556,7 @@ PyObject* chunk_attn(PyObject* const* a) {
   const Tensor o = given != nullptr ? *given : at::empty_like(c.q);
   Tensor lse;
   if (want) lse = at::empty({c.q.size(0), c.q.size(1)}, c.q.options().dtype(at::kFloat));
-  const size_t n = g_lib.chunk_attn_workspace_size(c.Hq, c.d.D);
+  const size_t n = g_lib.chunk_attn_workspace_size(c.d.D);
   const Tensor ws = scratch(n, c.q);
   void* s = stream();
   call("aoakv_chunk_attn", [&] {
@@ -585,7 +585,7 @@ void attn_weights(PyObject* const* a) {
     raise(PyExc_ValueError, "weights and kv_data have different page counts");
   const int32_t* start = per_sequence(a[15], "start", c.t.B);
   uint32_t* err = error_word(a[16]);
-  const size_t n = g_lib.attn_weights_workspace_size(c.d.H);
+  const size_t n = g_lib.attn_weights_workspace_size();
   const Tensor ws = scratch(n, c.q);
   void* s = stream();
   call("aoakv_attn_weights", [&] {

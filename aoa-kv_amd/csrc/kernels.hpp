@@ -295,7 +295,14 @@ struct ChunkArgs {
   float sm_scale, soft_cap;   // soft_cap 0: none
   PageGeom g;
   uint32_t* error;            // receives kErrTruncated, or nullptr
+  float* parts;               // the workspace: two slots per workgroup
+  uint32_t page_rcp;          // (set by the launch) divides by S
 };
+// Tokens of a sequence's table at most: positions are divided by the page size
+// as x * (2^32 / S + 1) >> 32, exact for x * S < 2^32.
+constexpr uint32_t kMaxChunkTokens = 1u << 27;
+size_t chunk_attn_workspace(uint32_t head_dim);
+size_t attn_weights_workspace();
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
 hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
 

@@ -488,13 +488,14 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  * the sum of exp(t).  A row that sees no key: o = 0, lse = -inf.  What keys and
  * values hold where a row does not see them changes nothing, NaN and inf too.
  *
- * num_qo_heads is any multiple of num_kv_heads.  max_pages >= every sequence's
- * page count: a longer table is cut to it and AOAKV_WS_ERR_TRUNCATED set in
+ * num_qo_heads is any multiple of num_kv_heads (and num_q_tokens * num_qo_heads
+ * / num_kv_heads < 2^30, max_pages * page_size <= 2^27).  max_pages >= every
+ * sequence's page count: a longer table is cut to it and AOAKV_WS_ERR_TRUNCATED set in
  * *error_word (NULL: not reported), as in aoakv_topk_filtering.  workspace:
  * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
  * initialisation and is free again when the call's work on `stream` is done.
  */
-size_t aoakv_chunk_attn_workspace_size(uint32_t num_qo_heads, uint32_t head_dim);
+size_t aoakv_chunk_attn_workspace_size(uint32_t head_dim);
 int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
                      uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
                      const int32_t* kv_indices, const int32_t* kv_last_page_len,
@@ -519,7 +520,7 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
  * bits.  A batch whose sequences share a page is not allowed.  Slots behind a
  * sequence's last token are not touched.
  */
-size_t aoakv_attn_weights_workspace_size(uint32_t num_kv_heads);
+size_t aoakv_attn_weights_workspace_size(void);
 int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
                        const int32_t* start, float* weights, uint32_t num_q_tokens,
                        const void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,
