@@ -255,11 +255,6 @@ __device__ inline uint32_t list_place() {
   return blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
 }
 
-// x / S for x * S < 2^32 (rcp = floor(2^32 / S) + 1, or 0 for S = 1)
-__device__ inline uint32_t div_page(uint32_t x, uint32_t rcp) {
-  return rcp == 0u ? x : __umulhi(x, rcp);
-}
-
 // ---------------------------------------------------------------- attention
 constexpr int kCap = 1, kBias = 2;  // MOD bits
 

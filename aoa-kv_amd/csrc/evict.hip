@@ -6,8 +6,6 @@
 namespace aoakv {
 namespace {
 
-constexpr uint32_t kEvThreads = 1024;
-
 // tokens of sequence b, held to the call's page bound
 __device__ inline uint32_t seq_tokens(const int32_t* indptr, const int32_t* last_page_len,
                                       uint32_t b, uint32_t max_pages, uint32_t S,
@@ -22,159 +20,359 @@ __device__ inline uint32_t seq_tokens(const int32_t* indptr, const int32_t* last
   return (uint32_t)(P - 1) * S + (uint32_t)last;
 }
 
-// the sum of x over the workgroup's threads before this one, and the total
-__device__ inline uint32_t block_scan(uint32_t x, uint32_t* s_wave, uint32_t& total) {
-  const uint32_t lane = __lane_id(), wave = threadIdx.x / kWave;
-  uint32_t y = x;
-#pragma unroll
-  for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
-    const uint32_t z = __shfl_up(y, d);
-    if (lane >= d) y += z;
-  }
-  __syncthreads();
-  if (lane == kWave - 1u) s_wave[wave] = y;
-  __syncthreads();
-  uint32_t before = 0u;
-  total = 0u;
-  for (uint32_t w = 0; w < kEvThreads / kWave; ++w) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
-  return before + y - x;
-}
+// ---------------------------------------------------------------- choice
+constexpr uint32_t kKeepThreads = 1024;
+constexpr uint32_t kKeepWaves = kKeepThreads / kWave;
+constexpr uint32_t kRun = 4u * kKeepThreads;  // tokens a workgroup takes at once, 4 per thread
+constexpr uint32_t kCopies = 16u;             // of the histogram, one per lane of 16
 
-// One workgroup per (kv head, sequence).  The order of two weights is that of
-// their keys (NaN lowest, -0 as 0); 8 bits of the key at a time, a histogram
-// finds the key of the last token kept, and how many of the tokens with just
-// that key (the lowest positions) are kept with it.
-__global__ __launch_bounds__(kEvThreads) void keep_kernel(KeepArgs a) {
-  __shared__ uint32_t s_hist[256], s_wave[kEvThreads / kWave], s_pick[2];
+// One workgroup per (kv head, sequence).  Two weights are ordered as the
+// integers order_key makes of them (NaN lowest, -0 as 0).  Eight bits of them
+// at a time from the top, a histogram of the tokens that agree so far finds
+// where the last kept one lies, until that bin is kept whole; then a token's
+// place in the row is the number of larger tokens before it plus that of kept
+// equal ones.  The tokens are held in registers (RUNS x 4 per thread), loaded
+// once where a sequence has no more than that, else once per step.
+//
+// The histogram has 16 copies, because weights share few exponents: without
+// them a wave's additions to one word would go one after the other.
+// 2048 of 18,000 to 32,768 tokens, 4 x 32 heads: 143 us with a token per thread
+// and loop trip, every step from memory.
+template <int RUNS, bool VEC>
+__global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
+  __shared__ uint32_t s_hist[256 * kCopies];
+  __shared__ uint32_t s_bins[256];
+  __shared__ uint32_t s_wave[RUNS][kKeepWaves];
+  __shared__ uint32_t s_pick[3];
   const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const uint32_t lane = __lane_id(), wave = tid / kWave;
   const uint32_t L = seq_tokens(a.kv_indptr, a.kv_last_page_len, b, a.max_pages, a.S, a.error);
-  const uint32_t page0 = (uint32_t)a.kv_indptr[b];
+  const int32_t* ids = a.kv_indices + (uint32_t)a.kv_indptr[b];
   int32_t* out = a.kept + ((size_t)b * a.H + h) * a.stride;
   if (L <= a.keep) {
-    for (uint32_t j = tid; j < L; j += kEvThreads) out[j] = (int32_t)j;
+    for (uint32_t j = tid; j < L; j += kKeepThreads) out[j] = (int32_t)j;
     return;
   }
   const uint32_t lo = a.sink, hi = L - a.recent;  // the tokens that compete (lo <= hi)
-  auto key_of = [&](uint32_t j) {
-    const uint32_t page = (uint32_t)a.kv_indices[page0 + j / a.S];
-    const float w = a.weights[((size_t)page * a.H + h) * a.S + j % a.S] + 0.f;
-    return w == w ? order_key(w) : 0u;
+  const uint32_t S = a.S, segment = kRun * RUNS;
+
+  uint32_t key[RUNS][4];
+  auto load = [&](uint32_t seg) {
+    float w[RUNS][4];
+    if constexpr (VEC) {  // 4 tokens of a thread lie in one page
+      uint32_t page[RUNS], slot[RUNS];
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        uint32_t j = seg + (uint32_t)i * kRun + 4u * tid;
+        j = j < L ? j : 0u;
+        const uint32_t p = div_page(j, a.page_rcp);
+        slot[i] = j - p * S;
+        page[i] = (uint32_t)ids[p];
+      }
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(
+            a.weights + ((size_t)page[i] * a.H + h) * S + slot[i]);
+        w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
+          j = j < L ? j : 0u;
+          const uint32_t p = div_page(j, a.page_rcp);
+          w[i][e] = a.weights[((size_t)(uint32_t)ids[p] * a.H + h) * S + (j - p * S)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = w[i][e] + 0.f;
+        key[i][e] = x == x ? order_key(x) : 0u;
+      }
   };
+
   uint32_t need = a.keep - a.sink - a.recent, prefix = 0u, mask = 0u;
+  const bool one = L <= segment;
+  if (one) load(0u);
   for (int shift = 24; shift >= 0 && need != 0u; shift -= 8) {
-    if (tid < 256u) s_hist[tid] = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < 256u * kCopies / kKeepThreads; ++i) s_hist[i * kKeepThreads + tid] = 0u;
     __syncthreads();
-    for (uint32_t j = lo + tid; j < hi; j += kEvThreads) {
-      const uint32_t k = key_of(j);
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+    for (uint32_t seg = 0; seg < hi; seg += segment) {
+      if (!one) load(seg);
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e >= lo && j + e < hi && (key[i][e] & mask) == prefix)
+            atomicAdd(&s_hist[(key[i][e] >> shift & 255u) * kCopies + lane % kCopies], 1u);
+      }
     }
     __syncthreads();
-    if (tid == 0u) {
-      uint32_t left = need, bin = 255u;
-      while (s_hist[bin] < left) left -= s_hist[bin--];
-      s_pick[0] = bin;
-      s_pick[1] = left;
+    if (tid < 256u) {
+      uint32_t n = 0u;
+#pragma unroll
+      for (uint32_t i = 0; i < kCopies; ++i) n += s_hist[tid * kCopies + (tid + i) % kCopies];
+      s_bins[tid] = n;
+    }
+    __syncthreads();
+    if (wave == 0u) {  // lane l has bins 255 - 4 l and the three below
+      uint32_t n[4], sum = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += n[i] = s_bins[255u - 4u * lane - (uint32_t)i];
+      uint32_t upto = sum;
+#pragma unroll
+      for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
+        const uint32_t x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+      }
+      uint32_t left = need - (upto - sum);  // (wraps past the bin sought: no lane's then)
+      if (upto - sum < need && need <= upto) {
+        int i = 0;
+        while (n[i] < left) left -= n[i++];
+        s_pick[0] = 255u - 4u * lane - (uint32_t)i;
+        s_pick[1] = left;
+        s_pick[2] = n[i];
+      }
     }
     __syncthreads();
     prefix |= s_pick[0] << shift;
     mask |= 255u << shift;
     need = s_pick[1];
-    __syncthreads();
+    if (need == s_pick[2]) break;  // the bin is kept whole
   }
-  // need: tokens with the key `prefix` that are kept
-  uint32_t at = 0u, ties = 0u;
+
+  // kept: the forced ones, those above `prefix` under `mask`, and the first
+  // `need` of those at it
   const bool any = a.keep > a.sink + a.recent;
-  for (uint32_t j0 = 0; j0 < L; j0 += kEvThreads) {
-    const uint32_t j = j0 + tid;
-    bool take = false, tie = false;
-    if (j < L) {
-      if (j < lo || j >= hi) take = true;
-      else if (any) {
-        const uint32_t k = key_of(j);
-        take = k > prefix;
-        tie = k == prefix;
+  uint32_t above = 0u, ties = 0u;  // in the runs before
+  for (uint32_t seg = 0; seg < L; seg += segment) {
+    if (!one) load(seg);
+    uint32_t mine[RUNS], upto[RUNS];  // tokens above (low half) and ties of the run
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      mine[i] = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
+        const bool forced = j < lo || j >= hi;
+        const uint32_t k = key[i][e] & mask;
+        if (j < L && (forced || (any && k > prefix))) mine[i] += 1u;
+        else if (j < L && any && k == prefix) mine[i] += 1u << 16;
       }
+      upto[i] = mine[i];
     }
-    uint32_t n;
-    const uint32_t t = block_scan(tie ? 1u : 0u, s_wave, n);
-    take = take || (tie && ties + t < need);
-    ties += n;
-    const uint32_t p = block_scan(take ? 1u : 0u, s_wave, n);
-    if (take) out[at + p] = (int32_t)j;
-    at += n;
+#pragma unroll
+    for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1)
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const uint32_t x = __shfl_up(upto[i], d);
+        if (lane >= d) upto[i] += x;
+      }
+    __syncthreads();
+    if (lane == kWave - 1u) {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) s_wave[i][wave] = upto[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      uint32_t before = 0u, all = 0u;
+#pragma unroll
+      for (uint32_t x = 0; x < kKeepWaves; ++x) {
+        before += x < wave ? s_wave[i][x] : 0u;
+        all += s_wave[i][x];
+      }
+      before += upto[i] - mine[i];
+      uint32_t n = above + (before & 0xFFFFu), t = ties + (before >> 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
+        const bool forced = j < lo || j >= hi;
+        const uint32_t k = key[i][e] & mask;
+        if (j >= L) continue;
+        if (forced || (any && k > prefix)) {
+          out[n + (t < need ? t : need)] = (int32_t)j;
+          ++n;
+        } else if (any && k == prefix) {
+          if (t < need) out[n + t] = (int32_t)j;
+          ++t;
+        }
+      }
+      above += all & 0xFFFFu;
+      ties += all >> 16;
+    }
   }
 }
 
-// One workgroup per (kv head, sequence), page by page in order: a token's new
-// slot is never behind its old one, so a page's tokens are loaded before any
-// slot that a later page still reads is written.
-template <int D>
-__global__ __launch_bounds__(D) void compact_kernel(CompactArgs a) {
-  const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x, S = a.S;
-  __shared__ f16 s_mean[D];
+// ---------------------------------------------------------------- packing
+constexpr uint32_t kPackThreads = 512;
+
+// A workgroup takes steps of K or of V of one (kv head, sequence): each lane
+// group of D / 8 lanes holds MOST tokens at a time (whole pages where a page is
+// shorter, else one page), so all of a step's loads are in flight together and
+// a page's statistics need no other group.  In place one workgroup takes a
+// head's steps in order: a token's new slot is never behind its old one, so
+// a step that has been loaded whole overwrites no later step's tokens.  Else
+// the steps of a head are dealt to gridDim.z / 2 workgroups.
+template <int D, int MOST>
+__global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
+  constexpr uint32_t kLanes = D / 8, kGroups = kPackThreads / kLanes;
+  constexpr uint32_t kTokens = kGroups * MOST;  // of a step, at most
+  __shared__ uint32_t s_page[kTokens], s_slot[kTokens];
+  const uint32_t h = blockIdx.x, b = blockIdx.y, which = blockIdx.z % 2u;
+  const uint32_t tid = threadIdx.x, l = tid % kLanes, grp = tid / kLanes, S = a.S;
   const uint32_t L = seq_tokens(a.kv_indptr, a.kv_last_page_len, b, a.max_pages, S, a.error);
   const uint32_t n = L < a.keep ? L : a.keep;
   const int32_t* kept = a.kept + ((size_t)b * a.H + h) * a.stride;
-  const uint32_t page0 = (uint32_t)a.kv_indptr[b], new0 = (uint32_t)a.new_indptr[b];
-  const uint32_t meta0 = (uint32_t)a.meta_indptr[b];
-  for (uint32_t p = 0; p * S < n; ++p) {
-    const uint32_t c = n - p * S < S ? n - p * S : S;
-    f16 k[kMaxPageSize], v[kMaxPageSize];
-    float w[kMaxPageSize];
-    for (uint32_t e = 0; e < c; ++e) {
-      uint32_t j = (uint32_t)kept[p * S + e];
-      j = j < L ? j : L - 1u;
-      const uint32_t page = (uint32_t)a.kv_indices[page0 + j / S];
-      k[e] = a.kv[elem_off(a.g, page, 0, h, j % S) + d];
-      v[e] = a.kv[elem_off(a.g, page, 1, h, j % S) + d];
-      if (a.weights != nullptr) w[e] = a.weights[((size_t)page * a.H + h) * S + j % S];
+  const int32_t* ids = a.kv_indices + (uint32_t)a.kv_indptr[b];
+  const int32_t* new_ids = a.new_indices + (uint32_t)a.new_indptr[b];
+  const int32_t* meta_ids = a.meta_indices + (uint32_t)a.meta_indptr[b];
+  const uint32_t pages = S < (uint32_t)MOST ? (uint32_t)MOST / S : 1u;  // per group
+  const uint32_t per = pages * S, step = kGroups * per;
+
+  for (uint32_t j0 = blockIdx.z / 2u * step; j0 < n; j0 += gridDim.z / 2u * step) {
+    __syncthreads();  // the step before is stored
+    float w[(kTokens + kPackThreads - 1) / kPackThreads];
+#pragma unroll
+    for (uint32_t i = 0; i < kTokens; i += kPackThreads) {
+      const uint32_t t = i + tid;
+      if (t < step && j0 + t < n) {
+        uint32_t j = (uint32_t)kept[j0 + t];
+        j = j < L ? j : L - 1u;
+        const uint32_t p = div_page(j, a.page_rcp);
+        const uint32_t page = (uint32_t)ids[p], slot = j - p * S;
+        s_page[t] = page;
+        s_slot[t] = slot;
+        if (which == 0u && a.weights != nullptr)
+          w[i / kPackThreads] = a.weights[((size_t)page * a.H + h) * S + slot];
+      }
     }
     __syncthreads();
-    const uint32_t to = (uint32_t)a.new_indices[new0 + p];
-    f16 kmax = (f16)-65504.0f, kmin = (f16)65504.0f;  // as a bulk append's
-    float sum = 0.f;
-    for (uint32_t e = 0; e < c; ++e) {
-      kmax = k[e] > kmax ? k[e] : kmax;
-      kmin = k[e] < kmin ? k[e] : kmin;
-      sum += (float)v[e];
-      a.kv[elem_off(a.g, to, 0, h, e) + d] = k[e];
-      a.kv[elem_off(a.g, to, 1, h, e) + d] = v[e];
-      if (a.weights != nullptr && d == 0u) a.weights[((size_t)to * a.H + h) * S + e] = w[e];
+    const uint32_t first = j0 + grp * per;  // the group's first token
+    const uint32_t c = first < n ? (n - first < per ? n - first : per) : 0u;
+    H8 x[MOST];
+#pragma unroll
+    for (uint32_t t = 0; t < (uint32_t)MOST; ++t)
+      if (t < c)
+        x[t] = ld16(a.kv + elem_off(a.g, s_page[grp * per + t], which, h, s_slot[grp * per + t]) +
+                    l * kVec);
+    const uint32_t p0 = div_page(first, a.page_rcp);  // the group's first new page
+    uint32_t to = c != 0u ? (uint32_t)new_ids[p0] : 0u;
+    if (a.in_place) {  // every load of the step is back before its first store
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
     }
-    const uint32_t mp = (uint32_t)a.meta_indices[meta0 + p / S];
-    a.meta[elem_off(a.g, mp, 0, h, p % S) + d] = kmax;
-    a.meta[elem_off(a.g, mp, 1, h, p % S) + d] = kmin;
-    const f16 mean = r16(sum / (float)c);
-    a.v_mean[((size_t)to * a.H + h) * D + d] = mean;
-    s_mean[d] = mean;
-    __syncthreads();
-    if (d == 0u) {
-      float acc = 0.f;
-      for (int i = 0; i < D; ++i) acc += (float)s_mean[i] * (float)s_mean[i];
-      f16 nrm = r16((float)__builtin_sqrt((double)acc));
-      nrm = r16((float)nrm + 1e-8f);
-      a.v_log_norm[(size_t)to * a.H + h] = r16((float)log((double)(float)nrm));
+    H8 kmax, kmin;
+    float sum[kVec];
+    uint32_t e = 0u, p = p0;
+#pragma unroll
+    for (uint32_t t = 0; t < (uint32_t)MOST; ++t) {
+      if (t >= c) continue;
+      if (e == 0u) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          kmax.v[j] = (f16)-65504.0f;  // as a bulk append starts a page
+          kmin.v[j] = (f16)65504.0f;
+          sum[j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if (which == 0u) {
+          kmax.v[j] = x[t].v[j] > kmax.v[j] ? x[t].v[j] : kmax.v[j];
+          kmin.v[j] = x[t].v[j] < kmin.v[j] ? x[t].v[j] : kmin.v[j];
+        } else {
+          sum[j] = sum[j] + (float)x[t].v[j];
+        }
+      }
+      st16(a.kv + elem_off(a.g, to, which, h, e) + l * kVec, x[t]);
+      if (++e == S || t + 1u == c) {  // the page's last token
+        if (which == 0u) {
+          const uint32_t mp = div_page(p, a.page_rcp), me = p - mp * S;
+          const uint32_t page = (uint32_t)meta_ids[mp];
+          st16(a.meta + elem_off(a.g, page, 0, h, me) + l * kVec, kmax);
+          st16(a.meta + elem_off(a.g, page, 1, h, me) + l * kVec, kmin);
+        } else {
+          H8 mean;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) mean.v[j] = r16(sum[j] / (float)e);
+          st16(a.v_mean + ((size_t)to * a.H + h) * D + l * kVec, mean);
+        }
+        e = 0u;
+        ++p;
+        if (t + 1u < c) to = (uint32_t)new_ids[p];
+      }
     }
-    __syncthreads();
+    // the log-norms (in a loop of their own: once per token above would be
+    // most of the code)
+    if (which == 1u) {
+#pragma nounroll
+      for (uint32_t q = 0; q * S < c; ++q) {
+        const size_t at = (size_t)(uint32_t)new_ids[p0 + q] * a.H + h;
+        const H8 mean = ld16(a.v_mean + at * D + l * kVec);  // (this lane's own store)
+        f16 norm;
+        if constexpr (kLanes == (uint32_t)kLanesPerRow) norm = log_norm_row(mean);
+        else norm = grp_log_norm<kLanes>(mean, l);
+        if (l == 0u) a.v_log_norm[at] = norm;
+      }
+    }
+    if (which == 0u && a.weights != nullptr) {
+#pragma unroll
+      for (uint32_t i = 0; i < kTokens; i += kPackThreads) {
+        const uint32_t t = i + tid;
+        if (t < step && j0 + t < n) {
+          const uint32_t q = div_page(j0 + t, a.page_rcp);
+          a.weights[((size_t)(uint32_t)new_ids[q] * a.H + h) * S + (j0 + t - q * S)] =
+              w[i / kPackThreads];
+        }
+      }
+    }
   }
 }
 
+template <int D>
+void launch_pack(const CompactArgs& a, uint32_t batch, hipStream_t s) {
+  const uint32_t most = a.S > 16u ? 32u : 16u;
+  const uint32_t step = kPackThreads / (D / 8) * (a.S < most ? most / a.S * a.S : a.S);
+  const uint64_t steps = ((uint64_t)a.keep + step - 1u) / step;
+  const uint32_t z = a.in_place ? 1u : (uint32_t)(steps < 16384u ? steps : 16384u);
+  const dim3 grid(a.H, batch, 2u * z), block(kPackThreads);
+  if (most == 16u) hipLaunchKernelGGL((compact_kernel<D, 16>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((compact_kernel<D, 32>), grid, block, 0, s, a);
+}
+
+uint32_t rcp_of(uint32_t S) { return S == 1u ? 0u : (uint32_t)((1ull << 32) / S) + 1u; }
+
 }  // namespace
 
-hipError_t launch_keep(const KeepArgs& a, uint32_t batch, hipStream_t s) {
-  hipLaunchKernelGGL(keep_kernel, dim3(a.H, batch), dim3(kEvThreads), 0, s, a);
+hipError_t launch_keep(const KeepArgs& args, uint32_t batch, hipStream_t s) {
+  KeepArgs a = args;
+  a.page_rcp = rcp_of(a.S);
+  const dim3 grid(a.H, batch), block(kKeepThreads);
+  // 4096 tokens per sequence at most: 4 per thread; else 32
+  const bool few = (uint64_t)a.max_pages * a.S <= kRun;
+  const bool vec = a.S % 4u == 0u && reinterpret_cast<uintptr_t>(a.weights) % 16u == 0u;
+  if (few && vec) hipLaunchKernelGGL((keep_kernel<1, true>), grid, block, 0, s, a);
+  else if (few) hipLaunchKernelGGL((keep_kernel<1, false>), grid, block, 0, s, a);
+  else if (vec) hipLaunchKernelGGL((keep_kernel<8, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((keep_kernel<8, false>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
-hipError_t launch_compact(const CompactArgs& a, uint32_t batch, uint32_t head_dim, hipStream_t s) {
-  const dim3 grid(a.H, batch);
+hipError_t launch_compact(const CompactArgs& args, uint32_t batch, uint32_t head_dim,
+                          hipStream_t s) {
+  CompactArgs a = args;
+  a.page_rcp = rcp_of(a.S);
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL(compact_kernel<64>, grid, dim3(64), 0, s, a); break;
-    case 128: hipLaunchKernelGGL(compact_kernel<128>, grid, dim3(128), 0, s, a); break;
-    default: hipLaunchKernelGGL(compact_kernel<256>, grid, dim3(256), 0, s, a); break;
+    case 64: launch_pack<64>(a, batch, s); break;
+    case 128: launch_pack<128>(a, batch, s); break;
+    default: launch_pack<256>(a, batch, s); break;
   }
   return hipGetLastError();
 }

@@ -54,30 +54,6 @@ __device__ __host__ constexpr float sqrt_d() {
   return D == 64 ? 8.0f : D == 256 ? 16.0f : kSqrtHeadDim;
 }
 
-// log(norm(V̄) + 1e-8) of one D-dim fp16 vector held by an N-lane group, as
-// log_norm_row: fp32 sum of squares in dim order, carried lane to lane,
-// correctly rounded root, fp16 rounding after each op.
-template <uint32_t N>
-__device__ inline f16 grp_log_norm(const H8& vbar, uint32_t l) {
-  const uint32_t base = __lane_id() & ~(N - 1u);
-  float acc = 0.f;
-#pragma unroll
-  for (uint32_t src = 0; src < N; ++src) {
-    if (l == src) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const float x = (float)vbar.v[j];
-        const float sq = x * x;
-        acc = acc + sq;
-      }
-    }
-    acc = __shfl(acc, (int)(base | src), kWave);
-  }
-  f16 nrm = r16((float)__builtin_sqrt((double)acc));
-  nrm = r16((float)nrm + 1e-8f);
-  return r16((float)log((double)(float)nrm));
-}
-
 // RoPE of the 8 dims lane l of an N-lane group holds (D = 8N dims), at
 // position pos: rotate-half with the partner dims d +- D/2 in lane l ^ N/2.
 template <uint32_t N>

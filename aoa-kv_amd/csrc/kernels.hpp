@@ -301,6 +301,10 @@ struct ChunkArgs {
 // Tokens of a sequence's table at most: positions are divided by the page size
 // as x * (2^32 / S + 1) >> 32, exact for x * S < 2^32.
 constexpr uint32_t kMaxChunkTokens = 1u << 27;
+// x / S for x * S < 2^32 (rcp = floor(2^32 / S) + 1, or 0 for S = 1)
+__device__ inline uint32_t div_page(uint32_t x, uint32_t rcp) {
+  return rcp == 0u ? x : __umulhi(x, rcp);
+}
 size_t chunk_attn_workspace(uint32_t head_dim);
 size_t attn_weights_workspace();
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
@@ -316,6 +320,7 @@ struct KeepArgs {
   int32_t* kept;         // [B, H, stride]
   uint32_t stride, keep, sink, recent, max_pages, H, S;
   uint32_t* error;
+  uint32_t page_rcp;     // (set by the launch) divides by S
 };
 hipError_t launch_keep(const KeepArgs& a, uint32_t batch, hipStream_t s);
 
@@ -338,6 +343,7 @@ struct CompactArgs {
   uint32_t max_pages, H, S;
   PageGeom g;
   uint32_t* error;
+  uint32_t page_rcp;     // (set by the launch) divides by S
 };
 hipError_t launch_compact(const CompactArgs& a, uint32_t batch, uint32_t head_dim, hipStream_t s);
 
