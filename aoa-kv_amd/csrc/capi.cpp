@@ -1106,7 +1106,7 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
   REQUIRE(o, "chunk_attn: null pointer argument");
   a.o = static_cast<aoakv::f16*>(o);
   a.lse = lse;
-  a.parts = static_cast<float*>(workspace);
+  a.cuts = workspace;
   return hip_status(aoakv::launch_chunk_attn(a, head_dim, static_cast<hipStream_t>(stream)),
                     "chunk_attn");
 }
@@ -1134,7 +1134,7 @@ int aoakv_attn_weights(const void* q, const float* lse, const int32_t* q_indptr,
   a.lse = const_cast<float*>(lse);  // (only read by the weights)
   a.weights = weights;
   a.start = start;
-  a.parts = static_cast<float*>(workspace);
+  a.cuts = workspace;
   return hip_status(aoakv::launch_attn_weights(a, head_dim, static_cast<hipStream_t>(stream)),
                     "attn_weights");
 }

@@ -72,7 +72,13 @@ struct Item {
   __device__ int32_t tile(int32_t i) const { return i < cut ? i : i - cut + first; }
 };
 
-__device__ inline int32_t group(const ChunkArgs& a) { return (int32_t)(a.Hq / a.H); }
+__device__ inline int32_t group(const ChunkArgs& a) { return (int32_t)a.G; }
+// r / G of a packed row (group_rcp = floor(2^32 / G) + 1 where that divides
+// every row of the call exactly, else 0)
+__device__ inline int32_t token_of(const ChunkArgs& a, int32_t r) {
+  if (a.G == 1u) return r;
+  return a.group_rcp != 0u ? (int32_t)__umulhi((uint32_t)r, a.group_rcp) : r / (int32_t)a.G;
+}
 __device__ inline int32_t div_up(int32_t x, int32_t y) { return (x + y - 1) / y; }
 
 // Items of 128 rows, tiles of 64 keys.
@@ -81,8 +87,8 @@ struct ByRows {
     return div_up(s.n * group(a), kChRows);
   }
   static __device__ Item item(const ChunkArgs& a, const Seq& s, int32_t x) {
-    const int32_t G = group(a), i0 = x * kChRows / G,
-                  i1 = min(s.n - 1, (x * kChRows + kChRows - 1) / G);
+    const int32_t i0 = token_of(a, x * kChRows),
+                  i1 = min(s.n - 1, token_of(a, x * kChRows + kChRows - 1));
     const int32_t hi = a.causal ? min(max(s.off + i1 + 1, 0), s.L) : s.L;
     const int32_t lo = a.window != 0u ? max(s.off + i0 - (int32_t)a.window + 1, 0) : 0;
     const int32_t he = div_up(hi, kChTile), pe = div_up(s.prefix, kChTile), lt = lo / kChTile;
@@ -118,7 +124,7 @@ struct PlanLds {
 __device__ inline uint64_t scan_units(uint64_t x, PlanLds& l, uint64_t& total) {
   const uint32_t lane = __lane_id(), wave = threadIdx.x / kWave;
   uint64_t y = x;
-#pragma unroll
+#pragma nounroll  // (run once: its instructions are fetched cold)
   for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
     const uint64_t z = __shfl_up((unsigned long long)y, d);
     if (lane >= d) y += z;
@@ -189,8 +195,11 @@ struct Walk {
   // goes to unit u of all heads, total() units each (u < H * total); total()
   // was called before
   __device__ void seek(uint64_t u, uint64_t per_head) {
-    h = (uint32_t)(u / per_head);
-    const uint64_t y = u % per_head;
+    // u / per_head < 256: a quotient in fp32 is off by one at most
+    h = (uint32_t)((float)u * __builtin_amdgcn_rcpf((float)per_head));
+    h -= (uint64_t)h * per_head > u ? 1u : 0u;
+    h += (uint64_t)(h + 1u) * per_head <= u ? 1u : 0u;
+    const uint64_t y = u - (uint64_t)h * per_head;
     if (a.B > kChThreads) {
       uint64_t t = 0u;
       for (uint32_t first = 0u;; first += kChThreads) {
@@ -244,10 +253,34 @@ struct Walk {
   }
 };
 
-// The share of workgroup w: units [w * share, (w + 1) * share) of them.
-__device__ inline uint64_t share_of(uint64_t units, uint32_t workgroups, uint32_t least) {
-  const uint64_t s = (units + workgroups - 1u) / workgroups;
+// The share of workgroup w: units [w * share, (w + 1) * share) of them
+// (at least units / workgroups; the factor's rounding is below the 1 added).
+__device__ inline uint64_t share_of(const ChunkArgs& a, uint64_t units, uint32_t least) {
+  const uint64_t s = (uint64_t)((double)units * a.share_rcp) + 1u;
   return s > least ? s : least;
+}
+
+// The item that the border before a workgroup's share cuts, for the launch
+// that joins its parts: slot 1 of the workgroup before, slot 0 of this one to
+// `last`.  last 0: no cut, or not the item's first.
+struct Cut {
+  uint32_t last, h, b;
+  int32_t x, q0, n;
+  uint32_t pad[2];
+};
+template <class By>
+__device__ inline Cut cut_of(const Walk<By>& w, uint32_t place, uint64_t share) {
+  Cut c{};
+  if (w.at == 0u || w.at > share) return c;  // (at == share: it begins where the share before does)
+  const Seq& s = w.seq();
+  const uint32_t after = (uint32_t)By::item(w.a, s, w.x).count + kItemUnits - w.at;
+  c.last = place + (share >= after ? 0u : (after - 1u) / (uint32_t)share);
+  c.h = w.h;
+  c.b = w.b;
+  c.x = w.x;
+  c.q0 = s.q0;
+  c.n = s.n;
+  return c;
 }
 
 // Workgroup b runs on XCD b % 8: neighbours in the list share an XCD (and its L2).
@@ -264,6 +297,7 @@ __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kChRows
 template <int D>
 constexpr uint32_t attn_per_cu() { return D == 256 ? 1u : 2u; }
 constexpr uint32_t kCus = 256u;
+constexpr size_t kCutBytes = kCus * 2u * sizeof(Cut);  // (2 workgroups per CU at most)
 constexpr uint32_t kAttnLeast = 4u;  // units of a share at least
 
 // Row r of a sequence's packed rows.
@@ -272,8 +306,8 @@ struct Row {
   uint32_t h;   // query head
 };
 __device__ inline Row row_of(const ChunkArgs& a, uint32_t hk, int32_t r) {
-  const int32_t G = group(a), tok = r / G;
-  return Row{tok, hk * (uint32_t)G + (uint32_t)(r - tok * G)};
+  const int32_t tok = token_of(a, r);
+  return Row{tok, hk * a.G + (uint32_t)r - (uint32_t)tok * a.G};
 }
 
 // o and lse of a row: O dims 32 t + crow(i, g) of the lane's row
@@ -309,11 +343,15 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 
   Walk<ByRows> w(a, s_plan);
   const uint64_t per_head = w.total(), units = per_head * a.H;
-  const uint64_t share = share_of(units, gridDim.x, kAttnLeast);
+  const uint64_t share = share_of(a, units, kAttnLeast);
   uint64_t u = list_place() * share;
   const uint64_t u1 = min(u + share, units);
-  if (u >= u1) return;
+  if (u >= u1) {
+    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
+    return;
+  }
   w.seek(u, per_head);
+  if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
 
   const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
   // cap: c tanh(x / c) = c - 2 c / (1 + e^(2 x / c))
@@ -329,7 +367,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     const int g = lane / 32, c = lane % 32;
     constexpr int kNI = 16 / Sh::kRPI;  // load instructions per wave and tile
     constexpr int kRow16 = 16 * Sh::kRowBytes;
-    const int lrow = lane / Sh::kCh, lslot = lane % Sh::kCh;
+    const int lrow = lane / Sh::kCh;
     // lane-constant offsets into a tile (see prefill.hip)
     const int vm = (lane % 16) / 4, va4 = lane % 4, vG = lane / 16;
     auto v_off = [&](int t, int key0) {
@@ -337,14 +375,21 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       const int dim = 32 * t + 16 * (vG % 2) + 4 * va4;
       return row * Sh::kRowBytes + 16 * ((dim / 8) ^ v_swz<Sh::kCh>(row)) + 2 * (dim % 8);
     };
-    int k_off[Sh::kKS], v_lo[Sh::kDB], v_hi[Sh::kDB];
+    // (the swizzles are XORs above the bits of s8 and t, so each offset is the
+    // first one XOR a constant: at D = 256, where 32 registers of offsets would
+    // be spilled, they are made where they are used)
+    constexpr bool kXor = D == 256;
+    int k_off[kXor ? 1 : Sh::kKS], v_lo[kXor ? 1 : Sh::kDB], v_hi[kXor ? 1 : Sh::kDB];
 #pragma unroll
-    for (int s8 = 0; s8 < Sh::kKS; ++s8) k_off[s8] = tile_off<D>(c, 2 * s8 + g);
+    for (int s8 = 0; s8 < (kXor ? 1 : Sh::kKS); ++s8) k_off[s8] = tile_off<D>(c, 2 * s8 + g);
 #pragma unroll
-    for (int t = 0; t < Sh::kDB; ++t) {
+    for (int t = 0; t < (kXor ? 1 : Sh::kDB); ++t) {
       v_lo[t] = v_off(t, 4 * g);
       v_hi[t] = v_off(t, 4 * g + 8);
     }
+    auto k_at = [&](int s8) { return kXor ? k_off[0] ^ (32 * s8) : k_off[s8 % Sh::kKS]; };
+    auto lo_at = [&](int t) { return kXor ? v_lo[0] ^ (64 * t) : v_lo[t]; };
+    auto hi_at = [&](int t) { return kXor ? v_hi[0] ^ (64 * t) : v_hi[t]; };
 
     const Seq s = w.seq();
     const Item item = ByRows::item(a, s, w.x);
@@ -370,10 +415,10 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     // keys the row sees: below s.prefix, and [lo, hi)
     const int32_t hi = a.causal ? min(pos + 1, s.L) : s.L, lo = pos - window + 1;
     // first and last position of the wave's rows and of the item's
-    const int32_t G = group(a);
-    const int32_t wp0 = s.off + min(r0, R - 1) / G, wp1 = s.off + min(r0 + 31, R - 1) / G;
-    const int32_t ip0 = s.off + w.x * kChRows / G,
-                  ip1 = s.off + min(w.x * kChRows + kChRows - 1, R - 1) / G;
+    const int32_t wp0 = s.off + token_of(a, min(r0, R - 1)),
+                  wp1 = s.off + token_of(a, min(r0 + 31, R - 1));
+    const int32_t ip0 = s.off + token_of(a, w.x * kChRows),
+                  ip1 = s.off + token_of(a, min(w.x * kChRows + kChRows - 1, R - 1));
     // whether rows at positions p0 .. p1 all see the 64 keys from k0 on
     auto all_see = [&](int32_t k0, int32_t p0, int32_t p1) {
       return k0 + kChTile <= s.prefix ||
@@ -387,36 +432,37 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 
     // ---- tile loads: wave w fills rows 16 w .. 16 w + 15 of K and V
     struct PageIds {
-      uint32_t id[kNI], slot[kNI];
+      uint32_t id[S16 ? 1 : kNI];
     };
     const uint32_t npages = div_page((uint32_t)s.L + a.S - 1u, a.page_rcp);
     const __attribute__((address_space(4))) int32_t* kv_idx =
         (const __attribute__((address_space(4))) int32_t*)(a.kv_indices + s.page0);
+    // (a page past the sequence reads the last one: its keys are masked)
     auto page_of = [&](int32_t tile) {
       const uint32_t key0 = (uint32_t)(tile * kChTile + 16 * wave);
       PageIds ph;
       if constexpr (S16) {  // the wave's 16 rows lie in one page
-        uint32_t p = div_page(key0, a.page_rcp);
-        p = p < npages ? p : npages - 1u;
-        ph.id[0] = (uint32_t)kv_idx[p];
-        ph.slot[0] = a.S == 32u ? key0 & 16u : 0u;
+        const uint32_t p = div_page(key0, a.page_rcp);
+        ph.id[0] = (uint32_t)kv_idx[p < npages ? p : npages - 1u];
       } else {
 #pragma unroll
         for (int i = 0; i < kNI; ++i) {
-          const uint32_t key = key0 + (uint32_t)(Sh::kRPI * i + lrow);
-          uint32_t p = div_page(key, a.page_rcp);
-          ph.slot[i] = key - p * a.S;
-          p = p < npages ? p : npages - 1u;
-          ph.id[i] = (uint32_t)a.kv_indices[s.page0 + p];
+          const uint32_t p = div_page(key0 + (uint32_t)(Sh::kRPI * i + lrow), a.page_rcp);
+          ph.id[i] = (uint32_t)a.kv_indices[s.page0 + (p < npages ? p : npages - 1u)];
         }
       }
       return ph;
     };
-    auto load_tile = [&](char* buf, const PageIds& ph) {
+    auto load_tile = [&](char* buf, const PageIds& ph, int32_t tile) {
+      int ln = lane;
+      if constexpr (kXor) asm volatile("" : "+v"(ln));  // (as the offsets above)
+      const int lrow = ln / Sh::kCh, lslot = ln % Sh::kCh;
+      const uint32_t key0 = (uint32_t)(tile * kChTile + 16 * wave);
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int tr = 16 * wave + Sh::kRPI * i + lrow;
-        const uint32_t slot = S16 ? ph.slot[0] + (uint32_t)(tr & 15) : ph.slot[i];
+        const uint32_t key = key0 + (uint32_t)(Sh::kRPI * i + lrow);
+        const uint32_t slot = S16 ? key & (a.S - 1u) : key - div_page(key, a.page_rcp) * a.S;
         const size_t e = elem_off(a.g, ph.id[S16 ? 0 : i], 0, hk, slot);
         load_lds16(a.kv + e + 8 * (lslot ^ k_swz<Sh::kCh>(tr)),
                    buf + (16 * wave + Sh::kRPI * i) * Sh::kRowBytes);
@@ -436,9 +482,9 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     auto vfrag = [&](const lds_char* sV, int t, int kk) {
       const int rows = kk * kRow16;
       const half4 x = __builtin_bit_cast(
-          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + v_lo[t] + rows)));
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + lo_at(t) + rows)));
       const half4 y = __builtin_bit_cast(
-          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + v_hi[t] + rows)));
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(sV + hi_at(t) + rows)));
       return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
@@ -512,16 +558,21 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     };
 
     auto tile = [&](const lds_char* sK, const lds_char* sV, int32_t k0) {
+      if constexpr (kXor) {
+        asm volatile("" : "+v"(k_off[0]));
+        asm volatile("" : "+v"(v_lo[0]));
+        asm volatile("" : "+v"(v_hi[0]));
+      }
       floatx16 acc_s[2];
       if constexpr (Sh::kKS <= 8) {
         half8 kf0[Sh::kKS], kf1[Sh::kKS];
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8)
-          kf0[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(sK + k_off[s8]);
+          kf0[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(sK + k_at(s8));
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8)
           kf1[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-              sK + k_off[s8] + 2 * kRow16);
+              sK + k_at(s8) + 2 * kRow16);
         __builtin_amdgcn_sched_barrier(0);
         acc_s[0] = floatx16{};
 #pragma unroll
@@ -535,7 +586,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 #pragma unroll
           for (int j = 0; j < kB; ++j)
             kf[j] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-                sK + k_off[(bt % (kNB / 2)) * kB + j] + (bt / (kNB / 2)) * 2 * kRow16);
+                sK + k_at((bt % (kNB / 2)) * kB + j) + (bt / (kNB / 2)) * 2 * kRow16);
         };
         half8 kfa[kB], kfb[kB];
         acc_s[0] = floatx16{};
@@ -647,7 +698,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     __syncthreads();  // the item before is done with the buffers
     PageIds ids{};
     if (t0 < t1) {
-      load_tile(s_buf0, page_of(item.tile(t0)));
+      load_tile(s_buf0, page_of(item.tile(t0)), item.tile(t0));
       if (t0 + 1 < t1) ids = page_of(item.tile(t0 + 1));
     }
     for (int32_t it = t0; it < t1; it += 2) {
@@ -659,7 +710,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (i + 1 < t1) {
-          load_tile(v == 0 ? s_buf1 : s_buf0, ids);
+          load_tile(v == 0 ? s_buf1 : s_buf0, ids, item.tile(i + 1));
           if (i + 2 < t1) ids = page_of(item.tile(i + 2));
         }
         const int32_t k0 = item.tile(i) * kChTile;
@@ -702,38 +753,18 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
   }
 }
 
-// Where the item that the border before workgroup w's share cuts begins and
-// ends: its parts are slot 1 of workgroup `first` and slot 0 of first + 1 ..
-// last.  False if the border cuts none, or it is not the item's first cut.
-template <class By>
-__device__ inline bool seek_cut(Walk<By>& w, uint32_t place, uint32_t workgroups, uint32_t least,
-                                uint32_t& last) {
-  const uint64_t per_head = w.total(), units = per_head * w.a.H;
-  const uint64_t share = share_of(units, workgroups, least);
-  const uint64_t u = place * share;
-  if (u >= units) return false;
-  w.seek(u, per_head);
-  if (w.at == 0u || w.at > share) return false;  // (at == share: begins where the share before does)
-  const Item item = By::item(w.a, w.seq(), w.x);
-  last = (uint32_t)((u - w.at + (uint32_t)item.count + kItemUnits - 1u) / share);
-  return true;
-}
-
 // Joins an item's parts: workgroup (w, sub) takes 32 of its rows, a thread one
 // row and D / 8 dims.
 template <int D>
-__global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a, uint32_t workgroups) {
-  __shared__ PlanLds s_plan;
-  Walk<ByRows> w(a, s_plan);
+__global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
   const uint32_t place = blockIdx.x / 4u + 1u, sub = blockIdx.x % 4u;
-  uint32_t last = 0u;
-  if (!seek_cut(w, place, workgroups, kAttnLeast, last)) return;
-  const Seq s = w.seq();
+  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[place];
+  if (cut.last == 0u) return;
   const int32_t r = (int32_t)(sub * 32u + threadIdx.x % 32u);
-  if (w.x * kChRows + r >= s.n * group(a)) return;
-  const Row row = row_of(a, w.h, w.x * kChRows + r);
+  if (cut.x * kChRows + r >= cut.n * group(a)) return;
+  const Row row = row_of(a, cut.h, cut.x * kChRows + r);
   const uint32_t j0 = threadIdx.x / 32u;
-  const uint32_t n = last - place + 2u;
+  const uint32_t n = cut.last - place + 2u;
   auto part = [&](uint32_t i) {
     return a.parts + (2u * (size_t)(place - 1u + i) + (i == 0u ? 1u : 0u)) * part_floats(D);
   };
@@ -755,7 +786,7 @@ __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a, uin
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const size_t at = (size_t)(s.q0 + row.tok) * a.Hq + row.h;
+  const size_t at = (size_t)(cut.q0 + row.tok) * a.Hq + row.h;
   f16* o = a.o + at * D + 4 * kV * j0;
 #pragma unroll
   for (int v = 0; v < kV; ++v)
@@ -816,11 +847,15 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
 
   Walk<ByKeys> w(a, s_plan);
   const uint64_t per_head = w.total(), units = per_head * a.H;
-  const uint64_t share = share_of(units, gridDim.x, kSumsLeast);
+  const uint64_t share = share_of(a, units, kSumsLeast);
   uint64_t u = list_place() * share;
   const uint64_t u1 = min(u + share, units);
-  if (u >= u1) return;
+  if (u >= u1) {
+    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
+    return;
+  }
   w.seek(u, per_head);
+  if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
 
   constexpr int kNI = 16 / Sh::kRPI;
   constexpr int kRow32 = 32 * Sh::kRowBytes;
@@ -896,8 +931,8 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int32_t rh = r0 + 32 * half;
-          const int32_t p0 = s.off + min(rh, R - 1) / group(a),
-                        p1 = s.off + min(rh + 31, R - 1) / group(a);
+          const int32_t p0 = s.off + token_of(a, min(rh, R - 1)),
+                        p1 = s.off + token_of(a, min(rh + 31, R - 1));
           // none of the wave's keys is seen, or all by all rows
           if (rh >= R || (k0 >= s.prefix && ((a.causal && k0 > p1) || p0 - (k0 + 31) >= window)))
             continue;
@@ -962,16 +997,14 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
 }
 
 // Joins an item's parts: a thread per key.
-__global__ __launch_bounds__(kChThreads) void weights_join_kernel(ChunkArgs a, uint32_t workgroups) {
-  __shared__ PlanLds s_plan;
-  Walk<ByKeys> w(a, s_plan);
+__global__ __launch_bounds__(kChRows) void weights_join_kernel(ChunkArgs a) {
   const uint32_t place = blockIdx.x + 1u;
-  uint32_t last = 0u;
-  if (!seek_cut(w, place, workgroups, kSumsLeast, last)) return;
-  if (threadIdx.x >= (uint32_t)kChRows) return;
+  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[place];
+  if (cut.last == 0u) return;
   float sum = a.parts[(2u * (size_t)(place - 1u) + 1u) * kChRows + threadIdx.x];
-  for (uint32_t i = place; i <= last; ++i) sum += a.parts[2u * (size_t)i * kChRows + threadIdx.x];
-  store_weight(a, w.seq(), w.b, w.h, w.x * kChRows + (int32_t)threadIdx.x, sum);
+  for (uint32_t i = place; i <= cut.last; ++i)
+    sum += a.parts[2u * (size_t)i * kChRows + threadIdx.x];
+  store_weight(a, load_seq(a, cut.b), cut.b, cut.h, cut.x * kChRows + (int32_t)threadIdx.x, sum);
 }
 
 // Workgroups of a call: those that fit on the chip at once, fewer where the
@@ -984,6 +1017,21 @@ uint32_t workgroups(const ChunkArgs& a, uint64_t items, uint64_t tiles, uint32_t
   return (uint32_t)((m + kXcds - 1u) / kXcds * kXcds);
 }
 
+// The factors that divide by the page size, the group and n workgroups; the
+// workspace holds the cuts, then the parts.
+ChunkArgs with_rcps(const ChunkArgs& args, uint32_t n) {
+  ChunkArgs a = args;
+  a.G = a.Hq / a.H;
+  a.page_rcp = a.S == 1u ? 0u : (uint32_t)((1ull << 32) / a.S) + 1u;
+  // (a sequence's last item reaches 127 rows past its own)
+  a.group_rcp = a.G > 1u && ((uint64_t)a.T * a.G + kChRows) * a.G < (1ull << 32)
+                    ? (uint32_t)((1ull << 32) / a.G) + 1u
+                    : 0u;
+  a.share_rcp = 1.0 / (double)n;
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(a.cuts) + kCutBytes);
+  return a;
+}
+
 template <int D, int MOD>
 hipError_t launch_attn(const ChunkArgs& a, uint32_t n, hipStream_t s) {
   if (a.S % 16u == 0u)
@@ -994,11 +1042,12 @@ hipError_t launch_attn(const ChunkArgs& a, uint32_t n, hipStream_t s) {
 }
 
 template <int D>
-hipError_t launch_attn(const ChunkArgs& a, hipStream_t s) {
-  const uint64_t G = a.Hq / a.H;
-  const uint32_t n = workgroups(a, (a.T * G) / kChRows + a.B,
-                                ((uint64_t)a.max_pages * a.S) / kChTile + 2u,
+hipError_t launch_attn(const ChunkArgs& args, hipStream_t s) {
+  const uint64_t G = args.Hq / args.H;
+  const uint32_t n = workgroups(args, (args.T * G) / kChRows + args.B,
+                                ((uint64_t)args.max_pages * args.S) / kChTile + 2u,
                                 kCus * attn_per_cu<D>(), kAttnLeast);
+  const ChunkArgs a = with_rcps(args, n);
   hipError_t e = hipSuccess;
   switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
     case 0: e = launch_attn<D, 0>(a, n, s); break;
@@ -1007,15 +1056,17 @@ hipError_t launch_attn(const ChunkArgs& a, hipStream_t s) {
     default: e = launch_attn<D, kCap | kBias>(a, n, s); break;
   }
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a, n);
+  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a);
   return hipGetLastError();
 }
 
 template <int D>
-hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
-  const uint64_t G = a.Hq / a.H;
-  const uint32_t n = workgroups(a, (uint64_t)a.B * (((uint64_t)a.max_pages * a.S) / kChRows + 1u),
-                                (a.T * G) / kChTile + 2u, kCus * kSumsPerCu, kSumsLeast);
+hipError_t launch_sums(const ChunkArgs& args, hipStream_t s) {
+  const uint64_t G = args.Hq / args.H;
+  const uint32_t n = workgroups(
+      args, (uint64_t)args.B * (((uint64_t)args.max_pages * args.S) / kChRows + 1u),
+      (args.T * G) / kChTile + 2u, kCus * kSumsPerCu, kSumsLeast);
+  const ChunkArgs a = with_rcps(args, n);
   const dim3 grid(n), block(kChThreads);
   switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
     case 0: hipLaunchKernelGGL((attn_weights_kernel<D, 0>), grid, block, 0, s, a); break;
@@ -1026,26 +1077,21 @@ hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
       break;
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  hipLaunchKernelGGL(weights_join_kernel, dim3(n - 1u), block, 0, s, a, n);
+  hipLaunchKernelGGL(weights_join_kernel, dim3(n - 1u), dim3(kChRows), 0, s, a);
   return hipGetLastError();
-}
-
-ChunkArgs with_rcp(const ChunkArgs& args) {
-  ChunkArgs a = args;
-  a.page_rcp = a.S == 1u ? 0u : (uint32_t)((1ull << 32) / a.S) + 1u;
-  return a;
 }
 
 }  // namespace
 
 size_t chunk_attn_workspace(uint32_t head_dim) {
   const size_t per_cu = head_dim == 256u ? attn_per_cu<256>() : attn_per_cu<128>();
-  return 2u * kCus * per_cu * part_floats((int)head_dim) * sizeof(float);
+  return kCutBytes + 2u * kCus * per_cu * part_floats((int)head_dim) * sizeof(float);
 }
-size_t attn_weights_workspace() { return 2u * kCus * kSumsPerCu * kChRows * sizeof(float); }
+size_t attn_weights_workspace() {
+  return kCutBytes + 2u * kCus * kSumsPerCu * kChRows * sizeof(float);
+}
 
-hipError_t launch_chunk_attn(const ChunkArgs& args, uint32_t head_dim, hipStream_t s) {
-  const ChunkArgs a = with_rcp(args);
+hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s) {
   switch (head_dim) {
     case 64: return launch_attn<64>(a, s);
     case 128: return launch_attn<128>(a, s);
@@ -1053,8 +1099,7 @@ hipError_t launch_chunk_attn(const ChunkArgs& args, uint32_t head_dim, hipStream
   }
 }
 
-hipError_t launch_attn_weights(const ChunkArgs& args, uint32_t head_dim, hipStream_t s) {
-  const ChunkArgs a = with_rcp(args);
+hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s) {
   switch (head_dim) {
     case 64: return launch_sums<64>(a, s);
     case 128: return launch_sums<128>(a, s);

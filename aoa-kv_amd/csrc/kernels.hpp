@@ -295,8 +295,12 @@ struct ChunkArgs {
   float sm_scale, soft_cap;   // soft_cap 0: none
   PageGeom g;
   uint32_t* error;            // receives kErrTruncated, or nullptr
-  float* parts;               // the workspace: two slots per workgroup
-  uint32_t page_rcp;          // (set by the launch) divides by S
+  void* cuts;                 // the workspace
+  // set by the launch: the workspace's two slots per workgroup, the group's
+  // heads, the factors that divide by S, G and the workgroups
+  float* parts;
+  uint32_t G, page_rcp, group_rcp;
+  double share_rcp;
 };
 // Tokens of a sequence's table at most: positions are divided by the page size
 // as x * (2^32 / S + 1) >> 32, exact for x * S < 2^32.
