@@ -1047,6 +1047,10 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   REQUIRE((uint64_t)num_q_tokens * (num_qo_heads / num_kv_heads) < (1ull << 30),
           "%s: too many rows (%u x %u query heads per kv head)", fn, num_q_tokens,
           num_qo_heads / num_kv_heads);
+  const uint64_t group = num_qo_heads / num_kv_heads;
+  REQUIRE((group & (group - 1u)) == 0u || (num_q_tokens + 128ull) * group * group < (1ull << 31),
+          "%s: too many rows (%u) for groups of %u query heads", fn, num_q_tokens,
+          (uint32_t)group);
   REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size <= aoakv::kMaxChunkTokens,
           "%s: max_pages %u of %u tokens not in [1, 2^27 tokens]", fn, max_pages, page_size);
   REQUIRE(window < (1u << 31), "%s: window %u out of range", fn, window);

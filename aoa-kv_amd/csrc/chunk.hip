@@ -33,7 +33,7 @@ namespace aoakv {
 namespace {
 
 constexpr uint32_t kChThreads = 256;
-constexpr int32_t kChRows = 128;  // rows (attention) or keys (weights) of an item
+constexpr int32_t kChRows = 128;  // rows of an item (attention)
 constexpr int32_t kChTile = 64;   // keys (attention) or rows (weights) of a tile
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kItemUnits = 1u;
@@ -73,11 +73,10 @@ struct Item {
 };
 
 __device__ inline int32_t group(const ChunkArgs& a) { return (int32_t)a.G; }
-// r / G of a packed row (group_rcp = floor(2^32 / G) + 1 where that divides
-// every row of the call exactly, else 0)
+// r / G of a packed row (group_rcp = ceil(2^31 / G): exact for powers of two, and
+// for r * G < 2^31; r < 2^30)
 __device__ inline int32_t token_of(const ChunkArgs& a, int32_t r) {
-  if (a.G == 1u) return r;
-  return a.group_rcp != 0u ? (int32_t)__umulhi((uint32_t)r, a.group_rcp) : r / (int32_t)a.G;
+  return (int32_t)__umulhi(2u * (uint32_t)r, a.group_rcp);
 }
 __device__ inline int32_t div_up(int32_t x, int32_t y) { return (x + y - 1) / y; }
 
@@ -96,17 +95,18 @@ struct ByRows {
     return Item{pe, lt, pe + max(he - lt, 0)};
   }
 };
-// Items of 128 keys, tiles of 64 rows.
+// Items of KEYS keys, tiles of ROWS rows.
+template <int32_t KEYS, int32_t ROWS>
 struct ByKeys {
-  static __device__ int32_t items(const ChunkArgs& a, const Seq& s) { return div_up(s.L, kChRows); }
+  static __device__ int32_t items(const ChunkArgs& a, const Seq& s) { return div_up(s.L, KEYS); }
   static __device__ Item item(const ChunkArgs& a, const Seq& s, int32_t x) {
-    const int32_t k0 = x * kChRows;
+    const int32_t k0 = x * KEYS;
     int32_t i0 = 0, i1 = s.n;
     if (k0 >= s.prefix) {
       if (a.causal) i0 = min(max(k0 - s.off, 0), s.n);
-      if (a.window != 0u) i1 = min(max((int32_t)a.window + k0 + kChRows - 1 - s.off, 0), s.n);
+      if (a.window != 0u) i1 = min(max((int32_t)a.window + k0 + KEYS - 1 - s.off, 0), s.n);
     }
-    const int32_t G = group(a), t0 = i0 * G / kChTile, t1 = div_up(i1 * G, kChTile);
+    const int32_t G = group(a), t0 = i0 * G / ROWS, t1 = div_up(i1 * G, ROWS);
     return Item{0, t0, i1 > i0 ? t1 - t0 : 0};
   }
 };
@@ -297,7 +297,7 @@ __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kChRows
 template <int D>
 constexpr uint32_t attn_per_cu() { return D == 256 ? 1u : 2u; }
 constexpr uint32_t kCus = 256u;
-constexpr size_t kCutBytes = kCus * 2u * sizeof(Cut);  // (2 workgroups per CU at most)
+constexpr size_t kCutBytes = kCus * 4u * sizeof(Cut);  // (4 workgroups per CU at most)
 constexpr uint32_t kAttnLeast = 4u;  // units of a share at least
 
 // Row r of a sequence's packed rows.
@@ -627,14 +627,16 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           }
       }
       if (!all_see(k0, wp0, wp1)) {
-        const int32_t first = k0 + 4 * g, pre = s.prefix - first, end = hi - first,
-                      begin = lo - first;
+        // (one unsigned comparison for the range, one for the prefix)
+        const int32_t first = k0 + 4 * g, pre = s.prefix - first;
+        const uint32_t begin = (uint32_t)(lo - first), span = (uint32_t)max(hi - lo, 0);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int32_t key = ks * 32 + crow(i, 0);
-            acc_s[ks][i] = key < pre || (key < end && key >= begin) ? acc_s[ks][i] : -INFINITY;
+            const bool see = (int)(key < pre) | (int)((uint32_t)key - begin < span);
+            acc_s[ks][i] = see ? acc_s[ks][i] : -INFINITY;
           }
       }
       float mt = acc_s[0][0];
@@ -797,7 +799,6 @@ __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
 }
 
 // ---------------------------------------------------------------- weights
-constexpr uint32_t kSumsPerCu = 2u;
 constexpr uint32_t kSumsLeast = 4u;
 
 // tanh(y): near 0, where 1 - 2 / (e^2y + 1) has no relative precision left, the
@@ -824,40 +825,74 @@ __device__ inline void store_weight(const ChunkArgs& a, const Seq& s, uint32_t b
   *w = (j < start ? *w : 0.f) + sum;
 }
 
-// One workgroup's share of the items of 128 keys.  Scores are S = Q K^T: a wave
-// holds 32 keys as B operands in registers (lane l: key l % 32) and reads 64
-// query rows at a time from LDS, so a key's sum is a sum over a lane's own
-// registers.  Each 32 rows are added up by themselves first: one chain of
+// position of a row that counts nothing (no row of the call, or one that sees no
+// key): outside of every range of positions
+constexpr int32_t kNoPos = INT32_MIN;
+
+// How the weights are cut.  BIG, where a sequence has many rows: a wave holds 2 x
+// 32 keys (64 registers at D = 128; each halves the reads of query rows per
+// product), tiles of 128 rows, two workgroups per CU.  Else the keys' own way
+// from memory is what takes the time: 32 keys, tiles of 32 rows, and four
+// workgroups per CU with their keys in flight.
+template <int D, bool BIG>
+struct SumShape {
+  static constexpr int kSets = BIG && D != 256 ? 2 : 1;  // of 32 keys per wave
+  static constexpr int32_t kKeys = 4 * 32 * kSets;       // of an item
+  static constexpr int32_t kRows = BIG ? (D == 256 ? 64 : 128) : 32;  // of a tile
+  static constexpr uint32_t kPerCu = BIG ? 2u : D == 256 ? 3u : 4u;   // workgroups
+};
+constexpr int32_t kMostKeys = 256;
+constexpr uint32_t kMostSums = 4u;
+constexpr uint32_t kWholeTiles = 4u;
+
+// One workgroup's share of the items.  Scores are S = Q K^T: a wave holds its
+// keys in registers (lane l: keys l % 32, + 32) and reads 32 query rows at a time
+// from LDS, so a key's sum is a sum over a lane's own registers.  Each 32 rows are added up by themselves first: one chain of
 // single additions over 16384 rows was 2e-6 off.
-template <int D, int MOD>
-__global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(ChunkArgs a) {
+template <int D, int MOD, bool BIG>
+__global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_weights_kernel(
+    ChunkArgs a) {
   using Sh = PfShape<D>;
-  __shared__ __attribute__((aligned(16))) char s_q0[Sh::kTileBytes];
-  __shared__ __attribute__((aligned(16))) char s_q1[Sh::kTileBytes];
+  using Cut_ = SumShape<D, BIG>;
+  constexpr int32_t kRows = Cut_::kRows;
+  __shared__ __attribute__((aligned(16))) char s_q0[kRows * Sh::kRowBytes];
+  __shared__ __attribute__((aligned(16))) char s_q1[kRows * Sh::kRowBytes];
   // of a tile's rows: -lse in units of log 2 (-inf: the row counts nothing),
   // position, slope
-  __shared__ __attribute__((aligned(16))) float s_neg[2][kChTile];
-  __shared__ __attribute__((aligned(16))) int32_t s_pos[2][kChTile];
-  __shared__ __attribute__((aligned(16))) float s_slope[2][kChTile];
+  __shared__ __attribute__((aligned(16))) float s_neg[2][kRows];
+  __shared__ __attribute__((aligned(16))) int32_t s_pos[2][kRows];
+  __shared__ __attribute__((aligned(16))) float s_slope[2][kRows];
   __shared__ PlanLds s_plan;
   const int tid = threadIdx.x;
   const int lane = (int)__lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int g = lane / 32, c = lane % 32;
 
-  Walk<ByKeys> w(a, s_plan);
+  constexpr int kSets = Cut_::kSets;
+  constexpr int32_t kKeys = Cut_::kKeys;
+  using By = ByKeys<kKeys, kRows>;
+  Walk<By> w(a, s_plan);
   const uint64_t per_head = w.total(), units = per_head * a.H;
   const uint64_t share = share_of(a, units, kSumsLeast);
   uint64_t u = list_place() * share;
   const uint64_t u1 = min(u + share, units);
   if (u >= u1) {
-    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
+    if (tid == 0 && !a.whole) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
     return;
   }
   w.seek(u, per_head);
-  if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
+  if (a.whole) {  // the items that begin in the share, whole
+    if (w.at != 0u) {
+      u += (uint32_t)By::item(a, w.seq(), w.x).count + kItemUnits - w.at;
+      if (u >= u1) return;
+      w.next();
+    }
+  } else if (tid == 0) {
+    reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
+  }
 
-  constexpr int kNI = 16 / Sh::kRPI;
+  constexpr int kWaveRows = kRows / 4;  // rows that a wave loads
+  constexpr int kNI = kWaveRows / Sh::kRPI;
   constexpr int kRow32 = 32 * Sh::kRowBytes;
   const int lrow = lane / Sh::kCh, lslot = lane % Sh::kCh;
   int q_off[Sh::kKS];
@@ -870,50 +905,179 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
 
   for (;;) {
     const Seq s = w.seq();
-    const Item item = ByKeys::item(a, s, w.x);
+    const Item item = By::item(a, s, w.x);
     const uint32_t hk = w.h;
     const uint32_t ue = (uint32_t)item.count + kItemUnits;
-    const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
+    const uint32_t ua = w.at, ub = a.whole ? ue : (uint32_t)min((uint64_t)ue, ua + (u1 - u));
     const int32_t t0 = max((int32_t)(ua - kItemUnits), 0), t1 = max((int32_t)(ub - kItemUnits), 0);
     const int32_t R = s.n * group(a);
-    const int32_t k0 = w.x * kChRows + wave * 32;  // the wave's first key
-    const int32_t key = k0 + c;
+    constexpr int32_t kWaveKeys = 32 * kSets;
+    const int32_t k0 = w.x * kKeys + wave * kWaveKeys;  // the wave's first key
 
-    half8 kf[Sh::kKS];
-    {
-      const uint32_t j = (uint32_t)min(key, s.L - 1), p = div_page(j, a.page_rcp);
+    half8 kf[kSets][Sh::kKS];
+#pragma unroll
+    for (int z = 0; z < kSets; ++z) {
+      const uint32_t j = (uint32_t)min(k0 + 32 * z + c, s.L - 1), p = div_page(j, a.page_rcp);
       const uint32_t page = (uint32_t)a.kv_indices[s.page0 + p];
       const f16* k = a.kv + elem_off(a.g, page, 0, hk, j - p * a.S) + 8 * g;
 #pragma unroll
-      for (int s8 = 0; s8 < Sh::kKS; ++s8) kf[s8] = *reinterpret_cast<const half8*>(k + 16 * s8);
+      for (int s8 = 0; s8 < Sh::kKS; ++s8) kf[z][s8] = *reinterpret_cast<const half8*>(k + 16 * s8);
     }
 
+    // row r of the packed rows lies at r * D + token * (Hq - G) * D of this
+    const f16* q0 = a.q + ((size_t)s.q0 * a.Hq + (size_t)hk * a.G) * D;
+    const uint32_t tok_step = (a.Hq - a.G) * D;
     auto load_tile = [&](char* buf, int32_t tile) {
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
-        const int tr = 16 * wave + Sh::kRPI * i + lrow;
-        const Row row = row_of(a, hk, min(tile * kChTile + tr, R - 1));
-        const f16* q = a.q + ((size_t)(s.q0 + row.tok) * a.Hq + row.h) * D;
-        load_lds16(q + 8 * (lslot ^ k_swz<Sh::kCh>(tr)),
-                   buf + (16 * wave + Sh::kRPI * i) * Sh::kRowBytes);
+        const int tr = kWaveRows * wave + Sh::kRPI * i + lrow;
+        const int32_t r = min(tile * kRows + tr, R - 1);
+        load_lds16(q0 + (size_t)(uint32_t)r * D + (size_t)(uint32_t)token_of(a, r) * tok_step +
+                       8 * (lslot ^ k_swz<Sh::kCh>(tr)),
+                   buf + (kWaveRows * wave + Sh::kRPI * i) * Sh::kRowBytes);
       }
     };
-    auto load_rows = [&](int v, int32_t tile) {
-      if (tid < kChTile) {
-        const int32_t r = tile * kChTile + tid;
+    // what s_neg, s_pos and s_slope get: fetched a tile ahead, stored after the
+    // tile before it is done (waiting for them no earlier)
+    struct RowData {
+      float lse, slope;
+      int32_t pos;
+      bool live;
+    };
+    auto fetch_row = [&](int32_t tile) {
+      RowData d{};
+      if (tid < kRows) {
+        const int32_t r = tile * kRows + tid;
         const Row row = row_of(a, hk, min(r, R - 1));
-        const float lse = a.lse[(size_t)(s.q0 + row.tok) * a.Hq + row.h];
-        s_neg[v][tid] = r < R && lse != -INFINITY ? -lse * kLog2e : -INFINITY;
-        s_pos[v][tid] = s.off + row.tok;
-        if constexpr (MOD & kBias) s_slope[v][tid] = a.slopes[row.h] * kLog2e;
+        d.lse = a.lse[(size_t)(s.q0 + row.tok) * a.Hq + row.h];
+        if constexpr (MOD & kBias) d.slope = a.slopes[row.h];
+        d.pos = s.off + row.tok;
+        d.live = r < R;
+      }
+      return d;
+    };
+    auto store_rows = [&](int v, const RowData& d) {
+      if (tid < kRows) {
+        const bool counts = d.live && d.lse != -INFINITY;
+        s_neg[v][tid] = counts ? -d.lse * kLog2e : -INFINITY;
+        s_pos[v][tid] = counts ? d.pos : kNoPos;
+        if constexpr (MOD & kBias) s_slope[v][tid] = d.slope * kLog2e;
+      }
+    };
+    // rows 32 half .. + 31 of a tile: their query fragments, -lse, and what MOD
+    // and the masks need
+    struct Rows {
+      float neg[16], slope[16];
+      int32_t pos[16];
+    };
+    auto read_q = [&](const lds_char* sQ, int half, half8 (&q)[Sh::kKS]) {
+#pragma unroll
+      for (int s8 = 0; s8 < Sh::kKS; ++s8)
+        q[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+            sQ + q_off[s8] + half * kRow32);
+    };
+    auto read_rows = [&](int v, int half, Rows& x, bool pos) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int at = 32 * half + 8 * q4 + 4 * g;  // rows crow(4 q4, g) ..
+        const float4 n = *reinterpret_cast<const float4*>(&s_neg[v][at]);
+        x.neg[4 * q4] = n.x, x.neg[4 * q4 + 1] = n.y, x.neg[4 * q4 + 2] = n.z,
+        x.neg[4 * q4 + 3] = n.w;
+        if (MOD & kBias || pos) {
+          const int4 y = *reinterpret_cast<const int4*>(&s_pos[v][at]);
+          x.pos[4 * q4] = y.x, x.pos[4 * q4 + 1] = y.y, x.pos[4 * q4 + 2] = y.z,
+          x.pos[4 * q4 + 3] = y.w;
+        }
+        if constexpr (MOD & kBias) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_slope[v][at]);
+          x.slope[4 * q4] = y.x, x.slope[4 * q4 + 1] = y.y, x.slope[4 * q4 + 2] = y.z,
+          x.slope[4 * q4 + 3] = y.w;
+        }
+      }
+    };
+    // probability of register i of a product
+    auto weight = [&](float t, const Rows& x, int i, int32_t key) {
+      if constexpr (MOD & kCap) t = cap2 * tanh_f32(t * cap_in);
+      else if constexpr (MOD != 0) t *= a.sm_scale * kLog2e;
+      if constexpr (MOD & kBias)
+        t = __builtin_fmaf(-x.slope[i], __builtin_fabsf((float)(x.pos[i] - key)), t);
+      return __builtin_amdgcn_exp2f(__builtin_fmaf(t, scale, x.neg[i]));
+    };
+    float sum[kSets] = {};
+    // A tile that the wave's keys are seen by whole.  The products of 32 rows and
+    // a set of keys follow each other, and the exponentials of one are issued
+    // between the matrix instructions of the next (held there by the scheduling
+    // barriers): with all products first, the two waves of a SIMD did the same
+    // thing at the same time and neither unit was busy more than half.
+    auto whole_tile = [&](const lds_char* sQ, int v) {
+      constexpr int kPer = 16 / Sh::kKS;  // elements per matrix instruction
+      constexpr int kN = kRows / 32 * kSets;  // products
+      half8 q[2][Sh::kKS];
+      Rows x;
+      read_q(sQ, 0, q[0]);
+      floatx16 acc[2];
+      float part = 0.f;
+#pragma unroll
+      for (int n = 0; n <= kN; ++n) {  // product n, exponentials of product n - 1
+        const int half = n / kSets, z = n % kSets, pz = (n + kSets - 1) % kSets;
+        if (n < kN && z == 0 && half + 1 < kRows / 32) read_q(sQ, half + 1, q[(half + 1) % 2]);
+        if (n > 0 && pz == 0) read_rows(v, (n - 1) / kSets, x, false);
+        if (n < kN) acc[n % 2] = floatx16{};
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8) {
+          if (n < kN) acc[n % 2] = mfma32(q[half % 2][s8], kf[z][s8], acc[n % 2]);
+          if (n > 0) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+              part += weight(acc[(n + 1) % 2][s8 * kPer + e], x, s8 * kPer + e,
+                             k0 + 32 * pz + c);
+          }
+          if (n > 0 && n < kN) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (n > 0) {
+          sum[pz] += part;
+          part = 0.f;
+        }
+      }
+    };
+    // ... or in part: a key is seen from a range of positions (one subtraction and
+    // one unsigned comparison per element; a chain of && became branches here and
+    // took 30 us per tile)
+    auto masked_half = [&](const lds_char* sQ, int v, int half, int32_t p0, int32_t p1) {
+      half8 q[Sh::kKS];
+      Rows x;
+      read_q(sQ, half, q);
+      read_rows(v, half, x, true);
+#pragma unroll
+      for (int z = 0; z < kSets; ++z) {
+        const int32_t kz = k0 + 32 * z;  // (none of these keys is seen)
+        if (kz >= s.prefix && ((a.causal && kz > p1) || p0 - (kz + 31) >= window)) continue;
+        floatx16 acc = floatx16{};
+#pragma unroll
+        for (int s8 = 0; s8 < Sh::kKS; ++s8) acc = mfma32(q[s8], kf[z][s8], acc);
+        const int32_t key = kz + c;
+        const int32_t from = key >= s.L                      ? INT32_MAX
+                             : key < s.prefix || !a.causal ? kNoPos + 1
+                                                             : key;
+        const int32_t to = key >= s.L ? INT32_MAX
+                           : key < s.prefix ? INT32_MAX
+                                            : key + (window - 1);
+        const uint32_t span = (uint32_t)to - (uint32_t)from;
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = weight(acc[i], x, i, key);
+          part += (uint32_t)x.pos[i] - (uint32_t)from <= span ? p : 0.f;
+        }
+        sum[z] += part;
       }
     };
 
-    float sum = 0.f;
     __syncthreads();  // the item before is done with the buffers
     if (t0 < t1) {
+      const RowData d = fetch_row(item.tile(t0));
       load_tile(s_q0, item.tile(t0));
-      load_rows(0, item.tile(t0));
+      store_rows(0, d);
     }
     for (int32_t it = t0; it < t1; it += 2) {
 #pragma unroll
@@ -923,72 +1087,41 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
         const lds_char* sQ = (const lds_char*)(v == 0 ? s_q0 : s_q1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        RowData next{};
         if (i + 1 < t1) {
+          next = fetch_row(item.tile(i + 1));
           load_tile(v == 0 ? s_q1 : s_q0, item.tile(i + 1));
-          load_rows(v ^ 1, item.tile(i + 1));
         }
-        const int32_t r0 = item.tile(i) * kChTile;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int32_t rh = r0 + 32 * half;
-          const int32_t p0 = s.off + token_of(a, min(rh, R - 1)),
-                        p1 = s.off + token_of(a, min(rh + 31, R - 1));
-          // none of the wave's keys is seen, or all by all rows
-          if (rh >= R || (k0 >= s.prefix && ((a.causal && k0 > p1) || p0 - (k0 + 31) >= window)))
-            continue;
-          const bool all = rh + 32 <= R && k0 + 32 <= s.L &&
-                           (k0 + 32 <= s.prefix ||
-                            ((!a.causal || k0 + 31 <= p0) && p1 - k0 < window));
-          floatx16 acc = floatx16{};
-          half8 qf[Sh::kKS];
-#pragma unroll
-          for (int s8 = 0; s8 < Sh::kKS; ++s8)
-            qf[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-                sQ + q_off[s8] + half * kRow32);
-#pragma unroll
-          for (int s8 = 0; s8 < Sh::kKS; ++s8) acc = mfma32(qf[s8], kf[s8], acc);
-          float part = 0.f;
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int at = 32 * half + 8 * q4 + 4 * g;  // rows crow(4 q4, g) ..
-            const float4 neg = *reinterpret_cast<const float4*>(&s_neg[v][at]);
-            const float ng[4] = {neg.x, neg.y, neg.z, neg.w};
-            int32_t ps[4] = {};
-            if (MOD & kBias || !all) {
-              const int4 x = *reinterpret_cast<const int4*>(&s_pos[v][at]);
-              ps[0] = x.x, ps[1] = x.y, ps[2] = x.z, ps[3] = x.w;
-            }
-            float sl[4] = {};
-            if constexpr (MOD & kBias) {
-              const float4 x = *reinterpret_cast<const float4*>(&s_slope[v][at]);
-              sl[0] = x.x, sl[1] = x.y, sl[2] = x.z, sl[3] = x.w;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float t = acc[4 * q4 + e];
-              if constexpr (MOD & kCap) t = cap2 * tanh_f32(t * cap_in);
-              else if constexpr (MOD != 0) t *= a.sm_scale * kLog2e;
-              if constexpr (MOD & kBias)
-                t = __builtin_fmaf(-sl[e], __builtin_fabsf((float)(ps[e] - key)), t);
-              float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t, scale, ng[e]));
-              if (!all) {
-                const bool see =
-                    key < s.L && ng[e] != -INFINITY &&
-                    (key < s.prefix || ((!a.causal || key <= ps[e]) && ps[e] - key < window));
-                p = see ? p : 0.f;
-              }
-              part += p;
-            }
+        // the tile's rows at positions p0 .. p1: all see all of the wave's keys,
+        // or some see some
+        const int32_t r0 = item.tile(i) * kRows;
+        const int32_t p0 = s.off + token_of(a, r0),
+                      p1 = s.off + token_of(a, min(r0 + kRows - 1, R - 1));
+        if (r0 + kRows <= R && k0 + kWaveKeys <= s.L &&
+            (k0 + kWaveKeys <= s.prefix ||
+             ((!a.causal || k0 + kWaveKeys - 1 <= p0) && p1 - k0 < window))) {
+          whole_tile(sQ, v);
+        } else if (k0 < s.prefix ||
+                   ((!a.causal || k0 <= p1) && p0 - (k0 + kWaveKeys - 1) < window)) {
+#pragma nounroll
+          for (int half = 0; half < kRows / 32; ++half) {
+            const int32_t rh = r0 + 32 * half;
+            if (rh >= R) break;
+            masked_half(sQ, v, half, s.off + token_of(a, rh),
+                        s.off + token_of(a, min(rh + 31, R - 1)));
           }
-          sum += part;
         }
+        if (i + 1 < t1) store_rows(v ^ 1, next);
       }
     }
-    sum = pair_sum(sum);
-    if (ua == 0u && ub == ue) {
-      if (g == 0) store_weight(a, s, w.b, hk, key, sum);
-    } else if (g == 0) {
-      a.parts[(2u * (size_t)list_place() + (ua == 0u ? 1u : 0u)) * kChRows + wave * 32 + c] = sum;
+    float* part =
+        a.parts + (2u * (size_t)list_place() + (ua == 0u ? 1u : 0u)) * kMostKeys + wave * kWaveKeys;
+#pragma unroll
+    for (int z = 0; z < kSets; ++z) {
+      const float x = pair_sum(sum[z]);
+      if (g != 0) continue;
+      if (ua == 0u && ub == ue) store_weight(a, s, w.b, hk, k0 + 32 * z + c, x);
+      else part[32 * z + c] = x;
     }
     u += ub - ua;
     if (u >= u1) return;
@@ -997,14 +1130,15 @@ __global__ __launch_bounds__(kChThreads, kSumsPerCu) void attn_weights_kernel(Ch
 }
 
 // Joins an item's parts: a thread per key.
-__global__ __launch_bounds__(kChRows) void weights_join_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(kMostKeys) void weights_join_kernel(ChunkArgs a) {
   const uint32_t place = blockIdx.x + 1u;
   const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[place];
   if (cut.last == 0u) return;
-  float sum = a.parts[(2u * (size_t)(place - 1u) + 1u) * kChRows + threadIdx.x];
+  float sum = a.parts[(2u * (size_t)(place - 1u) + 1u) * kMostKeys + threadIdx.x];
   for (uint32_t i = place; i <= cut.last; ++i)
-    sum += a.parts[2u * (size_t)i * kChRows + threadIdx.x];
-  store_weight(a, load_seq(a, cut.b), cut.b, cut.h, cut.x * kChRows + (int32_t)threadIdx.x, sum);
+    sum += a.parts[2u * (size_t)i * kMostKeys + threadIdx.x];
+  store_weight(a, load_seq(a, cut.b), cut.b, cut.h,
+               cut.x * (int32_t)blockDim.x + (int32_t)threadIdx.x, sum);
 }
 
 // Workgroups of a call: those that fit on the chip at once, fewer where the
@@ -1023,10 +1157,7 @@ ChunkArgs with_rcps(const ChunkArgs& args, uint32_t n) {
   ChunkArgs a = args;
   a.G = a.Hq / a.H;
   a.page_rcp = a.S == 1u ? 0u : (uint32_t)((1ull << 32) / a.S) + 1u;
-  // (a sequence's last item reaches 127 rows past its own)
-  a.group_rcp = a.G > 1u && ((uint64_t)a.T * a.G + kChRows) * a.G < (1ull << 32)
-                    ? (uint32_t)((1ull << 32) / a.G) + 1u
-                    : 0u;
+  a.group_rcp = ((1u << 31) + a.G - 1u) / a.G;
   a.share_rcp = 1.0 / (double)n;
   a.parts = reinterpret_cast<float*>(static_cast<char*>(a.cuts) + kCutBytes);
   return a;
@@ -1060,25 +1191,40 @@ hipError_t launch_attn(const ChunkArgs& args, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int D>
+template <int D, bool BIG>
 hipError_t launch_sums(const ChunkArgs& args, hipStream_t s) {
+  using Shape = SumShape<D, BIG>;
   const uint64_t G = args.Hq / args.H;
+  const uint64_t tiles = (args.T * G) / Shape::kRows + 2u;  // of an item, at most
   const uint32_t n = workgroups(
-      args, (uint64_t)args.B * (((uint64_t)args.max_pages * args.S) / kChRows + 1u),
-      (args.T * G) / kChTile + 2u, kCus * kSumsPerCu, kSumsLeast);
-  const ChunkArgs a = with_rcps(args, n);
+      args, (uint64_t)args.B * (((uint64_t)args.max_pages * args.S) / Shape::kKeys + 1u), tiles,
+      kCus * Shape::kPerCu, kSumsLeast);
+  ChunkArgs a = with_rcps(args, n);
+  // items of a few tiles are not worth cutting, nor a launch to join them
+  a.whole = tiles <= kWholeTiles ? 1u : 0u;
   const dim3 grid(n), block(kChThreads);
   switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
-    case 0: hipLaunchKernelGGL((attn_weights_kernel<D, 0>), grid, block, 0, s, a); break;
-    case kCap: hipLaunchKernelGGL((attn_weights_kernel<D, kCap>), grid, block, 0, s, a); break;
-    case kBias: hipLaunchKernelGGL((attn_weights_kernel<D, kBias>), grid, block, 0, s, a); break;
+    case 0: hipLaunchKernelGGL((attn_weights_kernel<D, 0, BIG>), grid, block, 0, s, a); break;
+    case kCap:
+      hipLaunchKernelGGL((attn_weights_kernel<D, kCap, BIG>), grid, block, 0, s, a);
+      break;
+    case kBias:
+      hipLaunchKernelGGL((attn_weights_kernel<D, kBias, BIG>), grid, block, 0, s, a);
+      break;
     default:
-      hipLaunchKernelGGL((attn_weights_kernel<D, (kCap | kBias)>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((attn_weights_kernel<D, (kCap | kBias), BIG>), grid, block, 0, s, a);
       break;
   }
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  hipLaunchKernelGGL(weights_join_kernel, dim3(n - 1u), dim3(kChRows), 0, s, a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || a.whole) return e;
+  hipLaunchKernelGGL(weights_join_kernel, dim3(n - 1u), dim3(Shape::kKeys), 0, s, a);
   return hipGetLastError();
+}
+
+// Rows per sequence from which the BIG cut is the faster one (SumShape).
+template <int D>
+hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
+  const uint64_t rows = (uint64_t)a.T * (a.Hq / a.H);
+  return rows >= 256u * (uint64_t)a.B ? launch_sums<D, true>(a, s) : launch_sums<D, false>(a, s);
 }
 
 }  // namespace
@@ -1088,7 +1234,7 @@ size_t chunk_attn_workspace(uint32_t head_dim) {
   return kCutBytes + 2u * kCus * per_cu * part_floats((int)head_dim) * sizeof(float);
 }
 size_t attn_weights_workspace() {
-  return kCutBytes + 2u * kCus * kSumsPerCu * kChRows * sizeof(float);
+  return kCutBytes + 2u * kCus * kMostSums * kMostKeys * sizeof(float);
 }
 
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s) {

@@ -296,10 +296,11 @@ struct ChunkArgs {
   PageGeom g;
   uint32_t* error;            // receives kErrTruncated, or nullptr
   void* cuts;                 // the workspace
-  // set by the launch: the workspace's two slots per workgroup, the group's
-  // heads, the factors that divide by S, G and the workgroups
+  // set by the launch: the workspace's two slots per workgroup; the group's
+  // heads; the factors that divide by S, G and the workgroups; whether items are
+  // not cut
   float* parts;
-  uint32_t G, page_rcp, group_rcp;
+  uint32_t G, page_rcp, group_rcp, whole;
   double share_rcp;
 };
 // Tokens of a sequence's table at most: positions are divided by the page size

@@ -488,8 +488,9 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  * the sum of exp(t).  A row that sees no key: o = 0, lse = -inf.  What keys and
  * values hold where a row does not see them changes nothing, NaN and inf too.
  *
- * num_qo_heads is any multiple of num_kv_heads (and num_q_tokens * num_qo_heads
- * / num_kv_heads < 2^30, max_pages * page_size <= 2^27).  max_pages >= every
+ * num_qo_heads is any multiple of num_kv_heads (and, with G the quotient,
+ * num_q_tokens * G < 2^30, (num_q_tokens + 128) * G * G < 2^31 where G is no
+ * power of two; max_pages * page_size <= 2^27).  max_pages >= every
  * sequence's page count: a longer table is cut to it and AOAKV_WS_ERR_TRUNCATED set in
  * *error_word (NULL: not reported), as in aoakv_topk_filtering.  workspace:
  * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
