@@ -65,7 +65,7 @@ SIGNATURES = {
     "aoakv_rms_norm_forward": [_p, _p, _p, _u32, _u32, _f32, _p],
     "aoakv_rope_append_kv_cache_prefill": [_p, _p, _p, _u32, _u32, _p, _p, _u32, _u32, _p, _p,
                                            _p, _p, _u32, _u32, _u32, _u32, _f32, _f32, _p],
-    "aoakv_chunk_attn_workspace_size": [_u32],
+    "aoakv_chunk_attn_workspace_size": [_u32, _u32, _u32, _u32, _u32],
     "aoakv_chunk_attn": [_p, _p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
                          _u32, _u32, _u32, _u32, _u32, _f32, _p, _sz, _p, _p],
     "aoakv_attn_weights_workspace_size": [],

@@ -1084,10 +1084,15 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   return AOAKV_OK;
 }
 
-size_t aoakv_chunk_attn_workspace_size(uint32_t head_dim) {
-  return head_dim == 64u || head_dim == 128u || head_dim == 256u
-             ? aoakv::chunk_attn_workspace(head_dim)
-             : 0u;
+size_t aoakv_chunk_attn_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
+                                       uint32_t num_qo_heads, uint32_t num_kv_heads,
+                                       uint32_t head_dim) {
+  // (the call itself refuses these)
+  if ((head_dim != 64u && head_dim != 128u && head_dim != 256u) || num_kv_heads == 0u ||
+      num_qo_heads > 256u || num_qo_heads % num_kv_heads != 0u)
+    return 0u;
+  return aoakv::chunk_attn_workspace(num_q_tokens, batch_size, num_qo_heads, num_kv_heads,
+                                     head_dim);
 }
 
 int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
@@ -1103,7 +1108,9 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
                          kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
                          num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
                          soft_cap, workspace, workspace_bytes,
-                         aoakv_chunk_attn_workspace_size(head_dim), error_word,
+                         aoakv_chunk_attn_workspace_size(num_q_tokens, batch_size, num_qo_heads,
+                                                         num_kv_heads, head_dim),
+                         error_word,
                          "chunk_attn"))
     return e;
   if (num_q_tokens == 0u) return ok();

@@ -66,6 +66,20 @@ __device__ inline Seq load_seq(const ChunkArgs& a, uint32_t b) {
   return s;
 }
 
+// A value that is the same in all lanes, in a scalar register (what comes from
+// LDS or a scan is not known to be: loops and tests on it would run in masks).
+__device__ inline uint32_t scalar(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+__device__ inline int32_t scalar(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline uint64_t scalar(uint64_t x) {
+  return (uint64_t)scalar((uint32_t)(x >> 32)) << 32 | scalar((uint32_t)x);
+}
+__device__ inline Seq scalar(const Seq& s) {
+  return Seq{scalar(s.q0), scalar(s.n), scalar(s.L), scalar(s.off), scalar(s.prefix),
+             scalar(s.page0)};
+}
+
 // An item's tiles: tile i of its list is tile i < cut ? i : i - cut + first.
 struct Item {
   int32_t cut, first, count;
@@ -157,7 +171,7 @@ struct Walk {
 
   __device__ Walk(const ChunkArgs& args, PlanLds& lds) : a(args), l(lds), base(0u), before(0u),
                                                          inside(0u), h(0u), b(0u), x(0), at(0u) {}
-  __device__ const Seq& seq() const { return l.seq[b - base]; }
+  __device__ Seq seq() const { return scalar(l.seq[b - base]); }
   __device__ void load(uint32_t first) {
     __syncthreads();
     if (first + threadIdx.x < a.B) l.seq[threadIdx.x] = load_seq(a, first + threadIdx.x);
@@ -179,7 +193,9 @@ struct Walk {
         u += (uint32_t)By::item(a, s, i).count + kItemUnits;
     }
     before = units_before;
-    const uint64_t p = scan_units(u, l, inside);
+    uint64_t sum;
+    const uint64_t p = scan_units(u, l, sum);
+    inside = scalar(sum);
     if (sb < nb && k == 0u) l.start[sb] = before + p;
     __syncthreads();
   }
@@ -196,7 +212,7 @@ struct Walk {
   // was called before
   __device__ void seek(uint64_t u, uint64_t per_head) {
     // u / per_head < 256: a quotient in fp32 is off by one at most
-    h = (uint32_t)((float)u * __builtin_amdgcn_rcpf((float)per_head));
+    h = scalar((uint32_t)((float)u * __builtin_amdgcn_rcpf((float)per_head)));
     h -= (uint64_t)h * per_head > u ? 1u : 0u;
     h += (uint64_t)(h + 1u) * per_head <= u ? 1u : 0u;
     const uint64_t y = u - (uint64_t)h * per_head;
@@ -214,8 +230,8 @@ struct Walk {
       if (s <= y && y < e) l.pick = i;
     }
     __syncthreads();
-    b = base + l.pick;
-    uint64_t rest = y - l.start[b - base];
+    b = base + scalar(l.pick);
+    uint64_t rest = y - scalar(l.start[b - base]);
     const Seq s = seq();
     const int32_t n = By::items(a, s);
     __syncthreads();
@@ -224,6 +240,7 @@ struct Walk {
       const uint64_t v = j < n ? (uint32_t)By::item(a, s, j).count + kItemUnits : 0u;
       uint64_t sum;
       const uint64_t p = scan_units(v, l, sum);
+      sum = scalar(sum);
       if (rest < sum) {
         if (p <= rest && rest < p + v) {
           l.pick = (uint32_t)j;
@@ -234,8 +251,8 @@ struct Walk {
       }
       rest -= sum;
     }
-    x = (int32_t)l.pick;
-    at = (uint32_t)l.off;
+    x = (int32_t)scalar(l.pick);
+    at = (uint32_t)scalar(l.off);
     __syncthreads();
   }
   // the next item (there is one)
@@ -256,30 +273,34 @@ struct Walk {
 // The share of workgroup w: units [w * share, (w + 1) * share) of them
 // (at least units / workgroups; the factor's rounding is below the 1 added).
 __device__ inline uint64_t share_of(const ChunkArgs& a, uint64_t units, uint32_t least) {
-  const uint64_t s = (uint64_t)((double)units * a.share_rcp) + 1u;
+  const uint64_t s = scalar((uint64_t)((double)units * a.share_rcp)) + 1u;
   return s > least ? s : least;
 }
 
-// The item that the border before a workgroup's share cuts, for the launch
-// that joins its parts: slot 1 of the workgroup before, slot 0 of this one to
-// `last`.  last 0: no cut, or not the item's first.
+// An item in parts, for the launch that joins them: n parts (0: nothing to join),
+// the first in slot `first`, the others in every step-th slot from first + 1 on.
 struct Cut {
-  uint32_t last, h, b;
-  int32_t x, q0, n;
-  uint32_t pad[2];
+  uint32_t n, h, b;
+  int32_t x, q0, rows;
+  uint32_t first, step;
+  __device__ size_t slot(uint32_t i) const { return i == 0u ? first : first + 1u + (i - 1u) * step; }
 };
+// The item that the border before workgroup `place`'s share cuts, where that is
+// its first cut: slot 1 of the workgroup before, slot 0 of the following ones.
 template <class By>
 __device__ inline Cut cut_of(const Walk<By>& w, uint32_t place, uint64_t share) {
   Cut c{};
   if (w.at == 0u || w.at > share) return c;  // (at == share: it begins where the share before does)
-  const Seq& s = w.seq();
+  const Seq s = w.seq();
   const uint32_t after = (uint32_t)By::item(w.a, s, w.x).count + kItemUnits - w.at;
-  c.last = place + (share >= after ? 0u : (after - 1u) / (uint32_t)share);
+  c.n = 2u + (share >= after ? 0u : (after - 1u) / (uint32_t)share);
   c.h = w.h;
   c.b = w.b;
   c.x = w.x;
   c.q0 = s.q0;
-  c.n = s.n;
+  c.rows = s.n * group(w.a);
+  c.first = 2u * place - 1u;
+  c.step = 2u;
   return c;
 }
 
@@ -330,9 +351,106 @@ __device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r,
     a.lse[row] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// One workgroup's share.  The tile loop is that of prefill.hip (S^T = K Q^T,
+// A call of many items: a launch before lists them (and the parts of those
+// longer than an equal share), the longest first, for one workgroup each.
+// Walking the keys of a head from its first on, side by side, the workgroups of
+// an XCD find them in its L2, and few items are cut.
+struct Entry {
+  uint32_t b;
+  int32_t x, t0, t1;
+  uint32_t slot;  // of the head's parts, or kWhole
+};
+struct ListHead {
+  uint32_t entries, parts, cuts;  // of each head
+};
+constexpr uint32_t kWhole = 0xFFFFFFFFu;
+constexpr size_t kListHeadBytes = 64;
+constexpr int32_t kListBins = 1024;
+
+__global__ __launch_bounds__(kChThreads) void chunk_list_kernel(ChunkArgs a, uint32_t slots,
+                                                                  uint32_t room) {
+  __shared__ PlanLds s_plan;
+  __shared__ uint32_t s_bin[kListBins], s_parts, s_cuts, s_wave[kChThreads / kWave];
+  const uint32_t tid = threadIdx.x;
+  Walk<ByRows> w(a, s_plan);
+  const uint64_t per_head = w.total();
+  const uint64_t share64 = per_head * a.H / slots + 1u;
+  const uint32_t share = (uint32_t)(share64 < 0x7FFFFFFFu ? share64 : 0x7FFFFFFFu);
+  for (uint32_t i = tid; i < (uint32_t)kListBins; i += kChThreads) s_bin[i] = 0u;
+  if (tid == 0u) s_parts = s_cuts = 0u;
+  __syncthreads();
+  // twice over all items: how many entries there are of each length (bins from
+  // the longest on), then their places
+  Entry* list = static_cast<Entry*>(a.list);
+  Cut* cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.cuts) + kListHeadBytes);
+  for (int pass = 0; pass < 2; ++pass) {
+    for (uint32_t first = 0u; first < a.B; first += kChThreads) {
+      if (a.B > kChThreads) w.load(first);
+      const uint32_t nb = min(a.B - first, kChThreads);
+      const uint32_t per = kChThreads >> (nb > 1u ? 32 - __clz(nb - 1u) : 0);
+      const uint32_t sb = tid / per;
+      if (sb >= nb) continue;
+      const Seq s = s_plan.seq[sb];
+      const int32_t n = ByRows::items(a, s);
+      for (int32_t x = (int32_t)(tid % per); x < n; x += (int32_t)per) {
+        const uint32_t count = (uint32_t)ByRows::item(a, s, x).count;
+        const uint32_t units = count + kItemUnits;
+        const uint32_t parts = units > share ? (units + share - 1u) / share : 1u;
+        const int32_t length = (int32_t)((count + parts - 1u) / parts);
+        const uint32_t bin = (uint32_t)(kListBins - 1 - min(length, kListBins - 1));
+        const uint32_t at = atomicAdd(&s_bin[bin], parts);
+        if (pass == 0) continue;
+        uint32_t slot = kWhole;
+        if (parts > 1u) {
+          slot = atomicAdd(&s_parts, parts);
+          Cut c{};
+          c.n = parts;
+          c.b = first + sb;
+          c.x = x;
+          c.q0 = s.q0;
+          c.rows = s.n * group(a);
+          c.first = slot;
+          c.step = 1u;
+          cuts[atomicAdd(&s_cuts, 1u)] = c;
+        }
+        // (room: what rows of a q_indptr that counts none twice can fill)
+        for (uint32_t i = 0; i < parts && at + i < room; ++i)
+          list[at + i] = Entry{first + sb, x, (int32_t)((uint64_t)count * i / parts),
+                               (int32_t)((uint64_t)count * (i + 1u) / parts),
+                               parts > 1u ? slot + i : kWhole};
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {  // bins to their first places
+      constexpr uint32_t kN = kListBins / kChThreads;
+      uint32_t v[kN], sum = 0u;
+      for (uint32_t i = 0; i < kN; ++i) sum += v[i] = s_bin[tid * kN + i];
+      uint32_t upto = sum;
+      for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
+        const uint32_t y = __shfl_up(upto, d);
+        if (__lane_id() >= d) upto += y;
+      }
+      if (__lane_id() == kWave - 1u) s_wave[tid / kWave] = upto;
+      __syncthreads();
+      for (uint32_t i = 0; i < tid / kWave; ++i) upto += s_wave[i];
+      uint32_t before = upto - sum;
+      if (tid == kChThreads - 1u) reinterpret_cast<ListHead*>(a.cuts)->entries = min(upto, room);
+      for (uint32_t i = 0; i < kN; ++i) {
+        s_bin[tid * kN + i] = before;
+        before += v[i];
+      }
+      __syncthreads();
+    }
+  }
+  if (tid == 0u) {
+    reinterpret_cast<ListHead*>(a.cuts)->parts = s_parts;
+    reinterpret_cast<ListHead*>(a.cuts)->cuts = s_cuts;
+  }
+}
+
+// One workgroup's share, or its entry of the list.  The tile loop is that of prefill.hip (S^T = K Q^T,
 // lane l holds row l % 32 of its wave's 32); scores are kept in units of log 2.
-template <int D, int MOD, bool S16>
+template <int D, int MOD, bool S16, bool LIST>
 __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kernel(ChunkArgs a) {
   using Sh = PfShape<D>;
   __shared__ __attribute__((aligned(16))) char s_buf0[2 * Sh::kTileBytes];
@@ -342,16 +460,19 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
 
   Walk<ByRows> w(a, s_plan);
-  const uint64_t per_head = w.total(), units = per_head * a.H;
-  const uint64_t share = share_of(a, units, kAttnLeast);
-  uint64_t u = list_place() * share;
-  const uint64_t u1 = min(u + share, units);
-  if (u >= u1) {
-    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
-    return;
+  uint64_t u = 0u, u1 = 0u;
+  if constexpr (!LIST) {
+    const uint64_t per_head = w.total(), units = per_head * a.H;
+    const uint64_t share = share_of(a, units, kAttnLeast);
+    u = list_place() * share;
+    u1 = min(u + share, units);
+    if (u >= u1) {
+      if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].n = 0u;
+      return;
+    }
+    w.seek(u, per_head);
+    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
   }
-  w.seek(u, per_head);
-  if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
 
   const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
   // cap: c tanh(x / c) = c - 2 c / (1 + e^(2 x / c))
@@ -391,16 +512,42 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     auto lo_at = [&](int t) { return kXor ? v_lo[0] ^ (64 * t) : v_lo[t]; };
     auto hi_at = [&](int t) { return kXor ? v_hi[0] ^ (64 * t) : v_hi[t]; };
 
-    const Seq s = w.seq();
-    const Item item = ByRows::item(a, s, w.x);
-    const uint32_t hk = w.h;
-    const uint32_t ue = (uint32_t)item.count + kItemUnits;
-    const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
-    const int32_t t0 = max((int32_t)(ua - kItemUnits), 0), t1 = max((int32_t)(ub - kItemUnits), 0);
+    // ---- the work: tiles t0 .. t1 - 1 of item ix of a sequence and kv head hk,
+    // whole or for a slot of the workspace
+    Seq s;
+    int32_t ix, t0, t1;
+    uint32_t hk, slot, units = 0u;
+    Item item;
+    if constexpr (LIST) {
+      // (an entry per workgroup, the longest of all heads first; heads as in
+      // prefill.hip: each XCD its own, walking their keys side by side)
+      const ListHead* head = reinterpret_cast<const ListHead*>(a.cuts);
+      const uint32_t k = blockIdx.x / a.H, hs = blockIdx.x % a.H;
+      if (k >= head->entries) return;
+      hk = a.H % kXcds == 0u ? hs % kXcds * (a.H / kXcds) + hs / kXcds : hs;
+      const Entry e = static_cast<const Entry*>(a.list)[k];
+      s = scalar(load_seq(a, e.b));
+      ix = e.x;
+      t0 = e.t0;
+      t1 = e.t1;
+      item = ByRows::item(a, s, ix);
+      slot = e.slot == kWhole ? kWhole : hk * head->parts + e.slot;
+    } else {
+      s = w.seq();
+      ix = w.x;
+      item = ByRows::item(a, s, ix);
+      hk = w.h;
+      const uint32_t ue = (uint32_t)item.count + kItemUnits;
+      const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
+      units = ub - ua;
+      t0 = (int32_t)((uint64_t)ua * (uint32_t)item.count / ue);
+      t1 = (int32_t)((uint64_t)ub * (uint32_t)item.count / ue);
+      slot = ua == 0u && ub == ue ? kWhole : 2u * list_place() + (ua == 0u ? 1u : 0u);
+    }
 
     // ---- this lane's row
     const int32_t R = s.n * group(a);
-    const int32_t r0 = w.x * kChRows + wave * 32;  // the wave's first row
+    const int32_t r0 = ix * kChRows + wave * 32;  // the wave's first row
     const int32_t r = r0 + c;
     const bool live = r < R;
     const Row row = row_of(a, hk, live ? r : R - 1);
@@ -417,8 +564,6 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     // first and last position of the wave's rows and of the item's
     const int32_t wp0 = s.off + token_of(a, min(r0, R - 1)),
                   wp1 = s.off + token_of(a, min(r0 + 31, R - 1));
-    const int32_t ip0 = s.off + token_of(a, w.x * kChRows),
-                  ip1 = s.off + token_of(a, min(w.x * kChRows + kChRows - 1, R - 1));
     // whether rows at positions p0 .. p1 all see the 64 keys from k0 on
     auto all_see = [&](int32_t k0, int32_t p0, int32_t p1) {
       return k0 + kChTile <= s.prefix ||
@@ -488,39 +633,22 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    // A tile that not every row sees whole.  A probability of 0 times a value of
-    // inf or NaN would be NaN in the product, so the values of keys that are
-    // none (unwritten slots) become 0; and where another value is not finite
-    // (rare), the O elements that it reaches are noted, and the product gets 0.
-    // Called by the whole workgroup.
-    auto clean_values = [&](char* vbuf, int32_t k0) {
-      constexpr int kN = Sh::kTileBytes / 16 / (int)kChThreads;
-      uint4* chunks = reinterpret_cast<uint4*>(vbuf);
-      uint32_t bad = 0u;
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const int at = tid + (int)kChThreads * j;
-        if (k0 + at / Sh::kCh >= s.L) {
-          chunks[at] = uint4{0u, 0u, 0u, 0u};
-        } else {
-          const uint4 x = chunks[at];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t y = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
-            // (exponent bits all set: adding 1 to them carries)
-            bad |= ((y & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-          }
-        }
-      }
-      if (!__syncthreads_or((int)(bad != 0u))) return;
-      // every wave looks through the tile for its own rows
+    // A value of inf or NaN that some rows of the wave do not see: a probability of
+    // 0 times it would be NaN in the product.  So where a tile that is masked in
+    // part holds any (rare; found in the fragments on their way), they are 0 in
+    // the product, and this notes the O elements that they reach.
+    auto note_values = [&](const lds_char* sV, int32_t k0) {
+      const int end = min(kChTile, s.L - k0) * Sh::kCh;  // (slots behind the end are nobody's)
 #pragma nounroll
-      for (int j = 0; j < Sh::kTileBytes / 16; j += kWave) {
+      for (int j = 0; j < end; j += kWave) {
         const int at = j + lane;
-        const H8 x = __builtin_bit_cast(H8, chunks[at]);
         bool odd = false;
+        if (at < end) {
+          const half8 x = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+              sV + 16 * at);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) odd |= !__builtin_isfinite((float)x.v[e]);
+          for (int e = 0; e < 8; ++e) odd |= !__builtin_isfinite((float)x[e]);
+        }
 #pragma nounroll
         for (uint64_t left = __builtin_amdgcn_ballot_w64(odd); left != 0u; left &= left - 1u) {
           const int src = __builtin_ctzll(left);
@@ -530,7 +658,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           const bool seen = key < s.prefix || (key < hi && key >= lo);
 #pragma nounroll
           for (int e = 0; e < 8; ++e) {
-            const uint32_t y = reinterpret_cast<const uint16_t*>(chunks + j + src)[e];
+            const uint32_t y = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+                sV + 16 * (j + src) + 2 * e);
             if ((y & 0x7C00u) != 0x7C00u) continue;
             // dim d0 + e is element 16 t + i of lane group dd / 4 % 2
             const int dd = (d0 + e) % 32, bit = 16 * ((d0 + e) / 32) + 4 * (dd / 8) + dd % 4;
@@ -545,16 +674,6 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           }
         }
       }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        H8 x = __builtin_bit_cast(H8, chunks[tid + (int)kChThreads * j]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!__builtin_isfinite((float)x.v[e])) x.v[e] = (f16)0.f;
-        chunks[tid + (int)kChThreads * j] = __builtin_bit_cast(uint4, x);
-      }
-      __syncthreads();
     };
 
     auto tile = [&](const lds_char* sK, const lds_char* sV, int32_t k0) {
@@ -626,8 +745,20 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
             acc_s[ks][i] = t;
           }
       }
+      bool dirty = false;
       if (!all_see(k0, wp0, wp1)) {
         // (one unsigned comparison for the range, one for the prefix)
+        uint32_t odd = 0u;  // values of inf or NaN (adding 1 to the exponent carries)
+#pragma unroll
+        for (int t = 0; t < Sh::kDB; ++t)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const u32x4 y = __builtin_bit_cast(u32x4, vfrag(sV, t, kk));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= (y[e] & 0x7C007C00u) + 0x04000400u;
+          }
+        dirty = __builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0u) != 0u;
+        if (dirty) note_values(sV, k0);
         const int32_t first = k0 + 4 * g, pre = s.prefix - first;
         const uint32_t begin = (uint32_t)(lo - first), span = (uint32_t)max(hi - lo, 0);
 #pragma unroll
@@ -675,25 +806,35 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       }
       l_run = l_run + lt;
       m_run = m_new;
-      half8 vfa[4], vfb[4];
+      auto add_values = [&](auto clean) {
+        auto frags = [&](int t, half8 (&f)[4]) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) vfa[kk] = vfrag(sV, 0, kk);
+          for (int kk = 0; kk < 4; ++kk) {
+            f[kk] = vfrag(sV, t, kk);
+            if constexpr (clean.value) {
 #pragma unroll
-      for (int t = 0; t < Sh::kDB; t += 2) {
+              for (int e = 0; e < 8; ++e)
+                f[kk][e] = __builtin_isfinite((float)f[kk][e]) ? f[kk][e] : (f16)0.f;
+            }
+          }
+        };
+        half8 vfa[4], vfb[4];
+        frags(0, vfa);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) vfb[kk] = vfrag(sV, t + 1, kk);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < Sh::kDB; t += 2) {
+          frags(t + 1, vfb);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) acc_o[t] = mfma32(vfa[kk], pb[kk / 2][kk % 2], acc_o[t]);
-        if (t + 2 < Sh::kDB) {
+          for (int kk = 0; kk < 4; ++kk) acc_o[t] = mfma32(vfa[kk], pb[kk / 2][kk % 2], acc_o[t]);
+          if (t + 2 < Sh::kDB) frags(t + 2, vfa);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) vfa[kk] = vfrag(sV, t + 2, kk);
+          for (int kk = 0; kk < 4; ++kk)
+            acc_o[t + 1] = mfma32(vfb[kk], pb[kk / 2][kk % 2], acc_o[t + 1]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          acc_o[t + 1] = mfma32(vfb[kk], pb[kk / 2][kk % 2], acc_o[t + 1]);
-      }
+      };
+      if (dirty) add_values(std::true_type{});
+      else add_values(std::false_type{});
     };
 
     // ---- the tiles of this part
@@ -716,7 +857,6 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           if (i + 2 < t1) ids = page_of(item.tile(i + 2));
         }
         const int32_t k0 = item.tile(i) * kChTile;
-        if (!all_see(k0, ip0, ip1)) clean_values(buf + Sh::kTileBytes, k0);  // uniform
         if (any_sees(k0)) tile((const lds_char*)buf, (const lds_char*)(buf + Sh::kTileBytes), k0);
       }
     }
@@ -731,10 +871,10 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           if (inf_neg[t / 4] >> bit & 1u) acc_o[t][i] -= INFINITY;
         }
       }
-    if (ua == 0u && ub == ue) {
+    if (slot == kWhole) {
       if (live) store_row<D>(a, s, row, g, m_run * scale, l_run, acc_o);
     } else if (live) {  // a part: m in units of log 2
-      float* part = a.parts + (2u * (size_t)list_place() + (ua == 0u ? 1u : 0u)) * part_floats(D);
+      float* part = a.parts + (size_t)slot * part_floats(D);
       float4* po = reinterpret_cast<float4*>(part) + wave * 32 + c;
 #pragma unroll
       for (int j = 0; j < Sh::kDB * 4; ++j) {
@@ -749,27 +889,36 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         pm[kChRows] = l_run;
       }
     }
-    u += ub - ua;
+    if constexpr (LIST) return;
+    u += units;
     if (u >= u1) return;
     w.next();
   }
 }
 
-// Joins an item's parts: workgroup (w, sub) takes 32 of its rows, a thread one
+// Joins an item's parts: workgroup (cut, sub) takes 32 of its rows, a thread one
 // row and D / 8 dims.
-template <int D>
+template <int D, bool LIST>
 __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
-  const uint32_t place = blockIdx.x / 4u + 1u, sub = blockIdx.x % 4u;
-  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[place];
-  if (cut.last == 0u) return;
+  const uint32_t place = blockIdx.x / 4u, sub = blockIdx.x % 4u;
+  Cut cut;
+  if constexpr (LIST) {
+    const ListHead* head = reinterpret_cast<const ListHead*>(a.cuts);
+    if (place / a.H >= head->cuts) return;
+    cut = reinterpret_cast<const Cut*>(static_cast<const char*>(a.cuts) +
+                                       kListHeadBytes)[place / a.H];
+    cut.h = place % a.H;
+    cut.first += cut.h * head->parts;
+  } else {
+    cut = reinterpret_cast<const Cut*>(a.cuts)[place + 1u];
+    if (cut.n == 0u) return;
+  }
   const int32_t r = (int32_t)(sub * 32u + threadIdx.x % 32u);
-  if (cut.x * kChRows + r >= cut.n * group(a)) return;
+  if (cut.x * kChRows + r >= cut.rows) return;
   const Row row = row_of(a, cut.h, cut.x * kChRows + r);
   const uint32_t j0 = threadIdx.x / 32u;
-  const uint32_t n = cut.last - place + 2u;
-  auto part = [&](uint32_t i) {
-    return a.parts + (2u * (size_t)(place - 1u + i) + (i == 0u ? 1u : 0u)) * part_floats(D);
-  };
+  const uint32_t n = cut.n;
+  auto part = [&](uint32_t i) { return a.parts + cut.slot(i) * part_floats(D); };
   float m = kPfNoMax, l = 0.f;
   for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, part(i)[kChRows * D + r]);
   constexpr int kV = D / 32;
@@ -832,14 +981,15 @@ constexpr int32_t kNoPos = INT32_MIN;
 // How the weights are cut.  BIG, where a sequence has many rows: a wave holds 2 x
 // 32 keys (64 registers at D = 128; each halves the reads of query rows per
 // product), tiles of 128 rows, two workgroups per CU.  Else the keys' own way
-// from memory is what takes the time: 32 keys, tiles of 32 rows, and four
-// workgroups per CU with their keys in flight.
+// from memory is what takes the time: 32 keys, tiles of 32 rows, and as many
+// workgroups per CU with their keys in flight as registers allow (the last 32
+// rows of 16384 tokens x 32 heads: 2 per CU 38 us, 3 32, 4, spilling, 41).
 template <int D, bool BIG>
 struct SumShape {
   static constexpr int kSets = BIG && D != 256 ? 2 : 1;  // of 32 keys per wave
   static constexpr int32_t kKeys = 4 * 32 * kSets;       // of an item
   static constexpr int32_t kRows = BIG ? (D == 256 ? 64 : 128) : 32;  // of a tile
-  static constexpr uint32_t kPerCu = BIG ? 2u : D == 256 ? 3u : 4u;   // workgroups
+  static constexpr uint32_t kPerCu = BIG || D == 256 ? 2u : D == 128 ? 3u : 4u;
 };
 constexpr int32_t kMostKeys = 256;
 constexpr uint32_t kMostSums = 4u;
@@ -877,7 +1027,7 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
   uint64_t u = list_place() * share;
   const uint64_t u1 = min(u + share, units);
   if (u >= u1) {
-    if (tid == 0 && !a.whole) reinterpret_cast<Cut*>(a.cuts)[list_place()].last = 0u;
+    if (tid == 0 && !a.whole) reinterpret_cast<Cut*>(a.cuts)[list_place()].n = 0u;
     return;
   }
   w.seek(u, per_head);
@@ -1131,12 +1281,10 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
 
 // Joins an item's parts: a thread per key.
 __global__ __launch_bounds__(kMostKeys) void weights_join_kernel(ChunkArgs a) {
-  const uint32_t place = blockIdx.x + 1u;
-  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[place];
-  if (cut.last == 0u) return;
-  float sum = a.parts[(2u * (size_t)(place - 1u) + 1u) * kMostKeys + threadIdx.x];
-  for (uint32_t i = place; i <= cut.last; ++i)
-    sum += a.parts[2u * (size_t)i * kMostKeys + threadIdx.x];
+  const Cut cut = reinterpret_cast<const Cut*>(a.cuts)[blockIdx.x + 1u];
+  if (cut.n == 0u) return;
+  float sum = 0.f;
+  for (uint32_t i = 0; i < cut.n; ++i) sum += a.parts[cut.slot(i) * kMostKeys + threadIdx.x];
   store_weight(a, load_seq(a, cut.b), cut.b, cut.h,
                cut.x * (int32_t)blockDim.x + (int32_t)threadIdx.x, sum);
 }
@@ -1163,31 +1311,66 @@ ChunkArgs with_rcps(const ChunkArgs& args, uint32_t n) {
   return a;
 }
 
-template <int D, int MOD>
+template <int D, int MOD, bool LIST>
 hipError_t launch_attn(const ChunkArgs& a, uint32_t n, hipStream_t s) {
   if (a.S % 16u == 0u)
-    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, true>), dim3(n), dim3(kChThreads), 0, s, a);
+    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, true, LIST>), dim3(n), dim3(kChThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, false>), dim3(n), dim3(kChThreads), 0, s, a);
+    hipLaunchKernelGGL((chunk_attn_kernel<D, MOD, false, LIST>), dim3(n), dim3(kChThreads), 0, s,
+                       a);
   return hipGetLastError();
+}
+
+template <int D, bool LIST>
+hipError_t launch_attn(const ChunkArgs& a, uint32_t n, hipStream_t s) {
+  switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
+    case 0: return launch_attn<D, 0, LIST>(a, n, s);
+    case kCap: return launch_attn<D, kCap, LIST>(a, n, s);
+    case kBias: return launch_attn<D, kBias, LIST>(a, n, s);
+    default: return launch_attn<D, kCap | kBias, LIST>(a, n, s);
+  }
+}
+
+// Entries of a head's list at most: its items, and the parts of those cut (a
+// part is longer than half a share, and all heads' shares fill the slots).
+uint64_t list_entries(const ChunkArgs& a, uint32_t slots) {
+  return (uint64_t)a.T * (a.Hq / a.H) / kChRows + a.B + 2u * slots / a.H + 1u;
+}
+// Whether a call has rows for so many items that they are listed (and a grid of
+// 32-bit work-items holds their workgroups).
+bool lists_items(const ChunkArgs& a, uint32_t slots) {
+  return (uint64_t)a.T * (a.Hq / a.H) / kChRows * a.H >= slots &&
+         list_entries(a, slots) * a.H < (1u << 24);
+}
+template <int D>
+constexpr uint32_t attn_slots() { return kCus * attn_per_cu<D>(); }
+size_t list_bytes(const ChunkArgs& a, uint32_t slots) {
+  return lists_items(a, slots) ? (list_entries(a, slots) * sizeof(Entry) + 255u) / 256u * 256u : 0u;
 }
 
 template <int D>
 hipError_t launch_attn(const ChunkArgs& args, hipStream_t s) {
+  constexpr uint32_t kSlots = attn_slots<D>();
+  if (lists_items(args, kSlots)) {
+    const uint64_t n = list_entries(args, kSlots) * args.H;
+    ChunkArgs a = with_rcps(args, kSlots);
+    a.list = a.parts;
+    a.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(a.parts) + list_bytes(a, kSlots));
+    hipLaunchKernelGGL(chunk_list_kernel, dim3(1), dim3(kChThreads), 0, s, a, kSlots,
+                       (uint32_t)(n / a.H));
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (hipError_t e = launch_attn<D, true>(a, (uint32_t)n, s); e != hipSuccess) return e;
+    hipLaunchKernelGGL((chunk_join_kernel<D, true>), dim3((kSlots / a.H + 1u) * a.H * 4u),
+                       dim3(kChThreads), 0, s, a);
+    return hipGetLastError();
+  }
   const uint64_t G = args.Hq / args.H;
   const uint32_t n = workgroups(args, (args.T * G) / kChRows + args.B,
-                                ((uint64_t)args.max_pages * args.S) / kChTile + 2u,
-                                kCus * attn_per_cu<D>(), kAttnLeast);
+                                ((uint64_t)args.max_pages * args.S) / kChTile + 2u, kSlots,
+                                kAttnLeast);
   const ChunkArgs a = with_rcps(args, n);
-  hipError_t e = hipSuccess;
-  switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
-    case 0: e = launch_attn<D, 0>(a, n, s); break;
-    case kCap: e = launch_attn<D, kCap>(a, n, s); break;
-    case kBias: e = launch_attn<D, kBias>(a, n, s); break;
-    default: e = launch_attn<D, kCap | kBias>(a, n, s); break;
-  }
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a);
+  if (hipError_t e = launch_attn<D, false>(a, n, s); e != hipSuccess) return e;
+  hipLaunchKernelGGL((chunk_join_kernel<D, false>), dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a);
   return hipGetLastError();
 }
 
@@ -1229,9 +1412,15 @@ hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
 
 }  // namespace
 
-size_t chunk_attn_workspace(uint32_t head_dim) {
-  const size_t per_cu = head_dim == 256u ? attn_per_cu<256>() : attn_per_cu<128>();
-  return kCutBytes + 2u * kCus * per_cu * part_floats((int)head_dim) * sizeof(float);
+size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim) {
+  ChunkArgs a{};
+  a.T = T;
+  a.B = B;
+  a.Hq = Hq;
+  a.H = H;
+  const uint32_t slots = head_dim == 256u ? attn_slots<256>() : attn_slots<128>();
+  return kCutBytes + list_bytes(a, slots) +
+         2u * (size_t)slots * part_floats((int)head_dim) * sizeof(float);
 }
 size_t attn_weights_workspace() {
   return kCutBytes + 2u * kCus * kMostSums * kMostKeys * sizeof(float);

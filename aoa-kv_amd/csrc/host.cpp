@@ -556,7 +556,7 @@ PyObject* chunk_attn(PyObject* const* a) {
   const Tensor o = given != nullptr ? *given : at::empty_like(c.q);
   Tensor lse;
   if (want) lse = at::empty({c.q.size(0), c.q.size(1)}, c.q.options().dtype(at::kFloat));
-  const size_t n = g_lib.chunk_attn_workspace_size(c.d.D);
+  const size_t n = g_lib.chunk_attn_workspace_size(c.T, (uint32_t)c.t.B, c.Hq, c.d.H, c.d.D);
   const Tensor ws = scratch(n, c.q);
   void* s = stream();
   call("aoakv_chunk_attn", [&] {

@@ -300,6 +300,7 @@ struct ChunkArgs {
   // heads; the factors that divide by S, G and the workgroups; whether items are
   // not cut
   float* parts;
+  void* list;
   uint32_t G, page_rcp, group_rcp, whole;
   double share_rcp;
 };
@@ -310,7 +311,7 @@ constexpr uint32_t kMaxChunkTokens = 1u << 27;
 __device__ inline uint32_t div_page(uint32_t x, uint32_t rcp) {
   return rcp == 0u ? x : __umulhi(x, rcp);
 }
-size_t chunk_attn_workspace(uint32_t head_dim);
+size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim);
 size_t attn_weights_workspace();
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
 hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);

@@ -496,7 +496,9 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
  * initialisation and is free again when the call's work on `stream` is done.
  */
-size_t aoakv_chunk_attn_workspace_size(uint32_t head_dim);
+size_t aoakv_chunk_attn_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
+                                       uint32_t num_qo_heads, uint32_t num_kv_heads,
+                                       uint32_t head_dim);
 int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
                      uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
                      const int32_t* kv_indices, const int32_t* kv_last_page_len,
