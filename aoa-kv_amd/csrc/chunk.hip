@@ -806,35 +806,31 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       }
       l_run = l_run + lt;
       m_run = m_new;
-      auto add_values = [&](auto clean) {
-        auto frags = [&](int t, half8 (&f)[4]) {
+      auto frags = [&](int t, half8 (&f)[4]) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            f[kk] = vfrag(sV, t, kk);
-            if constexpr (clean.value) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                f[kk][e] = __builtin_isfinite((float)f[kk][e]) ? f[kk][e] : (f16)0.f;
-            }
-          }
-        };
-        half8 vfa[4], vfb[4];
-        frags(0, vfa);
-#pragma unroll
-        for (int t = 0; t < Sh::kDB; t += 2) {
-          frags(t + 1, vfb);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) acc_o[t] = mfma32(vfa[kk], pb[kk / 2][kk % 2], acc_o[t]);
-          if (t + 2 < Sh::kDB) frags(t + 2, vfa);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int kk = 0; kk < 4; ++kk) f[kk] = vfrag(sV, t, kk);
+        if (dirty) {  // (uniform; a copy of the loop below for it spilled registers)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            acc_o[t + 1] = mfma32(vfb[kk], pb[kk / 2][kk % 2], acc_o[t + 1]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              f[kk][e] = __builtin_isfinite((float)f[kk][e]) ? f[kk][e] : (f16)0.f;
         }
       };
-      if (dirty) add_values(std::true_type{});
-      else add_values(std::false_type{});
+      half8 vfa[4], vfb[4];
+      frags(0, vfa);
+#pragma unroll
+      for (int t = 0; t < Sh::kDB; t += 2) {
+        frags(t + 1, vfb);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) acc_o[t] = mfma32(vfa[kk], pb[kk / 2][kk % 2], acc_o[t]);
+        if (t + 2 < Sh::kDB) frags(t + 2, vfa);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          acc_o[t + 1] = mfma32(vfb[kk], pb[kk / 2][kk % 2], acc_o[t + 1]);
+      }
     };
 
     // ---- the tiles of this part
