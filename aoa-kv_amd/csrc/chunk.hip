@@ -319,7 +319,7 @@ template <int D>
 constexpr uint32_t attn_per_cu() { return D == 256 ? 1u : 2u; }
 constexpr uint32_t kCus = 256u;
 constexpr size_t kCutBytes = kCus * 4u * sizeof(Cut);  // (4 workgroups per CU at most)
-constexpr uint32_t kAttnLeast = 4u;  // units of a share at least
+constexpr uint32_t kAttnLeast = 2u;  // units of a share at least
 
 // Row r of a sequence's packed rows.
 struct Row {
@@ -729,21 +729,38 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       }
       if constexpr (MOD != 0) {
         const float d0 = (float)(pos - k0 - 4 * g);  // crow(i, g) = crow(i, 0) + 4 g
+        const float pre = MOD & kCap ? 0.f : a.sm_scale * kLog2e;
+        if (MOD & kCap) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+          for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float t = acc_s[ks][i];
-            if constexpr (MOD & kCap)
-              t = __builtin_fmaf(-2.f * cap2,
-                                 __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * cap_in)),
-                                 cap2);
-            else
-              t *= a.sm_scale * kLog2e;
-            if constexpr (MOD & kBias)
-              t = __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(ks * 32 + crow(i, 0))), t);
-            acc_s[ks][i] = t;
+            for (int i = 0; i < 16; ++i)
+              acc_s[ks][i] = __builtin_fmaf(
+                  -2.f * cap2,
+                  __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(acc_s[ks][i] * cap_in)), cap2);
+        }
+        if constexpr (MOD & kBias) {
+          if (k0 + kChTile - 1 <= wp0) {  // no key behind a row: the distances need no |.|
+            const float far = -slope * d0;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float t = MOD & kCap ? acc_s[ks][i] + far
+                                           : __builtin_fmaf(acc_s[ks][i], pre, far);
+                acc_s[ks][i] = __builtin_fmaf(slope, (float)(ks * 32 + crow(i, 0)), t);
+              }
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float d = __builtin_fabsf(d0 - (float)(ks * 32 + crow(i, 0)));
+                const float t = MOD & kCap ? acc_s[ks][i] : acc_s[ks][i] * pre;
+                acc_s[ks][i] = __builtin_fmaf(-slope, d, t);
+              }
           }
+        }
       }
       bool dirty = false;
       if (!all_see(k0, wp0, wp1)) {
@@ -913,23 +930,50 @@ __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
   if (cut.x * kChRows + r >= cut.rows) return;
   const Row row = row_of(a, cut.h, cut.x * kChRows + r);
   const uint32_t j0 = threadIdx.x / 32u;
-  const uint32_t n = cut.n;
-  auto part = [&](uint32_t i) { return a.parts + cut.slot(i) * part_floats(D); };
+  // kAt parts at a time, their loads together: a part after the other, few rows
+  // over many parts took 17 us
+  constexpr int kV = D / 32, kAt = D == 256 ? 4 : 8;
   float m = kPfNoMax, l = 0.f;
-  for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, part(i)[kChRows * D + r]);
-  constexpr int kV = D / 32;
   float4 acc[kV] = {};
-  for (uint32_t i = 0; i < n; ++i) {
-    const float* p = part(i);
-    const float f = __builtin_amdgcn_exp2f(p[kChRows * D + r] - m);
-    l += p[kChRows * (D + 1) + r] * f;
+  for (uint32_t i0 = 0; i0 < cut.n; i0 += kAt) {
+    float pm[kAt], pl[kAt];
+    float4 po[kAt][kV];
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) {
+      pm[i] = kPfNoMax;
+      if (i0 + (uint32_t)i >= cut.n) continue;  // uniform
+      const float* p = a.parts + cut.slot(i0 + (uint32_t)i) * part_floats(D);
+      pm[i] = p[kChRows * D + r];
+      pl[i] = p[kChRows * (D + 1) + r];
+#pragma unroll
+      for (int v = 0; v < kV; ++v)
+        po[i][v] = reinterpret_cast<const float4*>(p)[(kV * j0 + v) * kChRows + r];
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) top = fmaxf(top, pm[i]);
+    const float keep = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= keep;
 #pragma unroll
     for (int v = 0; v < kV; ++v) {
-      const float4 y = reinterpret_cast<const float4*>(p)[(kV * j0 + v) * kChRows + r];
-      acc[v].x += y.x * f;
-      acc[v].y += y.y * f;
-      acc[v].z += y.z * f;
-      acc[v].w += y.w * f;
+      acc[v].x *= keep;
+      acc[v].y *= keep;
+      acc[v].z *= keep;
+      acc[v].w *= keep;
+    }
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) {
+      if (i0 + (uint32_t)i >= cut.n) break;  // uniform
+      const float f = __builtin_amdgcn_exp2f(pm[i] - m);
+      l += pl[i] * f;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        acc[v].x += po[i][v].x * f;
+        acc[v].y += po[i][v].y * f;
+        acc[v].z += po[i][v].z * f;
+        acc[v].w += po[i][v].w * f;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
