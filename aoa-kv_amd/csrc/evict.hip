@@ -24,24 +24,25 @@ __device__ inline uint32_t seq_tokens(const int32_t* indptr, const int32_t* last
 constexpr uint32_t kKeepThreads = 1024;
 constexpr uint32_t kKeepWaves = kKeepThreads / kWave;
 constexpr uint32_t kRun = 4u * kKeepThreads;  // tokens a workgroup takes at once, 4 per thread
-constexpr uint32_t kCopies = 16u;             // of the histogram, one per lane of 16
+constexpr uint32_t kBins = 2048u, kCopies = 4u;
 
 // One workgroup per (kv head, sequence).  Two weights are ordered as the
-// integers order_key makes of them (NaN lowest, -0 as 0).  Eight bits of them
-// at a time from the top, a histogram of the tokens that agree so far finds
-// where the last kept one lies, until that bin is kept whole; then a token's
-// place in the row is the number of larger tokens before it plus that of kept
-// equal ones.  The tokens are held in registers (RUNS x 4 per thread), loaded
-// once where a sequence has no more than that, else once per step.
+// integers that order_key makes of them (NaN lowest, -0 as 0); the first `sink`
+// and last `recent` tokens have the largest integer of all, so the choice is
+// that of the `keep` largest, ties to the lower position.  Eleven bits at a time
+// from the top, a histogram of the tokens that agree so far finds where the
+// last kept one lies, until that bin is kept whole; then a token's place in the
+// row is the number of larger tokens before it plus that of kept equal ones.
 //
-// The histogram has 16 copies, because weights share few exponents: without
-// them a wave's additions to one word would go one after the other.
-// 2048 of 18,000 to 32,768 tokens, 4 x 32 heads: 143 us with a token per thread
-// and loop trip, every step from memory.
+// Bound by the chain of steps in one workgroup (the weights are read once:
+// they are held in registers, 4 x RUNS per thread, and only longer sequences
+// load them again in each step).  2048 of up to 32768 tokens, 4 x 32 heads: 143
+// us with a token per thread and loop trip, 37 from registers in four steps of
+// 8 bits, 22 so.  The histogram has 4 copies, by lane, because equal weights (many are
+// exactly 0) would otherwise add to one word one after the other.
 template <int RUNS, bool VEC>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
-  __shared__ uint32_t s_hist[256 * kCopies];
-  __shared__ uint32_t s_bins[256];
+  __shared__ uint32_t s_hist[kBins * kCopies];
   __shared__ uint32_t s_wave[RUNS][kKeepWaves];
   __shared__ uint32_t s_pick[3];
   const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -90,66 +91,62 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     for (int i = 0; i < RUNS; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
         const float x = w[i][e] + 0.f;
-        key[i][e] = x == x ? order_key(x) : 0u;
+        uint32_t k = x == x ? order_key(x) : 0u;
+        k = j < lo || j >= hi ? 0xFFFFFFFFu : k;
+        key[i][e] = j < L ? k : 0u;  // (behind every token, so never kept)
       }
   };
 
-  uint32_t need = a.keep - a.sink - a.recent, prefix = 0u, mask = 0u;
+  uint32_t need = a.keep, prefix = 0u, mask = 0u;
   const bool one = L <= segment;
   if (one) load(0u);
-  for (int shift = 24; shift >= 0 && need != 0u; shift -= 8) {
+  for (int step = 0; step < 3; ++step) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0;
+    const uint32_t digit = step == 2 ? 1023u : 2047u;
 #pragma unroll
-    for (uint32_t i = 0; i < 256u * kCopies / kKeepThreads; ++i) s_hist[i * kKeepThreads + tid] = 0u;
+    for (uint32_t i = 0; i < kBins * kCopies / kKeepThreads; ++i)
+      s_hist[i * kKeepThreads + tid] = 0u;
     __syncthreads();
-    for (uint32_t seg = 0; seg < hi; seg += segment) {
+    for (uint32_t seg = 0; seg < L; seg += segment) {
       if (!one) load(seg);
 #pragma unroll
-      for (int i = 0; i < RUNS; ++i) {
-        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid;
+      for (int i = 0; i < RUNS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (j + e >= lo && j + e < hi && (key[i][e] & mask) == prefix)
-            atomicAdd(&s_hist[(key[i][e] >> shift & 255u) * kCopies + lane % kCopies], 1u);
-      }
+          if ((key[i][e] & mask) == prefix)
+            atomicAdd(&s_hist[(key[i][e] >> shift & digit) * kCopies + lane % kCopies], 1u);
     }
     __syncthreads();
-    if (tid < 256u) {
-      uint32_t n = 0u;
+    // thread t has bins 2047 - 2 t and the one below
+    const uint4 x = reinterpret_cast<const uint4*>(s_hist)[kBins - 1u - 2u * tid];
+    const uint4 y = reinterpret_cast<const uint4*>(s_hist)[kBins - 2u - 2u * tid];
+    const uint32_t n0 = x.x + x.y + x.z + x.w, n1 = y.x + y.y + y.z + y.w;
+    uint32_t upto = n0 + n1;
 #pragma unroll
-      for (uint32_t i = 0; i < kCopies; ++i) n += s_hist[tid * kCopies + (tid + i) % kCopies];
-      s_bins[tid] = n;
+    for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
+      const uint32_t z = __shfl_up(upto, d);
+      if (lane >= d) upto += z;
     }
+    if (lane == kWave - 1u) s_wave[0][wave] = upto;
     __syncthreads();
-    if (wave == 0u) {  // lane l has bins 255 - 4 l and the three below
-      uint32_t n[4], sum = 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += n[i] = s_bins[255u - 4u * lane - (uint32_t)i];
-      uint32_t upto = sum;
-#pragma unroll
-      for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
-        const uint32_t x = __shfl_up(upto, d);
-        if (lane >= d) upto += x;
-      }
-      uint32_t left = need - (upto - sum);  // (wraps past the bin sought: no lane's then)
-      if (upto - sum < need && need <= upto) {
-        int i = 0;
-        while (n[i] < left) left -= n[i++];
-        s_pick[0] = 255u - 4u * lane - (uint32_t)i;
-        s_pick[1] = left;
-        s_pick[2] = n[i];
-      }
+    for (uint32_t i = 0; i < kKeepWaves; ++i) upto += i < wave ? s_wave[0][i] : 0u;
+    const uint32_t before = upto - n0 - n1;
+    if (before < need && need <= upto) {
+      const bool second = need > before + n0;
+      s_pick[0] = kBins - 1u - 2u * tid - (second ? 1u : 0u);
+      s_pick[1] = need - before - (second ? n0 : 0u);
+      s_pick[2] = second ? n1 : n0;
     }
     __syncthreads();
     prefix |= s_pick[0] << shift;
-    mask |= 255u << shift;
+    mask |= digit << shift;
     need = s_pick[1];
     if (need == s_pick[2]) break;  // the bin is kept whole
   }
 
-  // kept: the forced ones, those above `prefix` under `mask`, and the first
-  // `need` of those at it
-  const bool any = a.keep > a.sink + a.recent;
+  // kept: the tokens above `prefix` under `mask`, and the first `need` at it
   uint32_t above = 0u, ties = 0u;  // in the runs before
   for (uint32_t seg = 0; seg < L; seg += segment) {
     if (!one) load(seg);
@@ -159,11 +156,8 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
       mine[i] = 0u;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
-        const bool forced = j < lo || j >= hi;
         const uint32_t k = key[i][e] & mask;
-        if (j < L && (forced || (any && k > prefix))) mine[i] += 1u;
-        else if (j < L && any && k == prefix) mine[i] += 1u << 16;
+        mine[i] += k > prefix ? 1u : k == prefix ? 1u << 16 : 0u;
       }
       upto[i] = mine[i];
     }
@@ -190,18 +184,15 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
       }
       before += upto[i] - mine[i];
       uint32_t n = above + (before & 0xFFFFu), t = ties + (before >> 16);
+      if (mine[i] != 0u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
-        const bool forced = j < lo || j >= hi;
-        const uint32_t k = key[i][e] & mask;
-        if (j >= L) continue;
-        if (forced || (any && k > prefix)) {
-          out[n + (t < need ? t : need)] = (int32_t)j;
-          ++n;
-        } else if (any && k == prefix) {
-          if (t < need) out[n + t] = (int32_t)j;
-          ++t;
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t j = seg + (uint32_t)i * kRun + 4u * tid + (uint32_t)e;
+          const uint32_t k = key[i][e] & mask;
+          if (k > prefix || (k == prefix && t < need))
+            out[n + (t < need ? t : need)] = (int32_t)j;
+          n += k > prefix ? 1u : 0u;
+          t += k == prefix ? 1u : 0u;
         }
       }
       above += all & 0xFFFFu;
@@ -211,7 +202,10 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
 }
 
 // ---------------------------------------------------------------- packing
-constexpr uint32_t kPackThreads = 512;
+// threads: in place, where one workgroup takes all of a head, many; else few, so
+// that the steps of several workgroups overlap on a CU (2048 tokens of 4 x 32
+// heads to new pages, 285 MB: 512 threads 79 us, 256 71)
+constexpr int kPackThreadsInPlace = 512, kPackThreads = 256;
 
 // A workgroup takes steps of K or of V of one (kv head, sequence): each lane
 // group of D / 8 lanes holds MOST tokens at a time (whole pages where a page is
@@ -220,9 +214,9 @@ constexpr uint32_t kPackThreads = 512;
 // head's steps in order: a token's new slot is never behind its old one, so
 // a step that has been loaded whole overwrites no later step's tokens.  Else
 // the steps of a head are dealt to gridDim.z / 2 workgroups.
-template <int D, int MOST>
-__global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
-  constexpr uint32_t kLanes = D / 8, kGroups = kPackThreads / kLanes;
+template <int D, int MOST, int THREADS>
+__global__ __launch_bounds__(THREADS) void compact_kernel(CompactArgs a) {
+  constexpr uint32_t kLanes = D / 8, kGroups = THREADS / kLanes;
   constexpr uint32_t kTokens = kGroups * MOST;  // of a step, at most
   __shared__ uint32_t s_page[kTokens], s_slot[kTokens];
   const uint32_t h = blockIdx.x, b = blockIdx.y, which = blockIdx.z % 2u;
@@ -238,9 +232,9 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
 
   for (uint32_t j0 = blockIdx.z / 2u * step; j0 < n; j0 += gridDim.z / 2u * step) {
     __syncthreads();  // the step before is stored
-    float w[(kTokens + kPackThreads - 1) / kPackThreads];
+    float w[(kTokens + THREADS - 1) / THREADS];
 #pragma unroll
-    for (uint32_t i = 0; i < kTokens; i += kPackThreads) {
+    for (uint32_t i = 0; i < kTokens; i += THREADS) {
       const uint32_t t = i + tid;
       if (t < step && j0 + t < n) {
         uint32_t j = (uint32_t)kept[j0 + t];
@@ -250,7 +244,7 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
         s_page[t] = page;
         s_slot[t] = slot;
         if (which == 0u && a.weights != nullptr)
-          w[i / kPackThreads] = a.weights[((size_t)page * a.H + h) * S + slot];
+          w[i / THREADS] = a.weights[((size_t)page * a.H + h) * S + slot];
       }
     }
     __syncthreads();
@@ -268,7 +262,7 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
-    H8 kmax, kmin;
+    H8 kmax, kmin, mean;
     float sum[kVec];
     uint32_t e = 0u, p = p0;
 #pragma unroll
@@ -299,7 +293,6 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
           st16(a.meta + elem_off(a.g, page, 0, h, me) + l * kVec, kmax);
           st16(a.meta + elem_off(a.g, page, 1, h, me) + l * kVec, kmin);
         } else {
-          H8 mean;
 #pragma unroll
           for (int j = 0; j < kVec; ++j) mean.v[j] = r16(sum[j] / (float)e);
           st16(a.v_mean + ((size_t)to * a.H + h) * D + l * kVec, mean);
@@ -310,12 +303,12 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
       }
     }
     // the log-norms (in a loop of their own: once per token above would be
-    // most of the code)
+    // most of the code); several pages' means are this lane's own stores
     if (which == 1u) {
 #pragma nounroll
       for (uint32_t q = 0; q * S < c; ++q) {
-        const size_t at = (size_t)(uint32_t)new_ids[p0 + q] * a.H + h;
-        const H8 mean = ld16(a.v_mean + at * D + l * kVec);  // (this lane's own store)
+        const size_t at = (size_t)(pages == 1u ? to : (uint32_t)new_ids[p0 + q]) * a.H + h;
+        if (pages != 1u) mean = ld16(a.v_mean + at * D + l * kVec);
         f16 norm;
         if constexpr (kLanes == (uint32_t)kLanesPerRow) norm = log_norm_row(mean);
         else norm = grp_log_norm<kLanes>(mean, l);
@@ -324,27 +317,32 @@ __global__ __launch_bounds__(kPackThreads) void compact_kernel(CompactArgs a) {
     }
     if (which == 0u && a.weights != nullptr) {
 #pragma unroll
-      for (uint32_t i = 0; i < kTokens; i += kPackThreads) {
+      for (uint32_t i = 0; i < kTokens; i += THREADS) {
         const uint32_t t = i + tid;
         if (t < step && j0 + t < n) {
           const uint32_t q = div_page(j0 + t, a.page_rcp);
           a.weights[((size_t)(uint32_t)new_ids[q] * a.H + h) * S + (j0 + t - q * S)] =
-              w[i / kPackThreads];
+              w[i / THREADS];
         }
       }
     }
   }
 }
 
-template <int D>
+template <int D, int THREADS>
 void launch_pack(const CompactArgs& a, uint32_t batch, hipStream_t s) {
   const uint32_t most = a.S > 16u ? 32u : 16u;
-  const uint32_t step = kPackThreads / (D / 8) * (a.S < most ? most / a.S * a.S : a.S);
+  const uint32_t step = THREADS / (D / 8) * (a.S < most ? most / a.S * a.S : a.S);
   const uint64_t steps = ((uint64_t)a.keep + step - 1u) / step;
   const uint32_t z = a.in_place ? 1u : (uint32_t)(steps < 16384u ? steps : 16384u);
-  const dim3 grid(a.H, batch, 2u * z), block(kPackThreads);
-  if (most == 16u) hipLaunchKernelGGL((compact_kernel<D, 16>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((compact_kernel<D, 32>), grid, block, 0, s, a);
+  const dim3 grid(a.H, batch, 2u * z), block(THREADS);
+  if (most == 16u) hipLaunchKernelGGL((compact_kernel<D, 16, THREADS>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((compact_kernel<D, 32, THREADS>), grid, block, 0, s, a);
+}
+template <int D>
+void launch_pack(const CompactArgs& a, uint32_t batch, hipStream_t s) {
+  if (a.in_place) launch_pack<D, kPackThreadsInPlace>(a, batch, s);
+  else launch_pack<D, kPackThreads>(a, batch, s);
 }
 
 uint32_t rcp_of(uint32_t S) { return S == 1u ? 0u : (uint32_t)((1ull << 32) / S) + 1u; }
