@@ -1,6 +1,8 @@
 // Eviction from the paged cache (gfx950): which tokens each kv head keeps by
 // the attention weight they received, and the cache packed down to them with
 // its page statistics.
+#include <type_traits>
+
 #include "kernels.hpp"
 
 namespace aoakv {
@@ -204,7 +206,8 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
 // ---------------------------------------------------------------- packing
 // threads: in place, where one workgroup takes all of a head, many; else few, so
 // that the steps of several workgroups overlap on a CU (2048 tokens of 4 x 32
-// heads to new pages, 285 MB: 512 threads 79 us, 256 71)
+// heads to new pages, 285 MB: 512 threads 79 us, 256 68; 59 with K and V as
+// code of their own below, 4.8 TB/s, the rate of a large copy)
 constexpr int kPackThreadsInPlace = 512, kPackThreads = 256;
 
 // A workgroup takes steps of K or of V of one (kv head, sequence): each lane
@@ -264,44 +267,50 @@ __global__ __launch_bounds__(THREADS) void compact_kernel(CompactArgs a) {
     }
     H8 kmax, kmin, mean;
     float sum[kVec];
-    uint32_t e = 0u, p = p0;
+    // (K and V each with their own code: half as many instructions to fetch)
+    auto store = [&](auto is_v) {
+      constexpr bool kV = is_v.value;
+      uint32_t e = 0u, p = p0;
 #pragma unroll
-    for (uint32_t t = 0; t < (uint32_t)MOST; ++t) {
-      if (t >= c) continue;
-      if (e == 0u) {
+      for (uint32_t t = 0; t < (uint32_t)MOST; ++t) {
+        if (t >= c) continue;
+        if (e == 0u) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            kmax.v[j] = (f16)-65504.0f;  // as a bulk append starts a page
+            kmin.v[j] = (f16)65504.0f;
+            sum[j] = 0.f;
+          }
+        }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
-          kmax.v[j] = (f16)-65504.0f;  // as a bulk append starts a page
-          kmin.v[j] = (f16)65504.0f;
-          sum[j] = 0.f;
+          if constexpr (!kV) {
+            kmax.v[j] = x[t].v[j] > kmax.v[j] ? x[t].v[j] : kmax.v[j];
+            kmin.v[j] = x[t].v[j] < kmin.v[j] ? x[t].v[j] : kmin.v[j];
+          } else {
+            sum[j] = sum[j] + (float)x[t].v[j];
+          }
         }
-      }
+        st16(a.kv + elem_off(a.g, to, which, h, e) + l * kVec, x[t]);
+        if (++e == S || t + 1u == c) {  // the page's last token
+          if constexpr (!kV) {
+            const uint32_t mp = div_page(p, a.page_rcp), me = p - mp * S;
+            const uint32_t page = (uint32_t)meta_ids[mp];
+            st16(a.meta + elem_off(a.g, page, 0, h, me) + l * kVec, kmax);
+            st16(a.meta + elem_off(a.g, page, 1, h, me) + l * kVec, kmin);
+          } else {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        if (which == 0u) {
-          kmax.v[j] = x[t].v[j] > kmax.v[j] ? x[t].v[j] : kmax.v[j];
-          kmin.v[j] = x[t].v[j] < kmin.v[j] ? x[t].v[j] : kmin.v[j];
-        } else {
-          sum[j] = sum[j] + (float)x[t].v[j];
+            for (int j = 0; j < kVec; ++j) mean.v[j] = r16(sum[j] / (float)e);
+            st16(a.v_mean + ((size_t)to * a.H + h) * D + l * kVec, mean);
+          }
+          e = 0u;
+          ++p;
+          if (t + 1u < c) to = (uint32_t)new_ids[p];
         }
       }
-      st16(a.kv + elem_off(a.g, to, which, h, e) + l * kVec, x[t]);
-      if (++e == S || t + 1u == c) {  // the page's last token
-        if (which == 0u) {
-          const uint32_t mp = div_page(p, a.page_rcp), me = p - mp * S;
-          const uint32_t page = (uint32_t)meta_ids[mp];
-          st16(a.meta + elem_off(a.g, page, 0, h, me) + l * kVec, kmax);
-          st16(a.meta + elem_off(a.g, page, 1, h, me) + l * kVec, kmin);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) mean.v[j] = r16(sum[j] / (float)e);
-          st16(a.v_mean + ((size_t)to * a.H + h) * D + l * kVec, mean);
-        }
-        e = 0u;
-        ++p;
-        if (t + 1u < c) to = (uint32_t)new_ids[p];
-      }
-    }
+    };
+    if (which == 0u) store(std::false_type{});
+    else store(std::true_type{});
     // the log-norms (in a loop of their own: once per token above would be
     // most of the code); several pages' means are this lane's own stores
     if (which == 1u) {
