@@ -74,6 +74,7 @@ class QuestAttention(nn.Module):
         self.rope_scale = cfg.rope_scale
         self.rope_theta = cfg.rope_theta
         self.single_launch = single_launch
+        self.observe_last = 32  # queries of a prompt whose attention an eviction goes by
         self.q_proj = nn.Linear(self.hidden_size, self.num_heads * self.head_dim, bias=False)
         self.k_proj = nn.Linear(self.hidden_size, self.num_key_value_heads * self.head_dim,
                                 bias=False)
@@ -94,7 +95,12 @@ class QuestAttention(nn.Module):
         with tr.range("RoPE+append_kv"):
             qutils.rope_append_kv(q, k, v, c, self.layer_idx, rope_scale=self.rope_scale,
                                   rope_theta=self.rope_theta)
-        if q_len > 1:
+        if q_len > 1 and c.tracks_weights:
+            with tr.range("prefill_attn"):
+                o, lse = qutils.chunk_forward(q, c, self.layer_idx, return_lse=True)
+            with tr.range("observe"):
+                qutils.observe(q, lse, c, self.layer_idx, last=self.observe_last)
+        elif q_len > 1:
             with tr.range("prefill_attn"):
                 o = qutils.prefill_forward(q, c, self.layer_idx)
         elif not c.need_estimate():
@@ -172,8 +178,13 @@ class QuestLlamaModel(nn.Module):
 
     def quest_init(self, page_size: int, max_seq_len: int, token_budget: int = 512,
                    dtype=torch.float16, device="cuda:0", value_aware: bool = True,
-                   semantics: str = "sim", layout: int = TensorLayout.HND):
-        """Allocates the paged caches for max_seq_len tokens (llama.py:520-552)."""
+                   semantics: str = "sim", layout: int = TensorLayout.HND,
+                   evict_keep: Optional[int] = None, evict_sink: int = 4,
+                   evict_recent: int = 32):
+        """Allocates the paged caches for max_seq_len tokens (llama.py:520-552).
+        evict_keep: after each prompt, every layer's cache is cut down to that
+        many tokens per kv head: the first evict_sink, the last evict_recent, and
+        those that the prompt's last queries attend to most."""
         assert self.iController is None, "Can't init Quest Controller twice."
         cfg = self.cfg
         self._page_budget = token_budget // page_size
@@ -182,6 +193,12 @@ class QuestLlamaModel(nn.Module):
             cfg.hidden_size // cfg.num_attention_heads, page_size, self._page_budget,
             max_seq_len, dtype, device, layout=layout, num_kv_heads=cfg.num_key_value_heads,
             value_aware=value_aware, semantics=semantics)
+        self._evict = None
+        if evict_keep is not None:
+            if evict_sink + evict_recent > evict_keep:
+                raise ValueError("evict_sink + evict_recent must not exceed evict_keep")
+            self._evict = (evict_keep, evict_sink, evict_recent)
+            self.iController.track_weights()
 
     def quest_clear(self):
         """Frees the sequence's pages for a new conversation (llama.py:554-560)."""
@@ -198,7 +215,10 @@ class QuestLlamaModel(nn.Module):
         if self._skip > 0:
             c.set_page_budget(self._max_page_limit)
             c.begin_forward(seq_len)
-        return self._layers(inputs_embeds, seq_len, tables_written=self._skip > 0)
+        h = self._layers(inputs_embeds, seq_len, tables_written=self._skip > 0)
+        if seq_len > 1 and self._evict is not None:
+            c.evict(*self._evict)
+        return h
 
     def _layers(self, h: torch.Tensor, seq_len: int, tables_written: bool) -> torch.Tensor:
         """The decoder layers and the final norm, switching to the page budget
@@ -230,11 +250,14 @@ class QuestLlamaModel(nn.Module):
         (the sequence outgrew the page budget), and the graph is captured
         again when it does.  The returned tensor is the graph's output
         buffer, overwritten by the next step.  Same results as ``forward``
-        (the page bound sizes grids only)."""
+        (the page bound sizes grids only).  After an eviction the steps run
+        eagerly: a token's position is then an argument from the host."""
         c = self.iController
         assert c is not None, "Please init Quest Controller first."
         assert tuple(inputs_embeds.shape[:2]) == (1, 1), "one token per decode step"
         assert not c.debug_checks, "debug_checks synchronize; not inside a graph"
+        if c.evicted:
+            return self.forward(inputs_embeds)
         if not getattr(self, "_graph_warm", False):
             # the first single-token step runs eagerly: the GEMM libraries set
             # up their single-row paths on first use, which a capture cannot do

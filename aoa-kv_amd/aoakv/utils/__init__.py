@@ -15,6 +15,14 @@ Same names, same argument meaning, same call order as QuestAttention.forward
 other ``topk_indices`` tensor of physical page ids, ``[Hkv, n]``, is attended
 as given (with the quest_kernel convention the last page is added, as the
 reference's ``decode_sparse_attn`` does with ``kv_last_page_idx``).
+
+Beyond the reference, a cache can be cut down to the tokens that attention goes
+to::
+
+    ctrl.track_weights()
+    o, lse = chunk_forward(q, ctrl, layer, return_lse=True)   # N >= 1 new tokens
+    observe(q, lse, ctrl, layer)                  # each token's weight is added up
+    ctrl.evict(keep, sink, recent)                # between forward passes
 """
 from __future__ import annotations
 
@@ -37,6 +45,8 @@ __all__ = [
     "append_kv",
     "rope_append_kv",
     "prefill_forward",
+    "chunk_forward",
+    "observe",
     "decode_estimate",
     "decode_topk",
     "decode_sparse_attn",
@@ -69,10 +79,16 @@ def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     reference's two calls at QuestAttention.py:98-111 -- in one launch (a
     prompt at the shapes ops.rope_append_kv_cache_prefill names).  q and k are
     left rotated, as the reference leaves them.  Call after begin_forward, like
-    append_kv."""
+    append_kv.  After an eviction, when a token's position is no longer its slot,
+    these are the two calls."""
     c = iController
     scale = 1.0 if rope_scale is None else rope_scale
     theta = 1e4 if rope_theta is None else rope_theta
+    if c.evicted:
+        ops.apply_rope_in_place(q.view(k.size(0), -1, c.head_dim), k,
+                                c.kv_cache.seqlen + c.evicted - k.size(0), scale, theta)
+        append_kv(k, v, c, layer_idx)
+        return
     if k.size(0) > 1:
         ops.rope_append_kv_cache_prefill(
             q, k, v, c.kv_cache.buf_layer(layer_idx), c.kv_indices_with_last,
@@ -116,6 +132,41 @@ def prefill_forward(q: torch.Tensor, iController: InferenceController, layer_idx
     return ops.prefill_with_paged_kv_cache(
         q, c.kv_cache.buf_layer(layer_idx), c.kv_indices_with_last, len(c.kv_cache.indicies),
         c.kv_cache.last_page_len, c.layout, causal=True)
+
+
+def chunk_forward(q: torch.Tensor, iController: InferenceController, layer_idx: int,
+                  window: int = 0, soft_cap: float = 0.0,
+                  slopes: Optional[torch.Tensor] = None,
+                  prefix_len: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Causal attention of the new tokens q [N, H, D] (N >= 1) over the cache with
+    the options of ``ops.chunk_attn``; with ``return_lse`` (o, lse).  Distances
+    and windows count cache slots, so after an eviction not positions."""
+    c = iController
+    c._q_indptr[1].fill_(q.size(0))
+    return ops.chunk_attn(q, c._q_indptr, c.kv_cache.buf_layer(layer_idx),
+                          c.kv_indptr_for_append, c.kv_indices_with_last, c.kv_last_page_len_t,
+                          c.decode_max_pages, c.layout, window=window, soft_cap=soft_cap,
+                          slopes=slopes, prefix_len=prefix_len, return_lse=return_lse,
+                          workspace=c.workspace)
+
+
+def observe(q: torch.Tensor, lse: torch.Tensor, iController: InferenceController, layer_idx: int,
+            last: Optional[int] = None, window: int = 0, soft_cap: float = 0.0,
+            slopes: Optional[torch.Tensor] = None, prefix_len: Optional[torch.Tensor] = None):
+    """Adds the attention weight of the new tokens' queries (``last``: of their
+    last ones alone) to the sums that ``iController.evict`` goes by; q, lse and
+    the options as ``chunk_forward`` had and gave them.  The new tokens' own sums
+    start from 0."""
+    c = iController
+    n = q.size(0)
+    rows = n if last is None else max(1, min(last, n))
+    c._start[0].fill_(c.kv_cache.seqlen - n)
+    c._q_indptr[1].fill_(rows)
+    ops.attn_weights(q[n - rows:], lse[n - rows:], c._q_indptr, c.attn_weights_layer(layer_idx),
+                     c.kv_cache.buf_layer(layer_idx), c.kv_indptr_for_append,
+                     c.kv_indices_with_last, c.kv_last_page_len_t, c.decode_max_pages, c.layout,
+                     window=window, soft_cap=soft_cap, slopes=slopes, prefix_len=prefix_len,
+                     start=c._start, workspace=c.workspace)
 
 
 def decode_estimate(q: torch.Tensor, iController: InferenceController, layer_idx: int

@@ -71,6 +71,12 @@ class InferenceController:
         self.v_mean = torch.zeros((num_layers, max_kv_pages, self.num_kv_heads, head_dim),
                                   dtype=dtype, device=device)
 
+        # eviction: the attention weight each cached token received (track_weights),
+        # and the tokens dropped so far (the next token's position is seqlen +
+        # evicted)
+        self._attn_weights = None
+        self.evicted = 0
+
         self._page_budget = page_budget
         self.inference_page_budget = None
 
@@ -93,6 +99,9 @@ class InferenceController:
         self._kv_indptr = torch.zeros(2, **i32)
         self._md_indptr = torch.zeros(2, **i32)
         self._lpl = torch.zeros(1, **i32)
+        # rows of a chunk and where its tokens begin (utils.chunk_forward, observe)
+        self._q_indptr = torch.zeros(2, **i32)
+        self._start = torch.zeros(1, **i32)
         self._up = {"kv": 0, "md": 0, "P": 0, "Pm": 0, "lpl": 0}
 
         # fixed-size decode buffers (one layer at a time)
@@ -238,7 +247,58 @@ class InferenceController:
                 what.append("a page table held more pages than the call was sized for")
             raise RuntimeError("aoakv decode workspace error: " + "; ".join(what))
 
+    # ------------------------------------------------------------ eviction
+    def track_weights(self):
+        """Allocate the sums of attention weight per layer, page, kv head and
+        slot (fp32), which utils.observe adds to and evict goes by."""
+        if self._attn_weights is None:
+            self._attn_weights = torch.zeros(
+                (self.num_layers, self.max_kv_pages, self.num_kv_heads, self.page_size),
+                dtype=torch.float32, device=self.device).unbind(0)
+
+    @property
+    def tracks_weights(self) -> bool:
+        return self._attn_weights is not None
+
+    def attn_weights_layer(self, layer_idx: int) -> torch.Tensor:
+        if self._attn_weights is None:
+            raise RuntimeError("track_weights() was not called")
+        return self._attn_weights[layer_idx]
+
+    def evict(self, keep: int, sink: int = 0, recent: int = 0) -> int:
+        """Drop all but ``keep`` tokens of every layer and kv head: the first
+        ``sink``, the last ``recent`` and those of the others that received the
+        most attention weight (utils.observe).  The caches are packed in place,
+        with their page statistics, the pages behind are given back, and the
+        tokens keep the rotation of the positions they had.  Call it between
+        forward passes (after every layer's append); the next begin_forward
+        writes the shorter tables.  Returns the number of tokens dropped (0:
+        there were no more than ``keep``)."""
+        L = self.kv_cache.seqlen
+        if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
+            raise ValueError(f"keep {keep}, sink {sink}, recent {recent}: sink + recent <= keep")
+        self.attn_weights_layer(0)
+        if L <= keep:
+            return 0
+        table = (self.kv_indptr_for_append, self.kv_indices_with_last, self.kv_last_page_len_t)
+        P = len(self.kv_cache.indicies)
+        kept = torch.empty((1, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
+        for i in range(self.num_layers):
+            w = self._attn_weights[i]
+            ops.keep_tokens(w, *table, keep, kept, P, sink=sink, recent=recent,
+                            workspace=self.workspace)
+            ops.compact_kv_cache(
+                kept, keep, self.kv_cache.buf_layer(i), *table, None, None,
+                self.metadata_cache.buf_layer(i), self.metadata_indptr_for_append,
+                self.metadata_indices, self.v_log_norm_layer(i), self.v_mean_layer(i), P,
+                self.layout, weights=w, workspace=self.workspace)
+        self.kv_cache.truncate(keep)
+        self.metadata_cache.truncate(len(self.kv_cache.indicies))
+        self.evicted += L - keep
+        return L - keep
+
     def clean_states(self):
+        self.evicted = 0
         self.kv_cache.release()
         self.metadata_cache.release()
         self._up.update(kv=0, md=0)

@@ -120,6 +120,17 @@ class KvCache:
         self._seqlen = total
         return len(self._indicies) - had
 
+    def truncate(self, seq_len: int) -> int:
+        """Keep the first seq_len tokens' slots and give the other pages back;
+        return the number of pages given back."""
+        if not 0 <= seq_len <= self._seqlen:
+            raise ValueError(f"{seq_len} tokens of {self._seqlen} cannot be kept")
+        page, had = self._pool.block_len, len(self._indicies)
+        while len(self._indicies) * page >= seq_len + page:
+            self._pool.free_block(self._indicies.pop())
+        self._seqlen = seq_len
+        return had - len(self._indicies)
+
     def release(self):
         self._seqlen = 0
         for idx in self._indicies:
