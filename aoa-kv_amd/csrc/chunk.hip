@@ -24,8 +24,16 @@
 // context and a long prompt all end at the same time.  An item that lies in one
 // share is finished there; the parts of one that does not go to the workspace,
 // two slots per workgroup (the part that its share begins with, and the one it
-// ends with), and a second launch joins them in order.  Nothing depends on
-// timing: equal calls give equal bits.
+// ends with), and a second launch joins them in order.  Where the call's rows make
+// an item for every workgroup that the GPU holds, the attention's items are listed
+// by a launch of one workgroup instead, the longest first, a workgroup each, and
+// only those longer than an equal share are cut.  Nothing depends on timing: equal
+// calls give equal bits.
+//
+// Registers.  No kernel here may spill one: the allocator, keeping part of a
+// spilled 128-bit tuple in an accumulation register, lost its fourth dword (head
+// dim 256, odd pages, listed: every score was wrong).  Fragments are read in
+// batches, and offsets made where they are used, as far as that takes.
 #include "kernels.hpp"
 #include "mfma_tile.hpp"
 
@@ -283,7 +291,9 @@ struct Cut {
   uint32_t n, h, b;
   int32_t x, q0, rows;
   uint32_t first, step;
-  __device__ size_t slot(uint32_t i) const { return i == 0u ? first : first + 1u + (i - 1u) * step; }
+  __device__ size_t slot(uint32_t i) const {
+    return i == 0u ? first : first + 1u + (i - 1u) * step;
+  }
 };
 // The item that the border before workgroup `place`'s share cuts, where that is
 // its first cut: slot 1 of the workgroup before, slot 0 of the following ones.
@@ -448,8 +458,17 @@ __global__ __launch_bounds__(kChThreads) void chunk_list_kernel(ChunkArgs a, uin
   }
 }
 
-// One workgroup's share, or its entry of the list.  The tile loop is that of prefill.hip (S^T = K Q^T,
-// lane l holds row l % 32 of its wave's 32); scores are kept in units of log 2.
+// One workgroup's share, or its entry of the list.  The tile loop is that of
+// prefill.hip (S^T = K Q^T, lane l holds row l % 32 of its wave's 32); scores are
+// kept in units of log 2.
+//
+// What bounds it: a tile's K and V fragments pass from LDS to the matrix cores at
+// 128 bytes a clock and CU, the rate at which the products consume them, and the
+// exponentials take as long again; two workgroups per CU run one beside the other.
+// 8192 tokens over themselves, causal: 32 heads of 128 600 us (920 TFLOP/s; 8 kv
+// heads the same), with slopes 660, a cap 690; 16 heads of 256 740; 32 of 64 355;
+// few rows over a long cache pass 5.4 TB/s.  64 rows per wave, which halves
+// the fragments, left one wave per SIMD and took 920 us.
 template <int D, int MOD, bool S16, bool LIST>
 __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kernel(ChunkArgs a) {
   using Sh = PfShape<D>;
@@ -687,7 +706,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         half8 kf0[Sh::kKS], kf1[Sh::kKS];
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8)
-          kf0[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(sK + k_at(s8));
+          kf0[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+              sK + k_at(s8));
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8)
           kf1[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
@@ -700,7 +720,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[1] = mfma32(kf1[s8], qreg[s8], acc_s[1]);
       } else {
-        constexpr int kB = 8, kNB = 2 * Sh::kKS / kB;  // batches of 8 fragments
+        constexpr int kB = 4, kNB = 2 * Sh::kKS / kB;  // batches of 4 fragments
+        // (batches of 8 spilled up to 35 registers and took 755 us at 8192 tokens for 740)
         auto kread = [&](int bt, half8 (&kf)[kB]) {
 #pragma unroll
           for (int j = 0; j < kB; ++j)
@@ -1037,8 +1058,9 @@ constexpr uint32_t kWholeTiles = 4u;
 
 // One workgroup's share of the items.  Scores are S = Q K^T: a wave holds its
 // keys in registers (lane l: keys l % 32, + 32) and reads 32 query rows at a time
-// from LDS, so a key's sum is a sum over a lane's own registers.  Each 32 rows are added up by themselves first: one chain of
-// single additions over 16384 rows was 2e-6 off.
+// from LDS, so a key's sum is a sum over a lane's own registers.  Each 32 rows are
+// added up by themselves first: one chain of single additions over 16384 rows was
+// 2e-6 off.
 template <int D, int MOD, bool BIG>
 __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_weights_kernel(
     ChunkArgs a) {
@@ -1085,9 +1107,11 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
   constexpr int kNI = kWaveRows / Sh::kRPI;
   constexpr int kRow32 = 32 * Sh::kRowBytes;
   const int lrow = lane / Sh::kCh, lslot = lane % Sh::kCh;
-  int q_off[Sh::kKS];
+  // (offsets as in the attention kernel: with slopes they are made where they are used)
+  constexpr bool kXor = (MOD & kBias) != 0;
+  int q_off[kXor ? 1 : Sh::kKS];
 #pragma unroll
-  for (int s8 = 0; s8 < Sh::kKS; ++s8) q_off[s8] = tile_off<D>(c, 2 * s8 + g);
+  for (int s8 = 0; s8 < (kXor ? 1 : Sh::kKS); ++s8) q_off[s8] = tile_off<D>(c, 2 * s8 + g);
   const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
   const float cap2 = a.soft_cap * kLog2e;
   const float cap_in = MOD & kCap ? a.sm_scale / a.soft_cap : 0.f;
@@ -1161,29 +1185,31 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
       int32_t pos[16];
     };
     auto read_q = [&](const lds_char* sQ, int half, half8 (&q)[Sh::kKS]) {
+      if constexpr (kXor) asm volatile("" : "+v"(q_off[0]));
 #pragma unroll
       for (int s8 = 0; s8 < Sh::kKS; ++s8)
         q[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-            sQ + q_off[s8] + half * kRow32);
+            sQ + (kXor ? q_off[0] ^ (32 * s8) : q_off[s8 % Sh::kKS]) + half * kRow32);
+    };
+    auto read_quad = [&](int v, int half, Rows& x, bool pos, int q4) {
+      const int at = 32 * half + 8 * q4 + 4 * g;  // rows crow(4 q4, g) ..
+      const float4 n = *reinterpret_cast<const float4*>(&s_neg[v][at]);
+      x.neg[4 * q4] = n.x, x.neg[4 * q4 + 1] = n.y, x.neg[4 * q4 + 2] = n.z,
+      x.neg[4 * q4 + 3] = n.w;
+      if (MOD & kBias || pos) {
+        const int4 y = *reinterpret_cast<const int4*>(&s_pos[v][at]);
+        x.pos[4 * q4] = y.x, x.pos[4 * q4 + 1] = y.y, x.pos[4 * q4 + 2] = y.z,
+        x.pos[4 * q4 + 3] = y.w;
+      }
+      if constexpr (MOD & kBias) {
+        const float4 y = *reinterpret_cast<const float4*>(&s_slope[v][at]);
+        x.slope[4 * q4] = y.x, x.slope[4 * q4 + 1] = y.y, x.slope[4 * q4 + 2] = y.z,
+        x.slope[4 * q4 + 3] = y.w;
+      }
     };
     auto read_rows = [&](int v, int half, Rows& x, bool pos) {
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int at = 32 * half + 8 * q4 + 4 * g;  // rows crow(4 q4, g) ..
-        const float4 n = *reinterpret_cast<const float4*>(&s_neg[v][at]);
-        x.neg[4 * q4] = n.x, x.neg[4 * q4 + 1] = n.y, x.neg[4 * q4 + 2] = n.z,
-        x.neg[4 * q4 + 3] = n.w;
-        if (MOD & kBias || pos) {
-          const int4 y = *reinterpret_cast<const int4*>(&s_pos[v][at]);
-          x.pos[4 * q4] = y.x, x.pos[4 * q4 + 1] = y.y, x.pos[4 * q4 + 2] = y.z,
-          x.pos[4 * q4 + 3] = y.w;
-        }
-        if constexpr (MOD & kBias) {
-          const float4 y = *reinterpret_cast<const float4*>(&s_slope[v][at]);
-          x.slope[4 * q4] = y.x, x.slope[4 * q4 + 1] = y.y, x.slope[4 * q4 + 2] = y.z,
-          x.slope[4 * q4 + 3] = y.w;
-        }
-      }
+      for (int q4 = 0; q4 < 4; ++q4) read_quad(v, half, x, pos, q4);
     };
     // probability of register i of a product
     auto weight = [&](float t, const Rows& x, int i, int32_t key) {
@@ -1202,7 +1228,11 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
     auto whole_tile = [&](const lds_char* sQ, int v) {
       constexpr int kPer = 16 / Sh::kKS;  // elements per matrix instruction
       constexpr int kN = kRows / 32 * kSets;  // products
-      half8 q[2][Sh::kKS];
+      // (slopes and positions take the registers of a buffer, and at D = 256 are
+      // read four rows at a time: none is spilled)
+      constexpr int kQ = MOD & kBias ? 1 : 2;
+      constexpr bool kQuads = MOD & kBias && D == 256;
+      half8 q[kQ][Sh::kKS];
       Rows x;
       read_q(sQ, 0, q[0]);
       floatx16 acc[2];
@@ -1210,13 +1240,18 @@ __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_w
 #pragma unroll
       for (int n = 0; n <= kN; ++n) {  // product n, exponentials of product n - 1
         const int half = n / kSets, z = n % kSets, pz = (n + kSets - 1) % kSets;
-        if (n < kN && z == 0 && half + 1 < kRows / 32) read_q(sQ, half + 1, q[(half + 1) % 2]);
-        if (n > 0 && pz == 0) read_rows(v, (n - 1) / kSets, x, false);
+        if (kQ == 2 && n < kN && z == 0 && half + 1 < kRows / 32)
+          read_q(sQ, half + 1, q[(half + 1) % kQ]);
+        if (kQ == 1 && n > 0 && n < kN && z == 0) read_q(sQ, half, q[0]);
+        if (n > 0 && kQuads) read_quad(v, (n - 1) / kSets, x, false, 0);
+        if (n > 0 && !kQuads && pz == 0) read_rows(v, (n - 1) / kSets, x, false);
         if (n < kN) acc[n % 2] = floatx16{};
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8) {
-          if (n < kN) acc[n % 2] = mfma32(q[half % 2][s8], kf[z][s8], acc[n % 2]);
+          if (n < kN) acc[n % 2] = mfma32(q[half % kQ][s8], kf[z][s8], acc[n % 2]);
           if (n > 0) {
+            const int q4 = s8 * kPer / 4 + 1;  // (needed four elements on)
+            if (kQuads && s8 * kPer % 4 == 0 && q4 < 4) read_quad(v, (n - 1) / kSets, x, false, q4);
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
               part += weight(acc[(n + 1) % 2][s8 * kPer + e], x, s8 * kPer + e,
