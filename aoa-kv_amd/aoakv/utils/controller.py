@@ -271,9 +271,8 @@ class InferenceController:
         most attention weight (utils.observe).  The caches are packed in place,
         with their page statistics, the pages behind are given back, and the
         tokens keep the rotation of the positions they had.  Call it between
-        forward passes (after every layer's append); the next begin_forward
-        writes the shorter tables.  Returns the number of tokens dropped (0:
-        there were no more than ``keep``)."""
+        forward passes (after every layer's append).  Returns the number of
+        tokens dropped (0: there were no more than ``keep``)."""
         L = self.kv_cache.seqlen
         if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
             raise ValueError(f"keep {keep}, sink {sink}, recent {recent}: sink + recent <= keep")
@@ -295,6 +294,9 @@ class InferenceController:
         self.kv_cache.truncate(keep)
         self.metadata_cache.truncate(len(self.kv_cache.indicies))
         self.evicted += L - keep
+        # the shorter tables, for the next eviction or chunk: before the pages
+        # that were given back can be taken in another order
+        self.begin_forward(0)
         return L - keep
 
     def clean_states(self):

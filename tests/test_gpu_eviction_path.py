@@ -191,3 +191,40 @@ def test_the_model_evicts_after_its_prompt():
     assert cut.iController.evicted == 0
     with pytest.raises(ValueError, match="evict_keep"):
         _model(cfg, evict_keep=20)
+
+
+def test_two_evictions_and_a_chunk_without_a_step_between():
+    """Each goes by the tokens that the one before left, and a chunk after them
+    by the pages it was given, in whatever order they come back."""
+    from aoakv.utils import chunk_forward, observe, rope_append_kv
+    _say("[evict path] twice")
+    c = controller(layers=1)
+    c.prepare_metadata(500)
+    c.begin_forward(500)
+    q, k, v = tokens(c, 500, 1)
+    rope_append_kv(q, k, v, c, 0)
+    _, lse = chunk_forward(q, c, 0, return_lse=True)
+    observe(q, lse, c, 0)
+    first, second = 300, 100
+    sums = lambda: c.attn_weights_layer(0)[torch.tensor(c.kv_cache.indicies, device=DEV)].transpose(
+        0, 1).reshape(c.num_kv_heads, -1)[:, :c.kv_cache.seqlen].clone()
+    assert c.evict(first) == 200
+    kv, w = cached(c, 0).clone(), sums()
+    assert c.evict(second, 2, 8) == 200 and c.evicted == 400
+    for h in range(c.num_kv_heads):
+        x = w[h].clone()
+        x[:2] = x[first - 8:] = float("inf")
+        best = torch.sort(x, descending=True, stable=True)[1][:second].sort()[0]
+        assert torch.equal(cached(c, 0)[:, h], kv[:, h, best])
+    c.kv_cache._pool._free.reverse()  # (as another sequence's pages may leave the pool)
+    kept = cached(c, 0).clone()
+    c.prepare_metadata(450)
+    c.begin_forward(450)
+    q, k, v = tokens(c, 450, 2)
+    rope_append_kv(q, k, v, c, 0)
+    o = chunk_forward(q, c, 0)
+    assert torch.equal(cached(c, 0)[:, :, :second], kept)
+    assert torch.equal(cached(c, 0)[:, :, second:], torch.stack([k, v]).transpose(1, 2))
+    for i in (0, 200, 449):
+        ref = attend(q[i], cached(c, 0)[:, :, :second + i + 1])
+        assert (o[i].double() - ref).abs().max() <= 2e-3
