@@ -298,8 +298,8 @@ def chunk_attn(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, ma
     q [T, Hq, D] fp16 holds the sequences' new tokens one after the other, rows
     q_indptr[b] .. q_indptr[b + 1] - 1 (int32, device) those of sequence b, the
     last of its cached ones (the page table counts them).  A score is
-    q . k / sqrt(D), then soft_cap * tanh(score / soft_cap) (``soft_cap`` > 0),
-    then less slopes[h] * distance (``slopes`` fp32 [Hq]).  A token sees itself
+    q . k / sqrt(D), then soft_cap * tanh(score / soft_cap) (``soft_cap`` > 0, at
+    most 1024), then less slopes[h] * distance (``slopes`` fp32 [Hq]).  A token sees itself
     and what is before it (all, without ``causal``), no further back than
     ``window`` tokens with itself (> 0), and the first prefix_len[b] tokens
     (int32 [B]) in any case.  Returns o [T, Hq, D], with ``return_lse`` also
@@ -344,8 +344,9 @@ def compact_kv_cache(kept, keep: int, kv_data, kv_indptr, kv_indices, kv_last_pa
     """Packs the cache down to the kept tokens (aoakv_compact_kv_cache): slot i
     of a head's new pages gets its token kept[b, h, i], with the page statistics
     of a bulk append and, if given, the ``weights`` moved along.  ``new_indptr``
-    and ``new_indices`` None: in place, into the first pages of the old lists;
-    else into pages that no sequence of the call holds.  The metadata tables are
+    and ``new_indices`` None: in place, into the first pages of the old lists
+    (pages that sequences share may not be packed so); else into pages that no
+    sequence of the call holds.  The metadata tables are
     the new lists'."""
     _host.compact_kv_cache(kept, keep, kv_data, kv_indptr, kv_indices, kv_last_page_len,
                            new_indptr, new_indices, metadata_data, metadata_indptr,

@@ -1028,6 +1028,8 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
                     "prefill_with_paged_kv_cache");
 }
 
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16u == 0u; }
+
 // The arguments that chunk_attn and attn_weights share.
 static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indptr,
                       uint32_t num_q_tokens, const void* kv_data, const int32_t* kv_indptr,
@@ -1054,11 +1056,12 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size <= aoakv::kMaxChunkTokens,
           "%s: max_pages %u of %u tokens not in [1, 2^27 tokens]", fn, max_pages, page_size);
   REQUIRE(window < (1u << 31), "%s: window %u out of range", fn, window);
-  REQUIRE(soft_cap >= 0.f && std::isfinite(soft_cap), "%s: soft_cap %g must be >= 0", fn,
-          (double)soft_cap);
+  // (c - 2 c / (1 + e^(2 x / c)) is off by about c * 2^-23: 2e-4 of a weight at 1024)
+  REQUIRE(soft_cap == 0.f || (soft_cap >= 1e-6f && soft_cap <= 1024.f),
+          "%s: soft_cap %g is neither 0 nor in [1e-6, 1024]", fn, (double)soft_cap);
+  REQUIRE(aligned16(q) && aligned16(kv_data), "%s: q or kv_data not aligned to 16 bytes", fn);
   REQUIRE(need == 0u || workspace, "%s: null workspace", fn);
-  REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16u == 0u,
-          "%s: workspace not aligned to 16 bytes", fn);
+  REQUIRE(aligned16(workspace), "%s: workspace not aligned to 16 bytes", fn);
   REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes < %zu needed", fn, workspace_bytes,
           need);
   a.q = static_cast<const aoakv::f16*>(q);
@@ -1115,6 +1118,7 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
     return e;
   if (num_q_tokens == 0u) return ok();
   REQUIRE(o, "chunk_attn: null pointer argument");
+  REQUIRE(aligned16(o), "chunk_attn: o not aligned to 16 bytes");
   a.o = static_cast<aoakv::f16*>(o);
   a.lse = lse;
   a.cuts = workspace;
@@ -1214,6 +1218,8 @@ int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t k
           "compact_kv_cache: null pointer argument");
   REQUIRE((new_indptr == nullptr) == (new_indices == nullptr),
           "compact_kv_cache: new_indptr and new_indices are both given or both NULL");
+  REQUIRE(aligned16(kv_data) && aligned16(metadata_data) && aligned16(v_mean),
+          "compact_kv_cache: kv_data, metadata_data or v_mean not aligned to 16 bytes");
   aoakv::CompactArgs a{};
   a.kept = kept;
   a.stride = kept_stride;

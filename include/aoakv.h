@@ -479,7 +479,7 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  * q_indptr[B] - 1 are not touched.  Row i of n_b is at position pos = L_b - n_b
  * + i; for the key at position j, with dot products and softmax in fp32,
  *   t = q . k / sqrt(head_dim)
- *   t = soft_cap * tanh(t / soft_cap)      if soft_cap > 0
+ *   t = soft_cap * tanh(t / soft_cap)      if soft_cap > 0 (1e-6 .. 1024)
  *   t = t - slopes[h] * |pos - j|          if slopes ([num_qo_heads] fp32)
  * counts where j <= pos (if causal) and pos - j < window (if window > 0), and
  * for j < prefix_len[b] (int32 [B], or NULL) whatever these say: a prefix that
@@ -490,9 +490,10 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  *
  * num_qo_heads is any multiple of num_kv_heads (and, with G the quotient,
  * num_q_tokens * G < 2^30, (num_q_tokens + 128) * G * G < 2^31 where G is no
- * power of two; max_pages * page_size <= 2^27).  max_pages >= every
- * sequence's page count: a longer table is cut to it and AOAKV_WS_ERR_TRUNCATED set in
- * *error_word (NULL: not reported), as in aoakv_topk_filtering.  workspace:
+ * power of two; max_pages * page_size <= 2^27); q, o and kv_data are aligned to
+ * 16 bytes.  max_pages >= every sequence's page count: a longer table is cut to
+ * it and AOAKV_WS_ERR_TRUNCATED set in *error_word (NULL: not reported), as in
+ * aoakv_topk_filtering.  workspace:
  * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
  * initialisation and is free again when the call's work on `stream` is done.
  */
@@ -559,8 +560,10 @@ int aoakv_keep_tokens(const float* weights, const int32_t* kv_indptr, const int3
  * metadata_indices list the metadata pages of the new page list.
  * new_indptr and new_indices NULL: in place, into the first pages of the
  * sequence's own list.  Otherwise no new page may be a page of kv_indices.
- * kept: ascending positions, as aoakv_keep_tokens writes them (one past the
- * sequence's end reads its last token).  The caller then shortens its table.
+ * No page may belong to two sequences of the call (in place, to any other
+ * sequence).  kept: ascending positions, as aoakv_keep_tokens writes them (one
+ * past the sequence's end reads its last token).  kv_data, metadata_data and
+ * v_mean are aligned to 16 bytes.  The caller then shortens its table.
  */
 int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t keep,
                            void* kv_data, const int32_t* kv_indptr, const int32_t* kv_indices,

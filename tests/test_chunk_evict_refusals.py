@@ -39,7 +39,9 @@ BAD = [(dict(dim=96), "head_dim"), (dict(page=0), "page_size"), (dict(page=33), 
        (dict(max_pages=0), "max_pages"), (dict(max_pages=1 << 30), "max_pages"),
        (dict(window=1 << 31), "window"), (dict(cap=-1.0), "soft_cap"),
        (dict(cap=float("nan")), "soft_cap"), (dict(cap=float("inf")), "soft_cap"),
-       (dict(rows=1 << 31), "rows"), (dict(ws=P + 8), "16 bytes"),
+       (dict(cap=1025.0), "soft_cap"), (dict(cap=1e-7), "soft_cap"),
+       (dict(rows=1 << 31), "rows"),
+       *[({k: P + 8}, "16 bytes") for k in ("ws", "q", "o", "kv", "meta", "mean")],
        (dict(keep=0), "keep"), (dict(keep=65), "keep"), (dict(sink=40, recent=40), "sink"),
        (dict(new_indptr=None), "both"), (dict(new_indices=None), "both"),
        *[({k: None}, "null") for k in ("q", "q_indptr", "kv", "indptr", "indices", "last", "kept",
