@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kChThreads) void chunk_list_kernel(ChunkArgs a, uin
 // 128 bytes a clock and CU, the rate at which the products consume them, and the
 // exponentials take as long again; two workgroups per CU run one beside the other.
 // 8192 tokens over themselves, causal: 32 heads of 128 600 us (920 TFLOP/s; 8 kv
-// heads the same), with slopes 660, a cap 690; 16 heads of 256 740; 32 of 64 355;
+// heads the same), with slopes 630, a cap 700; 16 heads of 256 730; 32 of 64 350;
 // few rows over a long cache pass 5.4 TB/s.  64 rows per wave, which halves
 // the fragments, left one wave per SIMD and took 920 us.
 template <int D, int MOD, bool S16, bool LIST>
@@ -494,7 +494,11 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
   }
 
-  const float scale = MOD == 0 ? a.sm_scale * kLog2e : 1.f;
+  // Slopes alone begin the scores with their distances, and the products are added
+  // to these (8192 tokens of 32 heads of 128 655 -> 631 us, of 64 416 -> 393; at
+  // head dim 256 the tile's start held more registers than there are).
+  constexpr bool kBegin = MOD == kBias && D != 256;
+  const float scale = MOD == 0 || kBegin ? a.sm_scale * kLog2e : 1.f;
   // cap: c tanh(x / c) = c - 2 c / (1 + e^(2 x / c))
   const float cap2 = a.soft_cap * kLog2e;
   const float cap_in = MOD & kCap ? 2.f * kLog2e * a.sm_scale / a.soft_cap : 0.f;
@@ -578,7 +582,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 #pragma unroll
       for (int s8 = 0; s8 < Sh::kKS; ++s8) qreg[s8] = *reinterpret_cast<const half8*>(q + 16 * s8);
     }
-    const float slope = MOD & kBias ? a.slopes[row.h] * kLog2e : 0.f;
+    const float slope = MOD & kBias ? a.slopes[row.h] * kLog2e / scale : 0.f;
     // keys the row sees: below s.prefix, and [lo, hi)
     const int32_t hi = a.causal ? min(pos + 1, s.L) : s.L, lo = pos - window + 1;
     // first and last position of the wave's rows and of the item's
@@ -640,6 +644,9 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
 #pragma unroll
     for (int t = 0; t < Sh::kDB; ++t) acc_o[t] = floatx16{};
     float m_run = kPfNoMax, l_run = 0.f;
+    // At head dim 64 a row's two lanes each keep the sum of their own keys until the
+    // item's end (with slopes 393 -> 371 us, a cap 512 -> 481; at 128 it spilled).
+    constexpr bool kHalves = D == 64;
     // O elements that a value of +inf / -inf / NaN (both) reaches, bit 16 t + i
     constexpr int kFlags = D == 256 ? 2 : 1;
     uint64_t inf_pos[kFlags] = {}, inf_neg[kFlags] = {};
@@ -696,6 +703,28 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       }
     };
 
+    // what the products of a tile are added to
+    auto begin_scores = [&](floatx16 (&x)[2], int32_t k0) {
+      x[0] = x[1] = floatx16{};
+      if constexpr (kBegin) {
+        const float d0 = (float)(pos - k0 - 4 * g);  // crow(i, g) = crow(i, 0) + 4 g
+        if (k0 + kChTile - 1 <= wp0) {  // no key behind a row: the distances need no |.|
+          const float far = -slope * d0;
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              x[ks][i] = __builtin_fmaf(slope, (float)(ks * 32 + crow(i, 0)), far);
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              x[ks][i] = -slope * __builtin_fabsf(d0 - (float)(ks * 32 + crow(i, 0)));
+        }
+      }
+    };
+
     auto tile = [&](const lds_char* sK, const lds_char* sV, int32_t k0) {
       if constexpr (kXor) {
         asm volatile("" : "+v"(k_off[0]));
@@ -714,10 +743,9 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           kf1[s8] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
               sK + k_at(s8) + 2 * kRow16);
         __builtin_amdgcn_sched_barrier(0);
-        acc_s[0] = floatx16{};
+        begin_scores(acc_s, k0);
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[0] = mfma32(kf0[s8], qreg[s8], acc_s[0]);
-        acc_s[1] = floatx16{};
 #pragma unroll
         for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[1] = mfma32(kf1[s8], qreg[s8], acc_s[1]);
       } else {
@@ -730,8 +758,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
                 sK + k_at((bt % (kNB / 2)) * kB + j) + (bt / (kNB / 2)) * 2 * kRow16);
         };
         half8 kfa[kB], kfb[kB];
-        acc_s[0] = floatx16{};
-        acc_s[1] = floatx16{};
+        begin_scores(acc_s, k0);
         kread(0, kfa);
 #pragma unroll
         for (int bt = 0; bt < kNB; bt += 2) {
@@ -749,7 +776,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
                 mfma32(kfb[j], qreg[((bt + 1) % (kNB / 2)) * kB + j], acc_s[(bt + 1) / (kNB / 2)]);
         }
       }
-      if constexpr (MOD != 0) {
+      if constexpr (MOD != 0 && !kBegin) {
         const float d0 = (float)(pos - k0 - 4 * g);  // crow(i, g) = crow(i, 0) + 4 g
         const float pre = MOD & kCap ? 0.f : a.sm_scale * kLog2e;
         if (MOD & kCap) {
@@ -834,7 +861,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           // sum l has them unrounded)
           pb[ks][i / 8][i % 8] = (f16)p;
         }
-      lt = pair_sum(lt);
+      if constexpr (!kHalves) lt = pair_sum(lt);
       if (move) {
         const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * scale);
         l_run = l_run * alpha;
@@ -906,6 +933,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
           if (inf_neg[t / 4] >> bit & 1u) acc_o[t][i] -= INFINITY;
         }
       }
+    if constexpr (kHalves) l_run = pair_sum(l_run);
     if (slot == kWhole) {
       if (live) store_row<D>(a, s, row, g, m_run * scale, l_run, acc_o);
     } else if (live) {  // a part: m in units of log 2
@@ -1417,7 +1445,9 @@ uint64_t list_entries(const ChunkArgs& a, uint32_t slots) {
   return (uint64_t)a.T * (a.Hq / a.H) / kChRows + a.B + 2u * slots / a.H + 1u;
 }
 // Whether a call has rows for so many items that they are listed (and a grid of
-// 32-bit work-items holds their workgroups).
+// 32-bit work-items holds their workgroups).  With fewer, equal shares are faster:
+// a windowed batch of prompts, chunks and single tokens 110 us, listed 134; drafted
+// tokens after 16384 60, listed 73.
 bool lists_items(const ChunkArgs& a, uint32_t slots) {
   return (uint64_t)a.T * (a.Hq / a.H) / kChRows * a.H >= slots &&
          list_entries(a, slots) * a.H < (1u << 24);
