@@ -184,7 +184,7 @@ class QuestLlamaModel(nn.Module):
         """Allocates the paged caches for max_seq_len tokens (llama.py:520-552).
         evict_keep: after each prompt, every layer's cache is cut down to that
         many tokens per kv head: the first evict_sink, the last evict_recent, and
-        those that the prompt's last queries attend to most."""
+        those that the last queries of the prompts attend to most."""
         assert self.iController is None, "Can't init Quest Controller twice."
         cfg = self.cfg
         self._page_budget = token_budget // page_size

@@ -156,17 +156,19 @@ def observe(q: torch.Tensor, lse: torch.Tensor, iController: InferenceController
     """Adds the attention weight of the new tokens' queries (``last``: of their
     last ones alone) to the sums that ``iController.evict`` goes by; q, lse and
     the options as ``chunk_forward`` had and gave them.  The new tokens' own sums
-    start from 0."""
+    start from 0, and so do those of tokens that were appended before them and
+    not observed (decode steps)."""
     c = iController
     n = q.size(0)
     rows = n if last is None else max(1, min(last, n))
-    c._start[0].fill_(c.kv_cache.seqlen - n)
+    c._start[0].fill_(c.unobserved_from(layer_idx, n))
     c._q_indptr[1].fill_(rows)
     ops.attn_weights(q[n - rows:], lse[n - rows:], c._q_indptr, c.attn_weights_layer(layer_idx),
                      c.kv_cache.buf_layer(layer_idx), c.kv_indptr_for_append,
                      c.kv_indices_with_last, c.kv_last_page_len_t, c.decode_max_pages, c.layout,
                      window=window, soft_cap=soft_cap, slopes=slopes, prefix_len=prefix_len,
                      start=c._start, workspace=c.workspace)
+    c.note_observed(layer_idx)
 
 
 def decode_estimate(q: torch.Tensor, iController: InferenceController, layer_idx: int

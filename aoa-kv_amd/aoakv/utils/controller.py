@@ -76,6 +76,9 @@ class InferenceController:
         # evicted)
         self._attn_weights = None
         self.evicted = 0
+        # tokens whose sums hold, per layer: those appended since without an
+        # observation have none, their slots hold what an earlier owner left
+        self._observed = [0] * num_layers
 
         self._page_budget = page_budget
         self.inference_page_budget = None
@@ -145,6 +148,8 @@ class InferenceController:
     # ------------------------------------------------------------ planning
     def prepare_metadata(self, seq_len: int):
         """Reserve cache slots for seq_len new tokens (controller.py:84-88)."""
+        if self._attn_weights is not None:  # (a cache may have been shortened)
+            self._observed = [min(n, self.kv_cache.seqlen) for n in self._observed]
         new_pages = self.kv_cache.append_seq(seq_len)
         self.metadata_cache.append_seq(new_pages)
 
@@ -265,14 +270,38 @@ class InferenceController:
             raise RuntimeError("track_weights() was not called")
         return self._attn_weights[layer_idx]
 
+    def unobserved_from(self, layer_idx: int, new_tokens: int) -> int:
+        """The first token of a layer whose sum starts from 0 when its newest
+        ``new_tokens`` are observed: of these, and of those appended before them
+        that were not observed (decode steps)."""
+        return min(self._observed[layer_idx], self.kv_cache.seqlen - new_tokens)
+
+    def note_observed(self, layer_idx: int):
+        """Every token of the layer has its sum now (utils.observe calls it)."""
+        self._observed[layer_idx] = self.kv_cache.seqlen
+
+    def _clear_unobserved(self, layer_idx: int):
+        """Sums of 0 for the tokens that were appended and not observed."""
+        first, S = self._observed[layer_idx], self.page_size
+        if first >= self.kv_cache.seqlen:
+            return
+        w, ids, p = self._attn_weights[layer_idx], self.kv_cache.indicies, first // S
+        if first % S:
+            w[ids[p], :, first % S:].zero_()
+            p += 1
+        if p < len(ids):
+            w.index_fill_(0, self._kv_ids[p:len(ids)].long(), 0.0)
+        self.note_observed(layer_idx)
+
     def evict(self, keep: int, sink: int = 0, recent: int = 0) -> int:
         """Drop all but ``keep`` tokens of every layer and kv head: the first
         ``sink``, the last ``recent`` and those of the others that received the
-        most attention weight (utils.observe).  The caches are packed in place,
-        with their page statistics, the pages behind are given back, and the
-        tokens keep the rotation of the positions they had.  Call it between
-        forward passes (after every layer's append).  Returns the number of
-        tokens dropped (0: there were no more than ``keep``)."""
+        most attention weight (utils.observe; none, where they were appended
+        and not observed since).  The caches are packed in place, with their page
+        statistics, the pages behind are given back, and the tokens keep the
+        rotation of the positions they had.  Call it between forward passes
+        (after every layer's append).  Returns the number of tokens dropped (0:
+        there were no more than ``keep``)."""
         L = self.kv_cache.seqlen
         if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
             raise ValueError(f"keep {keep}, sink {sink}, recent {recent}: sink + recent <= keep")
@@ -284,6 +313,7 @@ class InferenceController:
         kept = torch.empty((1, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
         for i in range(self.num_layers):
             w = self._attn_weights[i]
+            self._clear_unobserved(i)
             ops.keep_tokens(w, *table, keep, kept, P, sink=sink, recent=recent,
                             workspace=self.workspace)
             ops.compact_kv_cache(
@@ -293,6 +323,7 @@ class InferenceController:
                 self.layout, weights=w, workspace=self.workspace)
         self.kv_cache.truncate(keep)
         self.metadata_cache.truncate(len(self.kv_cache.indicies))
+        self._observed = [keep] * self.num_layers
         self.evicted += L - keep
         # the shorter tables, for the next eviction or chunk: before the pages
         # that were given back can be taken in another order
@@ -301,6 +332,7 @@ class InferenceController:
 
     def clean_states(self):
         self.evicted = 0
+        self._observed = [0] * self.num_layers
         self.kv_cache.release()
         self.metadata_cache.release()
         self._up.update(kv=0, md=0)
