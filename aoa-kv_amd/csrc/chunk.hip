@@ -328,6 +328,15 @@ __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kChRows
 template <int D>
 constexpr uint32_t attn_per_cu() { return D == 256 ? 1u : 2u; }
 constexpr uint32_t kCus = 256u;
+// Probabilities are rounded to fp16 for the second product (products of 32-bit
+// operands run at a sixteenth of the rate).  Beside the running maximum they are
+// 2^8 at most (see `up` below) and fp16 holds 2^15, so all of them, and the sum
+// and O that they make, are held 2^7 times as large: down to 2^-21 of that
+// maximum the rounding is 2^-11 of a probability, as the values' own, and below
+// it 2^-32 of the maximum.  (Without the factor, those below 2^-25 were missing
+// in O and counted in the sum: 16384 keys of e^-17.5 beside one of 1, 4e-4 of the
+// weight.)
+constexpr float kLift = 7.f, kLiftInv = 1.f / 128.f;
 constexpr size_t kCutBytes = kCus * 4u * sizeof(Cut);  // (4 workgroups per CU at most)
 constexpr uint32_t kAttnLeast = 2u;  // units of a share at least
 
@@ -341,7 +350,8 @@ __device__ inline Row row_of(const ChunkArgs& a, uint32_t hk, int32_t r) {
   return Row{tok, hk * a.G + (uint32_t)r - (uint32_t)tok * a.G};
 }
 
-// o and lse of a row: O dims 32 t + crow(i, g) of the lane's row
+// o and lse of a row: O dims 32 t + crow(i, g) of the lane's row; l and O are
+// lifted
 template <int D>
 __device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r, int g, float m2,
                                  float l, const floatx16 (&acc)[PfShape<D>::kDB]) {
@@ -358,7 +368,7 @@ __device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r,
       *reinterpret_cast<half4*>(o + t * 32 + crow(i0, g)) = v;
     }
   if (a.lse != nullptr && g == 0)
-    a.lse[row] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l)) * kLn2;
+    a.lse[row] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l * kLiftInv)) * kLn2;
 }
 
 // A call of many items: a launch before lists them (and the parts of those
@@ -848,7 +858,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       const bool up = (mt - m_run) * scale > 8.f;
       const bool move = __builtin_amdgcn_ballot_w64(up) != 0;
       const float m_new = up ? mt : m_run;
-      const float neg_m = -m_new * scale;
+      const float neg_m = __builtin_fmaf(-m_new, scale, kLift);
       float lt = 0.f;
       half8 pb[2][2];
 #pragma unroll
@@ -857,8 +867,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         for (int i = 0; i < 16; ++i) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc_s[ks][i], scale, neg_m));
           lt += p;
-          // (fp16: half a step of 2^-11 per probability, as the values' own; the
-          // sum l has them unrounded)
+          // (the sum l has them unrounded; kLift)
           pb[ks][i / 8][i % 8] = (f16)p;
         }
       if constexpr (!kHalves) lt = pair_sum(lt);
@@ -934,9 +943,11 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         }
       }
     if constexpr (kHalves) l_run = pair_sum(l_run);
+    // (in units of log 2, as the exponents had it)
+    const float m2 = kLift - __builtin_fmaf(-m_run, scale, kLift);
     if (slot == kWhole) {
-      if (live) store_row<D>(a, s, row, g, m_run * scale, l_run, acc_o);
-    } else if (live) {  // a part: m in units of log 2
+      if (live) store_row<D>(a, s, row, g, m2, l_run, acc_o);
+    } else if (live) {  // a part: O lifted, l not
       float* part = a.parts + (size_t)slot * part_floats(D);
       float4* po = reinterpret_cast<float4*>(part) + wave * 32 + c;
 #pragma unroll
@@ -948,8 +959,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       }
       if (g == 0) {
         float* pm = part + kChRows * D + wave * 32 + c;
-        pm[0] = m_run * scale;
-        pm[kChRows] = l_run;
+        pm[0] = m2;
+        pm[kChRows] = l_run * kLiftInv;
       }
     }
     if constexpr (LIST) return;
@@ -1026,7 +1037,7 @@ __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
       }
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : kLiftInv / l;
   const size_t at = (size_t)(cut.q0 + row.tok) * a.Hq + row.h;
   f16* o = a.o + at * D + 4 * kV * j0;
 #pragma unroll
