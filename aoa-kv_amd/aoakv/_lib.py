@@ -66,6 +66,7 @@ SIGNATURES = {
     "aoakv_rope_append_kv_cache_prefill": [_p, _p, _p, _u32, _u32, _p, _p, _u32, _u32, _p, _p,
                                            _p, _p, _u32, _u32, _u32, _u32, _f32, _f32, _p],
     "aoakv_chunk_attn_workspace_size": [_u32, _u32, _u32, _u32, _u32],
+    "aoakv_chunk_attn_call_workspace_size": [_u32, _u32, _u32, _u32, _u32, _u32, _u32],
     "aoakv_chunk_attn": [_p, _p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
                          _u32, _u32, _u32, _u32, _u32, _f32, _p, _sz, _p, _p],
     "aoakv_attn_weights_workspace_size": [],
@@ -85,6 +86,7 @@ _RESTYPES = {
     "aoakv_layer_workspace_size": _sz,
     "aoakv_prefill_workspace_size": _sz,
     "aoakv_chunk_attn_workspace_size": _sz,
+    "aoakv_chunk_attn_call_workspace_size": _sz,
     "aoakv_attn_weights_workspace_size": _sz,
 }
 

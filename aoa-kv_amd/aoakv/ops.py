@@ -306,7 +306,9 @@ def chunk_attn(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, ma
     the fp32 [T, Hq] log of each row's sum of exponentials (0 and -inf for a row
     that sees nothing).  Rows of no sequence are left as ``o`` held them.
     ``workspace``: a decode workspace whose error word receives
-    WS_ERR_TRUNCATED when a page table is longer than ``max_pages``."""
+    WS_ERR_TRUNCATED when a page table is longer than ``max_pages``.  The call takes
+    its scratch memory from torch's pool; where that has none it runs without it,
+    slower."""
     return _host.chunk_attn(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len,
                             max_pages, layout, int(causal), window, float(soft_cap), slopes,
                             prefix_len, o, int(return_lse), workspace)

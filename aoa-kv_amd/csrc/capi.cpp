@@ -1087,15 +1087,23 @@ static int fill_chunk(aoakv::ChunkArgs& a, const void* q, const int32_t* q_indpt
   return AOAKV_OK;
 }
 
-size_t aoakv_chunk_attn_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
-                                       uint32_t num_qo_heads, uint32_t num_kv_heads,
-                                       uint32_t head_dim) {
+size_t aoakv_chunk_attn_call_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
+                                            uint32_t max_pages, uint32_t num_qo_heads,
+                                            uint32_t num_kv_heads, uint32_t head_dim,
+                                            uint32_t page_size) {
   // (the call itself refuses these)
   if ((head_dim != 64u && head_dim != 128u && head_dim != 256u) || num_kv_heads == 0u ||
       num_qo_heads > 256u || num_qo_heads % num_kv_heads != 0u)
     return 0u;
   return aoakv::chunk_attn_workspace(num_q_tokens, batch_size, num_qo_heads, num_kv_heads,
-                                     head_dim);
+                                     head_dim, max_pages, page_size);
+}
+
+size_t aoakv_chunk_attn_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
+                                       uint32_t num_qo_heads, uint32_t num_kv_heads,
+                                       uint32_t head_dim) {
+  return aoakv_chunk_attn_call_workspace_size(num_q_tokens, batch_size, aoakv::kMaxChunkTokens,
+                                              num_qo_heads, num_kv_heads, head_dim, 1u);
 }
 
 int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr,
@@ -1110,11 +1118,7 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
   if (int e = fill_chunk(a, q, q_indptr, num_q_tokens, kv_data, kv_indptr, kv_indices,
                          kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
                          num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
-                         soft_cap, workspace, workspace_bytes,
-                         aoakv_chunk_attn_workspace_size(num_q_tokens, batch_size, num_qo_heads,
-                                                         num_kv_heads, head_dim),
-                         error_word,
-                         "chunk_attn"))
+                         soft_cap, workspace, workspace_bytes, 0u, error_word, "chunk_attn"))
     return e;
   if (num_q_tokens == 0u) return ok();
   REQUIRE(o, "chunk_attn: null pointer argument");
@@ -1122,6 +1126,11 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
   a.o = static_cast<aoakv::f16*>(o);
   a.lse = lse;
   a.cuts = workspace;
+  a.whole = workspace == nullptr ||
+            workspace_bytes < aoakv_chunk_attn_call_workspace_size(num_q_tokens, batch_size,
+                                                                   max_pages, num_qo_heads,
+                                                                   num_kv_heads, head_dim,
+                                                                   page_size);
   return hip_status(aoakv::launch_chunk_attn(a, head_dim, static_cast<hipStream_t>(stream)),
                     "chunk_attn");
 }

@@ -497,11 +497,19 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
     u = list_place() * share;
     u1 = min(u + share, units);
     if (u >= u1) {
-      if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()].n = 0u;
+      if (tid == 0 && !a.whole) reinterpret_cast<Cut*>(a.cuts)[list_place()].n = 0u;
       return;
     }
     w.seek(u, per_head);
-    if (tid == 0) reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
+    if (a.whole) {  // no workspace: the items that begin in the share, whole
+      if (w.at != 0u) {
+        u += (uint32_t)ByRows::item(a, w.seq(), w.x).count + kItemUnits - w.at;
+        if (u >= u1) return;
+        w.next();
+      }
+    } else if (tid == 0) {
+      reinterpret_cast<Cut*>(a.cuts)[list_place()] = cut_of(w, list_place(), share);
+    }
   }
 
   // Slopes alone begin the scores with their distances, and the products are added
@@ -572,7 +580,7 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
       item = ByRows::item(a, s, ix);
       hk = w.h;
       const uint32_t ue = (uint32_t)item.count + kItemUnits;
-      const uint32_t ua = w.at, ub = (uint32_t)min((uint64_t)ue, ua + (u1 - u));
+      const uint32_t ua = w.at, ub = a.whole ? ue : (uint32_t)min((uint64_t)ue, ua + (u1 - u));
       units = ub - ua;
       t0 = (int32_t)((uint64_t)ua * (uint32_t)item.count / ue);
       t1 = (int32_t)((uint64_t)ub * (uint32_t)item.count / ue);
@@ -1419,14 +1427,15 @@ uint32_t workgroups(const ChunkArgs& a, uint64_t items, uint64_t tiles, uint32_t
 }
 
 // The factors that divide by the page size, the group and n workgroups; the
-// workspace holds the cuts, then the parts.
+// workspace holds the cuts, then the parts (there may be none: a.whole).
 ChunkArgs with_rcps(const ChunkArgs& args, uint32_t n) {
   ChunkArgs a = args;
   a.G = a.Hq / a.H;
   a.page_rcp = a.S == 1u ? 0u : (uint32_t)((1ull << 32) / a.S) + 1u;
   a.group_rcp = ((1u << 31) + a.G - 1u) / a.G;
   a.share_rcp = 1.0 / (double)n;
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(a.cuts) + kCutBytes);
+  if (a.cuts != nullptr)
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(a.cuts) + kCutBytes);
   return a;
 }
 
@@ -1469,10 +1478,17 @@ size_t list_bytes(const ChunkArgs& a, uint32_t slots) {
   return lists_items(a, slots) ? (list_entries(a, slots) * sizeof(Entry) + 255u) / 256u * 256u : 0u;
 }
 
+// Workgroups of a call whose items are not listed.
+uint32_t share_workgroups(const ChunkArgs& a, uint32_t slots) {
+  const uint64_t G = a.Hq / a.H;
+  return workgroups(a, (a.T * G) / kChRows + a.B, ((uint64_t)a.max_pages * a.S) / kChTile + 2u,
+                    slots, kAttnLeast);
+}
+
 template <int D>
 hipError_t launch_attn(const ChunkArgs& args, hipStream_t s) {
   constexpr uint32_t kSlots = attn_slots<D>();
-  if (lists_items(args, kSlots)) {
+  if (!args.whole && lists_items(args, kSlots)) {
     const uint64_t n = list_entries(args, kSlots) * args.H;
     ChunkArgs a = with_rcps(args, kSlots);
     a.list = a.parts;
@@ -1485,12 +1501,9 @@ hipError_t launch_attn(const ChunkArgs& args, hipStream_t s) {
                        dim3(kChThreads), 0, s, a);
     return hipGetLastError();
   }
-  const uint64_t G = args.Hq / args.H;
-  const uint32_t n = workgroups(args, (args.T * G) / kChRows + args.B,
-                                ((uint64_t)args.max_pages * args.S) / kChTile + 2u, kSlots,
-                                kAttnLeast);
+  const uint32_t n = share_workgroups(args, kSlots);
   const ChunkArgs a = with_rcps(args, n);
-  if (hipError_t e = launch_attn<D, false>(a, n, s); e != hipSuccess) return e;
+  if (hipError_t e = launch_attn<D, false>(a, n, s); e != hipSuccess || a.whole) return e;
   hipLaunchKernelGGL((chunk_join_kernel<D, false>), dim3((n - 1u) * 4u), dim3(kChThreads), 0, s, a);
   return hipGetLastError();
 }
@@ -1533,15 +1546,19 @@ hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
 
 }  // namespace
 
-size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim) {
+size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim,
+                            uint32_t max_pages, uint32_t S) {
   ChunkArgs a{};
   a.T = T;
   a.B = B;
   a.Hq = Hq;
   a.H = H;
+  a.max_pages = max_pages;
+  a.S = S;
   const uint32_t slots = head_dim == 256u ? attn_slots<256>() : attn_slots<128>();
+  const uint32_t n = lists_items(a, slots) ? slots : share_workgroups(a, slots);
   return kCutBytes + list_bytes(a, slots) +
-         2u * (size_t)slots * part_floats((int)head_dim) * sizeof(float);
+         2u * (size_t)n * part_floats((int)head_dim) * sizeof(float);
 }
 size_t attn_weights_workspace() {
   return kCutBytes + 2u * kCus * kMostSums * kMostKeys * sizeof(float);

@@ -35,8 +35,8 @@ struct PyErr {};
   X(append_kv_cache_prefill) X(append_kv_cache_decode) X(rope_append_kv_cache_decode)  \
   X(rope_append_kv_cache_prefill) X(rms_norm_forward) X(estimate_attn_score)           \
   X(topk_filtering) X(decode_sparse_attn) X(sparse_decode_layer)                       \
-  X(prefill_workspace_size) X(prefill_with_workspace) X(chunk_attn_workspace_size)     \
-  X(chunk_attn) X(attn_weights_workspace_size) X(attn_weights) X(keep_tokens)          \
+  X(prefill_workspace_size) X(prefill_with_workspace)                                  \
+  X(chunk_attn_call_workspace_size) X(chunk_attn) X(attn_weights_workspace_size) X(attn_weights) X(keep_tokens)          \
   X(compact_kv_cache) X(last_error)
 
 struct Lib {
@@ -556,14 +556,23 @@ PyObject* chunk_attn(PyObject* const* a) {
   const Tensor o = given != nullptr ? *given : at::empty_like(c.q);
   Tensor lse;
   if (want) lse = at::empty({c.q.size(0), c.q.size(1)}, c.q.options().dtype(at::kFloat));
-  const size_t n = g_lib.chunk_attn_workspace_size(c.T, (uint32_t)c.t.B, c.Hq, c.d.H, c.d.D);
-  const Tensor ws = scratch(n, c.q);
+  size_t n = g_lib.chunk_attn_call_workspace_size(c.T, (uint32_t)c.t.B, c.max_pages, c.Hq, c.d.H,
+                                                  c.d.D, c.d.S);
+  Tensor ws;
+  if (n != 0) {
+    try {
+      ws = scratch(n, c.q);
+    } catch (const c10::OutOfMemoryError&) {
+      n = 0;  // no room (68 MB and a list at most): items are not cut
+    }
+  }
   void* s = stream();
   call("aoakv_chunk_attn", [&] {
     return g_lib.chunk_attn(ptr(c.q), ptr(o), want ? static_cast<float*>(ptr(lse)) : nullptr,
                             c.q_indptr, c.T, ptr(c.kv), c.t.indptr, c.t.indices, c.t.last,
                             c.prefix, c.slopes, (uint32_t)c.t.B, c.max_pages, c.Hq, c.d.H, c.d.D,
-                            c.d.S, c.d.layout, c.causal, c.window, c.cap, ptr(ws), n, err, s);
+                            c.d.S, c.d.layout, c.causal, c.window, c.cap,
+                            n != 0 ? ptr(ws) : nullptr, n, err, s);
   });
   if (!want) return THPVariable_Wrap(o);
   PyObject *x = THPVariable_Wrap(o), *y = THPVariable_Wrap(lse);

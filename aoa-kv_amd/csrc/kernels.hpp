@@ -296,12 +296,13 @@ struct ChunkArgs {
   PageGeom g;
   uint32_t* error;            // receives kErrTruncated, or nullptr
   void* cuts;                 // the workspace
+  uint32_t whole;             // items are not cut (the attention: without a workspace;
+                              // the weights: set by the launch)
   // set by the launch: the workspace's two slots per workgroup; the group's
-  // heads; the factors that divide by S, G and the workgroups; whether items are
-  // not cut
+  // heads; the factors that divide by S, G and the workgroups
   float* parts;
   void* list;
-  uint32_t G, page_rcp, group_rcp, whole;
+  uint32_t G, page_rcp, group_rcp;
   double share_rcp;
 };
 // Tokens of a sequence's table at most: positions are divided by the page size
@@ -311,7 +312,8 @@ constexpr uint32_t kMaxChunkTokens = 1u << 27;
 __device__ inline uint32_t div_page(uint32_t x, uint32_t rcp) {
   return rcp == 0u ? x : __umulhi(x, rcp);
 }
-size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim);
+size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uint32_t head_dim,
+                            uint32_t max_pages, uint32_t S);
 size_t attn_weights_workspace();
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
 hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);

@@ -494,9 +494,16 @@ int aoakv_prefill_with_workspace(const void* q, void* o, const void* kv_data,
  * 16 bytes.  max_pages >= every sequence's page count: a longer table is cut to
  * it and AOAKV_WS_ERR_TRUNCATED set in *error_word (NULL: not reported), as in
  * aoakv_topk_filtering.  workspace:
- * aoakv_chunk_attn_workspace_size bytes, aligned to 16; it needs no
- * initialisation and is free again when the call's work on `stream` is done.
+ * aoakv_chunk_attn_call_workspace_size bytes (aoakv_chunk_attn_workspace_size:
+ * enough for any context), aligned to 16; it needs no initialisation and is free
+ * again when the call's work on `stream` is done.  With fewer bytes, or NULL, the
+ * call runs without it: no 128 rows' keys are split then, which is slower where
+ * rows are few or of unequal lengths.
  */
+size_t aoakv_chunk_attn_call_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
+                                            uint32_t max_pages, uint32_t num_qo_heads,
+                                            uint32_t num_kv_heads, uint32_t head_dim,
+                                            uint32_t page_size);
 size_t aoakv_chunk_attn_workspace_size(uint32_t num_q_tokens, uint32_t batch_size,
                                        uint32_t num_qo_heads, uint32_t num_kv_heads,
                                        uint32_t head_dim);
