@@ -226,8 +226,10 @@ __global__ __launch_bounds__(kPfThreads, pf_blocks_per_cu<D>()) void prefill_ker
     // sub-tile are read before its MFMAs, and the second sub-tile's reads
     // go out before the first sub-tile's MFMAs, so no MFMA waits on a
     // just-issued LDS read.  At D = 256 (16 fragments per sub-tile) they go
-    // in batches of 8, each read while the previous batch's MFMAs run, to
-    // keep the registers of one wave per SIMD.
+    // in batches of 4, each read while the previous batch's MFMAs run, to
+    // keep the registers of one wave per SIMD: with batches of 8 up to 7 were
+    // spilled, and the allocator has lost a dword of a spilled fragment (see
+    // chunk.hip).
     floatx16 acc_s[2];
     if constexpr (Sh::kKS <= 8) {
       half8 kf0[Sh::kKS], kf1[Sh::kKS];
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(kPfThreads, pf_blocks_per_cu<D>()) void prefill_ker
 #pragma unroll
       for (int s8 = 0; s8 < Sh::kKS; ++s8) acc_s[1] = mfma32(kf1[s8], qreg[s8], acc_s[1]);
     } else {
-      constexpr int kB = 8;                      // fragments per batch
+      constexpr int kB = 4;                      // fragments per batch
       constexpr int kNB = 2 * Sh::kKS / kB;      // batches per tile (both sub-tiles)
       auto kread = [&](int bt, half8 (&kf)[kB]) {  // batch bt: sub-tile bt / (kNB / 2)
 #pragma unroll
