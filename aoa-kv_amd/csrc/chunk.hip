@@ -30,10 +30,11 @@
 // only those longer than an equal share are cut.  Nothing depends on timing: equal
 // calls give equal bits.
 //
-// Registers.  No kernel here may spill one: the allocator, keeping part of a
-// spilled 128-bit tuple in an accumulation register, lost its fourth dword (head
-// dim 256, odd pages, listed: every score was wrong).  Fragments are read in
-// batches, and offsets made where they are used, as far as that takes.
+// Registers.  No kernel here may spill a vector register: the allocator, keeping
+// part of a spilled 128-bit tuple in an accumulation register, lost its fourth
+// dword (head dim 256, odd pages, listed: every score was wrong).  Fragments are
+// read in batches, and offsets made where they are used, as far as that takes.
+// (Scalar registers are spilled, into lanes of a vector register.)
 #include "kernels.hpp"
 #include "mfma_tile.hpp"
 
@@ -375,7 +376,7 @@ __device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r,
 // longer than an equal share), the longest first, for one workgroup each.
 // Walking the keys of a head from its first on, side by side, the workgroups of
 // an XCD find them in its L2, and few items are cut.  The listing takes 5 us;
-// 8192 tokens of 32 heads took 740 us in shares and 651 so.
+// 8192 tokens of 32 heads take 680 us in shares and 574 so.
 struct Entry {
   uint32_t b;
   int32_t x, t0, t1;
@@ -476,10 +477,12 @@ __global__ __launch_bounds__(kChThreads) void chunk_list_kernel(ChunkArgs a, uin
 // What bounds it: a tile's K and V fragments pass from LDS to the matrix cores at
 // 128 bytes a clock and CU, the rate at which the products consume them, and the
 // exponentials take as long again; two workgroups per CU run one beside the other.
-// 8192 tokens over themselves, causal: 32 heads of 128 600 us (920 TFLOP/s; 8 kv
-// heads the same), with slopes 630, a cap 700; 16 heads of 256 730; 32 of 64 350;
-// few rows over a long cache pass 5.4 TB/s.  64 rows per wave, which halves
-// the fragments, left one wave per SIMD and took 920 us.
+// 8192 tokens over themselves, causal: 32 heads of 128 572 us (960 TFLOP/s; 8 kv
+// heads the same), with slopes 620, a cap 693; 16 heads of 256 722, 859 and 795; 32
+// of 64 347, 371 and 474 (smallest of 5 x 20 calls, normal inputs; with a few large
+// channels 637 to 648 with slopes).  Few rows over a long cache pass 5.3 TB/s.  64
+// rows per wave, which halves the fragments, left one wave per SIMD and took 920 us
+// (650 then).
 template <int D, int MOD, bool S16, bool LIST>
 __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kernel(ChunkArgs a) {
   using Sh = PfShape<D>;
@@ -513,8 +516,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
   }
 
   // Slopes alone begin the scores with their distances, and the products are added
-  // to these (8192 tokens of 32 heads of 128 655 -> 631 us, of 64 416 -> 393; at
-  // head dim 256 the tile's start held more registers than there are).
+  // to these (the step took 4 and 6 % off 8192 tokens of 32 heads of 128 and of 64;
+  // at head dim 256 the tile's start held more registers than there are).
   constexpr bool kBegin = MOD == kBias && D != 256;
   const float scale = MOD == 0 || kBegin ? a.sm_scale * kLog2e : 1.f;
   // cap: c tanh(x / c) = c - 2 c / (1 + e^(2 x / c))
@@ -1092,7 +1095,8 @@ constexpr int32_t kNoPos = INT32_MIN;
 // product), tiles of 128 rows, two workgroups per CU.  Else the keys' own way
 // from memory is what takes the time: 32 keys, tiles of 32 rows, and as many
 // workgroups per CU with their keys in flight as registers allow (the last 32
-// rows of 16384 tokens x 32 heads: 2 per CU 38 us, 3 32, 4, spilling, 41).
+// rows of 16384 tokens x 32 heads, one cache over and over: 2 per CU 38 us, 3 32,
+// 4, spilling, 41).
 template <int D, bool BIG>
 struct SumShape {
   static constexpr int kSets = BIG && D != 256 ? 2 : 1;  // of 32 keys per wave
@@ -1110,9 +1114,13 @@ constexpr uint32_t kWholeTiles = 4u;
 // added up by themselves first: one chain of single additions over 16384 rows was
 // 2e-6 off.
 //
-// Bound by the exponentials and the products issued between them where rows are
-// many (4096 tokens of 16 heads of 128: 63 us, of 256 103, of 64 46), by the keys'
-// way from memory where they are few (4.2 TB/s).
+// Bound by the exponentials and the products where rows are many (4096 tokens of
+// 16 heads of 128: 57 us, of 256 97, of 64 43; the products alone would take 29, 58
+// and 14 at a large product's rate, the exponentials with their multiply and add
+// about 20, so the two hardly overlap), and where they are few by the keys' way from
+// memory, an item's after the other's: 32 rows after 16384 tokens x 32 heads 41 us,
+// 3.3 TB/s, with caches in turn, and 32 where one stays in the memory-side cache; a
+// decode step of 16 sequences 87, 3.8 TB/s.
 template <int D, int MOD, bool BIG>
 __global__ __launch_bounds__(kChThreads, (SumShape<D, BIG>::kPerCu)) void attn_weights_kernel(
     ChunkArgs a) {
@@ -1465,9 +1473,17 @@ uint64_t list_entries(const ChunkArgs& a, uint32_t slots) {
   return (uint64_t)a.T * (a.Hq / a.H) / kChRows + a.B + 2u * slots / a.H + 1u;
 }
 // Whether a call has rows for so many items that they are listed (and a grid of
-// 32-bit work-items holds their workgroups).  With fewer, equal shares are faster:
-// a windowed batch of prompts, chunks and single tokens 110 us, listed 134; drafted
-// tokens after 16384 60, listed 73.
+// 32-bit work-items holds their workgroups).  Both ways, us in shares / listed, at x
+// items per workgroup that the GPU holds:
+//                                        x = 0.5       1          1.5        2          4
+//   prompt, 32 heads of 128              38 / 37     74 / 67   125 / 107  202 / 159  679 / 574
+//   prompt, 16 of 256                    50 / 48    100 / 89   164 / 142  259 / 205  850 / 722
+//   chunk after 8000, 32 / 8 of 128     170 / 193   333 / 388  516 / 542  710 / 679 1710 / 1615
+//   chunk after 8000, 16 of 256         217 / 269   434 / 542  688 / 752  952 / 845 2269 / 2035
+//   chunk after 8000, 32 of 64          114 / 117   227 / 224  359 / 311  487 / 445 1152 / 982
+// So the list starts where prompts want it; chunks after a long context would have
+// it from 2 on at 8 kv heads or head dim 256.  Fewer rows: a windowed batch of prompts, chunks and single
+// tokens 110 / 134 in the kernel, drafted tokens after 16384 60 / 73.
 bool lists_items(const ChunkArgs& a, uint32_t slots) {
   return (uint64_t)a.T * (a.Hq / a.H) / kChRows * a.H >= slots &&
          list_entries(a, slots) * a.H < (1u << 24);
@@ -1517,7 +1533,12 @@ hipError_t launch_sums(const ChunkArgs& args, hipStream_t s) {
       args, (uint64_t)args.B * (((uint64_t)args.max_pages * args.S) / Shape::kKeys + 1u), tiles,
       kCus * Shape::kPerCu, kSumsLeast);
   ChunkArgs a = with_rcps(args, n);
-  // items of a few tiles are not worth cutting, nor a launch to join them
+  // Items of a few tiles are not worth cutting, nor a launch to join them: 32, 64,
+  // 128, 256 and 512 rows of one sequence of 8000 keys, 8 kv heads, whole / cut 12 /
+  // 14, 13 / 17, 12 / 16, 15 / 18 and 30 / 25 us.  The bound is the call's rows,
+  // because a sequence's are known on the device alone: a decode step of 16
+  // sequences of 4 heads a group is whole (57.5; cut 59.2) and one of 17 is cut (69.6;
+  // whole 67.5), 64 273 (270).
   a.whole = tiles <= kWholeTiles ? 1u : 0u;
   const dim3 grid(n), block(kChThreads);
   switch ((a.soft_cap > 0.f ? kCap : 0) | (a.slopes != nullptr ? kBias : 0)) {
@@ -1537,7 +1558,12 @@ hipError_t launch_sums(const ChunkArgs& args, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Rows per sequence from which the BIG cut is the faster one (SumShape).
+// The BIG cut (SumShape) goes by the batch's rows per sequence, the longest being
+// known on the device alone.  4 sequences of 4096 keys, 8 kv heads, small / big: 64
+// rows each 20.6 / 22.6 us, 128 22 / 26, 256 30 / 31, 512 38 / 40, 1024 59 / 59, 2048
+// 100 / 88, 4096 172 / 153.  The border is below their crossing because an average
+// of 256 is often a long chunk among short ones (one of 4096 rows beside 31 of one:
+// 113 / 94, and with 129 on average still the small cut's).
 template <int D>
 hipError_t launch_sums(const ChunkArgs& a, hipStream_t s) {
   const uint64_t rows = (uint64_t)a.T * (a.Hq / a.H);

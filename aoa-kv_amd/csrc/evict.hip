@@ -40,8 +40,10 @@ constexpr uint32_t kBins = 2048u, kCopies = 4u;
 // they are held in registers, 4 x RUNS per thread, and only longer sequences
 // load them again in each step).  2048 of up to 32768 tokens, 4 x 32 heads: 143
 // us with a token per thread and loop trip, 37 from registers in four steps of
-// 8 bits, 22 so.  The histogram has 4 copies, by lane, because equal weights (many are
-// exactly 0) would otherwise add to one word one after the other.
+// 8 bits, 22 so (24 with caches in turn).  The histogram has 4 copies, by lane, because
+// equal weights (many are exactly 0) would otherwise add to one word one after the
+// other.  Slots behind a sequence's end count as the lowest weight in the first step,
+// so 5000 tokens take what 32768 do (22 us; up to 4096, with RUNS = 1, 6.6 to 7.8).
 template <int RUNS, bool VEC>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   __shared__ uint32_t s_hist[kBins * kCopies];
@@ -206,8 +208,10 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
 // ---------------------------------------------------------------- packing
 // threads: in place, where one workgroup takes all of a head, many; else few, so
 // that the steps of several workgroups overlap on a CU (2048 tokens of 4 x 32
-// heads to new pages, 285 MB: 512 threads 79 us, 256 68; 59 with K and V as
-// code of their own below, 4.8 TB/s, the rate of a large copy)
+// heads to new pages, 285 MB: 512 threads 79 us, 256 68; 59 with K and V as code of
+// their own below, 4.8 TB/s, and 70 to 73 with caches in turn).  In place 66 where
+// there are many heads; 2048 of 16384 tokens of one sequence at 32 and 8 heads 33 and
+// 30 us, to new pages 16 and 9.
 constexpr int kPackThreadsInPlace = 512, kPackThreads = 256;
 
 // A workgroup takes steps of K or of V of one (kv head, sequence): each lane
