@@ -30,7 +30,7 @@ HOST_SOURCE = "host.cpp"
 # build record beside the library (travels with it; the GPU box has no .git)
 BUILDINFO = os.path.join(PKG_DIR, "libaoakv.buildinfo.json")
 SOURCES = ["append.hip", "decode.hip", "prefill.hip", "generic.hip", "stream.hip", "norm.hip",
-           "chunk.hip", "evict.hip", "capi.cpp"]
+           "chunk.hip", "evict.hip", "append_fp8.hip", "chunk_fp8.hip", "decode_fp8.hip", "capi.cpp"]
 REPO_DIR = os.path.dirname(os.path.dirname(PKG_DIR))
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

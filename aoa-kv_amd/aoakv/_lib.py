@@ -76,6 +76,16 @@ SIGNATURES = {
                           _p, _p],
     "aoakv_compact_kv_cache": [_p, _u32, _u32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
                                _u32, _u32, _u32, _u32, _u32, _u32, _p, _p],
+    "aoakv_append_kv_cache_fp8": [_p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _u32,
+                                  _u32, _u32, _u32, _u32, _p],
+    "aoakv_rope_append_kv_cache_fp8": [_p, _p, _p, _p, _u32, _u32, _p, _p, _p, _p, _p, _p, _p, _p,
+                                       _p, _p, _u32, _u32, _u32, _u32, _u32, _f32, _f32, _p],
+    "aoakv_read_kv_cache_fp8": [_p, _p, _p, _u32, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32,
+                                _p],
+    "aoakv_chunk_attn_fp8": [_p, _p, _p, _p, _u32, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32,
+                             _u32, _u32, _u32, _u32, _u32, _u32, _f32, _p, _sz, _p, _p],
+    "aoakv_decode_sparse_attn_fp8": [_p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _p, _p, _sz, _u32,
+                                     _u32, _u32, _u32, _u32, _u32, _u32, _u32, _p],
     "aoakv_rope_append_kv_cache_decode": [_p, _p, _p, _u32, _u32, _p, _p, _p, _p, _p, _p, _p,
                                           _p, _p, _u32, _u32, _u32, _u32, _f32, _f32, _p],
 }

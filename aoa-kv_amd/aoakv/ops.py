@@ -354,3 +354,70 @@ def compact_kv_cache(kept, keep: int, kv_data, kv_indptr, kv_indices, kv_last_pa
                            new_indptr, new_indices, metadata_data, metadata_indptr,
                            metadata_indices, v_log_norm, v_mean, max_pages, layout, weights,
                            workspace)
+
+
+# ---- a paged cache held in 8 bits: kv_data float8_e4m3fn, kv_exp int8 [max_pages, 2, Hkv]
+# with the exponents of the scales of K and V of each page and kv head (aoakv.h)
+
+def append_kv_cache_fp8(k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices,
+                        kv_last_page_len, layout: int, metadata_data=None, metadata_indptr=None,
+                        metadata_indices=None, v_log_norm=None, v_mean=None):
+    """Appends new tokens of every sequence of a batch to a cache held in 8 bits
+    (aoakv_append_kv_cache_fp8).
+
+    k, v [T, Hkv, D] fp16 hold the sequences' new tokens one after the other, rows
+    token_indptr[b] .. token_indptr[b + 1] - 1 (int32, device) those of sequence b, the last
+    of its cached ones (the page table counts them).  An element becomes a code and its
+    block's exponent in ``kv_exp``, off by at most 2^-4 of itself.  With the five arguments
+    of the page statistics these are written as append_kv_cache_prefill writes them, from
+    the fp16 rows, so that estimate_topk selects the pages it would select of an fp16
+    cache."""
+    _host.append_kv_cache_fp8(k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices,
+                              kv_last_page_len, layout, metadata_data, metadata_indptr,
+                              metadata_indices, v_log_norm, v_mean)
+
+
+def rope_append_kv_cache_fp8(q, k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices,
+                             kv_last_page_len, layout: int, rope_scale: float = 1.0,
+                             rope_theta: float = 1e4, metadata_data=None, metadata_indptr=None,
+                             metadata_indices=None, v_log_norm=None, v_mean=None):
+    """append_kv_cache_fp8 with q [T, Hq, D] and k turned on the way, each token by its own
+    position (aoakv_rope_append_kv_cache_fp8): q in place, k on its way into the cache
+    alone.  Angles are exact at every position, where apply_rope_in_place rounds them to
+    fp32."""
+    _host.rope_append_kv_cache_fp8(q, k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices,
+                                   kv_last_page_len, layout, float(rope_scale),
+                                   float(rope_theta), metadata_data, metadata_indptr,
+                                   metadata_indices, v_log_norm, v_mean)
+
+
+def read_kv_cache_fp8(num_tokens: int, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices,
+                      kv_last_page_len, layout: int, k=None, v=None):
+    """The last tokens of every sequence of a cache held in 8 bits as fp16 rows k, v
+    [num_tokens, Hkv, D] (aoakv_read_kv_cache_fp8): rows by ``token_indptr`` as in
+    append_kv_cache_fp8, the elements' exact values.  Rows of no token are left as ``k`` and
+    ``v`` held them."""
+    return _host.read_kv_cache_fp8(num_tokens, token_indptr, kv_data, kv_exp, kv_indptr,
+                                   kv_indices, kv_last_page_len, layout, k, v)
+
+
+def chunk_attn_fp8(q, q_indptr, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len,
+                   max_pages: int, layout: int, causal: bool = True, window: int = 0,
+                   soft_cap: float = 0.0, slopes=None, prefix_len=None, o=None,
+                   return_lse: bool = False, workspace=None):
+    """``chunk_attn`` over a cache held in 8 bits (aoakv_chunk_attn_fp8), with its arguments
+    and results."""
+    return _host.chunk_attn_fp8(q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len,
+                                max_pages, layout, int(causal), window, float(soft_cap), slopes,
+                                prefix_len, o, int(return_lse), workspace, kv_exp)
+
+
+def decode_sparse_attn_fp8(q, o, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len,
+                           sel_pages, token_budget: int, workspace, max_pages: int, layout: int,
+                           token_budgets=None, flags: int = 0):
+    """``decode_sparse_attn`` over a cache held in 8 bits (aoakv_decode_sparse_attn_fp8): one
+    token per sequence, sel_pages [B, Hkv, n] as topk_filtering and estimate_topk write it,
+    None = every page.  ``workspace``: as decode_workspace makes it."""
+    _host.decode_sparse_attn_fp8(q, o, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len,
+                                 sel_pages, token_budget, workspace, max_pages, layout,
+                                 token_budgets, flags)

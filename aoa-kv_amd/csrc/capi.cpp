@@ -34,6 +34,28 @@ RopeFreqs rope_freqs(float rope_scale, float rope_theta, uint32_t head_dim) {
   last.r = r;
   return r;
 }
+
+// f_i / 2 pi of f_i = theta^(-2 i / D) / scale: of the turns that a position makes of it
+// only the fraction counts
+static RopeTurns rope_turns(float rope_scale, float rope_theta, uint32_t head_dim) {
+  thread_local struct {
+    float scale, theta;
+    uint32_t dim = 0u;
+    RopeTurns r;
+  } last;
+  if (last.dim == head_dim && last.scale == rope_scale && last.theta == rope_theta) return last.r;
+  RopeTurns r{};
+  for (uint32_t i = 0; i < head_dim / 2u; ++i) {
+    const long double f = std::pow((long double)rope_theta, -2.0L * i / head_dim) /
+                          rope_scale / 6.283185307179586476925286766559L;
+    r.turns[i] = (uint64_t)std::ldexp(f - std::floor(f), 64);
+  }
+  last.scale = rope_scale;
+  last.theta = rope_theta;
+  last.dim = head_dim;
+  last.r = r;
+  return r;
+}
 }  // namespace aoakv
 
 namespace {
@@ -1133,6 +1155,227 @@ int aoakv_chunk_attn(const void* q, void* o, float* lse, const int32_t* q_indptr
                                                                    page_size);
   return hip_status(aoakv::launch_chunk_attn(a, head_dim, static_cast<hipStream_t>(stream)),
                     "chunk_attn");
+}
+
+int aoakv_chunk_attn_fp8(const void* q, void* o, float* lse, const int32_t* q_indptr,
+                         uint32_t num_q_tokens, const void* kv_data, const int8_t* kv_exp,
+                         const int32_t* kv_indptr, const int32_t* kv_indices,
+                         const int32_t* kv_last_page_len, const int32_t* prefix_len,
+                         const float* slopes, uint32_t batch_size, uint32_t max_pages,
+                         uint32_t num_qo_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                         uint32_t page_size, uint32_t layout, uint32_t causal, uint32_t window,
+                         float soft_cap, void* workspace, size_t workspace_bytes,
+                         uint32_t* error_word, void* stream) {
+  aoakv::ChunkArgs a{};
+  if (int e = fill_chunk(a, q, q_indptr, num_q_tokens, kv_data, kv_indptr, kv_indices,
+                         kv_last_page_len, prefix_len, slopes, batch_size, max_pages,
+                         num_qo_heads, num_kv_heads, head_dim, page_size, layout, causal, window,
+                         soft_cap, workspace, workspace_bytes, 0u, error_word, "chunk_attn_fp8"))
+    return e;
+  REQUIRE(kv_exp, "chunk_attn_fp8: null pointer argument");
+  if (num_q_tokens == 0u) return ok();
+  REQUIRE(o, "chunk_attn_fp8: null pointer argument");
+  REQUIRE(aligned16(o), "chunk_attn_fp8: o not aligned to 16 bytes");
+  a.kv = nullptr;
+  a.kv8 = static_cast<const uint8_t*>(kv_data);
+  a.kv_exp = kv_exp;
+  a.o = static_cast<aoakv::f16*>(o);
+  a.lse = lse;
+  a.cuts = workspace;
+  a.whole = workspace == nullptr ||
+            workspace_bytes < aoakv_chunk_attn_call_workspace_size(num_q_tokens, batch_size,
+                                                                   max_pages, num_qo_heads,
+                                                                   num_kv_heads, head_dim,
+                                                                   page_size);
+  return hip_status(aoakv::launch_chunk_attn_fp8(a, head_dim, static_cast<hipStream_t>(stream)),
+                    "chunk_attn_fp8");
+}
+
+// What the calls that write to and read from a cache of codes have alike.
+static int fill_fp8(aoakv::AppendFp8Args& a, const int32_t* token_indptr, uint32_t num_tokens,
+                    const void* kv_data, const int8_t* kv_exp, const int32_t* kv_indptr,
+                    const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                    uint32_t batch_size, uint32_t num_qo_heads, uint32_t num_heads,
+                    uint32_t head_dim, uint32_t page_size, uint32_t layout, const char* fn) {
+  if (int e = check_shape(head_dim, page_size, layout, num_heads)) return e;
+  REQUIRE(token_indptr && kv_data && kv_exp && kv_indptr && kv_indices && kv_last_page_len,
+          "%s: null pointer argument", fn);
+  REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
+  REQUIRE(aligned16(kv_data), "%s: kv_data not aligned to 16 bytes", fn);
+  // (a dispatch's work-items are counted in 32 bits: 2^24 workgroups of 256)
+  const uint64_t heads = 2048u / head_dim;
+  const uint64_t groups = (num_heads + heads - 1u) / heads + (num_qo_heads + heads - 1u) / heads;
+  REQUIRE((num_tokens / page_size + 2ull * batch_size) * groups < (1ull << 24),
+          "%s: too many tokens (%u) in one call", fn, num_tokens);
+  a.tok_indptr = token_indptr;
+  a.kv = static_cast<uint8_t*>(const_cast<void*>(kv_data));
+  a.kv_exp = const_cast<int8_t*>(kv_exp);
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.T = num_tokens;
+  a.B = batch_size;
+  a.H = num_heads;
+  a.Hq = num_qo_heads;
+  a.S = page_size;
+  a.g = aoakv::make_geom(layout, num_heads, page_size, head_dim);
+  return AOAKV_OK;
+}
+
+static int append_fp8(void* q, const void* k, const void* v, const int32_t* token_indptr,
+                      uint32_t num_tokens, uint32_t num_qo_heads, void* kv_data, int8_t* kv_exp,
+                      const int32_t* kv_indptr, const int32_t* kv_indices,
+                      const int32_t* kv_last_page_len, void* metadata_data,
+                      const int32_t* metadata_indptr, const int32_t* metadata_indices,
+                      void* v_log_norm, void* v_mean, uint32_t batch_size, uint32_t num_heads,
+                      uint32_t head_dim, uint32_t page_size, uint32_t layout, float rope_scale,
+                      float rope_theta, void* stream, const char* fn) {
+  aoakv::AppendFp8Args a{};
+  if (int e = fill_fp8(a, token_indptr, num_tokens, kv_data, kv_exp, kv_indptr, kv_indices,
+                       kv_last_page_len, batch_size, num_qo_heads, num_heads, head_dim, page_size,
+                       layout, fn))
+    return e;
+  const int given = (metadata_data != nullptr) + (metadata_indptr != nullptr) +
+                    (metadata_indices != nullptr) + (v_log_norm != nullptr) + (v_mean != nullptr);
+  REQUIRE(given == 0 || given == 5, "%s: the page statistics' arguments are all given or all NULL",
+          fn);
+  REQUIRE(aligned16(metadata_data) && aligned16(v_mean),
+          "%s: metadata_data or v_mean not aligned to 16 bytes", fn);
+  if (num_tokens == 0u) return ok();
+  REQUIRE(k && v, "%s: null pointer argument", fn);
+  REQUIRE(aligned16(k) && aligned16(v), "%s: k or v not aligned to 16 bytes", fn);
+  a.k = static_cast<const aoakv::f16*>(k);
+  a.v = static_cast<const aoakv::f16*>(v);
+  a.meta = static_cast<aoakv::f16*>(metadata_data);
+  a.meta_indptr = metadata_indptr;
+  a.meta_indices = metadata_indices;
+  a.v_log_norm = static_cast<aoakv::f16*>(v_log_norm);
+  a.v_mean = static_cast<aoakv::f16*>(v_mean);
+  if (num_qo_heads != 0u) {
+    REQUIRE(q, "%s: null pointer argument", fn);
+    REQUIRE(aligned16(q), "%s: q not aligned to 16 bytes", fn);
+    const size_t row = (size_t)num_tokens * head_dim * sizeof(aoakv::f16);
+    auto apart = [&](const void* x) {
+      const uintptr_t q0 = (uintptr_t)q, x0 = (uintptr_t)x;
+      return q0 + row * num_qo_heads <= x0 || x0 + row * num_heads <= q0;
+    };
+    REQUIRE(apart(k) && apart(v), "%s: q shares memory with k or v", fn);
+    a.q = static_cast<aoakv::f16*>(q);
+    a.rope = aoakv::rope_turns(rope_scale, rope_theta, head_dim);
+  }
+  return hip_status(aoakv::launch_append_fp8(a, head_dim, static_cast<hipStream_t>(stream)), fn);
+}
+
+int aoakv_append_kv_cache_fp8(const void* k, const void* v, const int32_t* token_indptr,
+                              uint32_t num_tokens, void* kv_data, int8_t* kv_exp,
+                              const int32_t* kv_indptr, const int32_t* kv_indices,
+                              const int32_t* kv_last_page_len, void* metadata_data,
+                              const int32_t* metadata_indptr, const int32_t* metadata_indices,
+                              void* v_log_norm, void* v_mean, uint32_t batch_size,
+                              uint32_t num_heads, uint32_t head_dim, uint32_t page_size,
+                              uint32_t layout, void* stream) {
+  return append_fp8(nullptr, k, v, token_indptr, num_tokens, 0u, kv_data, kv_exp, kv_indptr,
+                    kv_indices, kv_last_page_len, metadata_data, metadata_indptr,
+                    metadata_indices, v_log_norm, v_mean, batch_size, num_heads, head_dim,
+                    page_size, layout, 1.f, 1.f, stream, "append_kv_cache_fp8");
+}
+
+int aoakv_rope_append_kv_cache_fp8(void* q, const void* k, const void* v,
+                                   const int32_t* token_indptr, uint32_t num_tokens,
+                                   uint32_t num_qo_heads, void* kv_data, int8_t* kv_exp,
+                                   const int32_t* kv_indptr, const int32_t* kv_indices,
+                                   const int32_t* kv_last_page_len, void* metadata_data,
+                                   const int32_t* metadata_indptr,
+                                   const int32_t* metadata_indices, void* v_log_norm,
+                                   void* v_mean, uint32_t batch_size, uint32_t num_heads,
+                                   uint32_t head_dim, uint32_t page_size, uint32_t layout,
+                                   float rope_scale, float rope_theta, void* stream) {
+  const char* fn = "rope_append_kv_cache_fp8";
+  REQUIRE(num_qo_heads >= 1u && num_qo_heads <= 256u, "%s: num_qo_heads %u out of range [1, 256]",
+          fn, num_qo_heads);
+  if (int e = check_rope(rope_scale, rope_theta, fn)) return e;
+  return append_fp8(q, k, v, token_indptr, num_tokens, num_qo_heads, kv_data, kv_exp, kv_indptr,
+                    kv_indices, kv_last_page_len, metadata_data, metadata_indptr,
+                    metadata_indices, v_log_norm, v_mean, batch_size, num_heads, head_dim,
+                    page_size, layout, rope_scale, rope_theta, stream, fn);
+}
+
+int aoakv_read_kv_cache_fp8(void* k, void* v, const int32_t* token_indptr, uint32_t num_tokens,
+                            const void* kv_data, const int8_t* kv_exp, const int32_t* kv_indptr,
+                            const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                            uint32_t batch_size, uint32_t num_heads, uint32_t head_dim,
+                            uint32_t page_size, uint32_t layout, void* stream) {
+  aoakv::AppendFp8Args a{};
+  if (int e = fill_fp8(a, token_indptr, num_tokens, kv_data, kv_exp, kv_indptr, kv_indices,
+                       kv_last_page_len, batch_size, 0u, num_heads, head_dim, page_size, layout,
+                       "read_kv_cache_fp8"))
+    return e;
+  if (num_tokens == 0u) return ok();
+  REQUIRE(k && v, "read_kv_cache_fp8: null pointer argument");
+  REQUIRE(aligned16(k) && aligned16(v), "read_kv_cache_fp8: k or v not aligned to 16 bytes");
+  a.k_out = static_cast<aoakv::f16*>(k);
+  a.v_out = static_cast<aoakv::f16*>(v);
+  return hip_status(aoakv::launch_read_fp8(a, head_dim, static_cast<hipStream_t>(stream)),
+                    "read_kv_cache_fp8");
+}
+
+int aoakv_decode_sparse_attn_fp8(const void* q, void* o, const void* kv_data,
+                                 const int8_t* kv_exp, const int32_t* kv_indptr,
+                                 const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                 const int32_t* sel_pages, uint32_t sel_stride,
+                                 uint32_t token_budget, const int32_t* token_budgets,
+                                 void* workspace, size_t workspace_bytes, uint32_t batch_size,
+                                 uint32_t max_pages, uint32_t num_qo_heads, uint32_t num_kv_heads,
+                                 uint32_t head_dim, uint32_t page_size, uint32_t layout,
+                                 uint32_t flags, void* stream) {
+  const char* fn = "decode_sparse_attn_fp8";
+  if (int e = check_flags(flags, AOAKV_FLAG_QUEST_KERNEL, fn)) return e;
+  if (int e = check_shape(head_dim, page_size, layout, num_qo_heads)) return e;
+  if (int e = check_group(num_qo_heads, num_kv_heads)) return e;
+  REQUIRE(q && o && kv_data && kv_exp && kv_indptr && kv_indices && kv_last_page_len && workspace,
+          "%s: null pointer argument", fn);
+  REQUIRE(batch_size >= 1u && batch_size <= 65535u, "%s: bad batch_size %u", fn, batch_size);
+  REQUIRE(max_pages >= 1u && (uint64_t)max_pages * page_size <= aoakv::kMaxChunkTokens,
+          "%s: max_pages %u of %u tokens not in [1, 2^27 tokens]", fn, max_pages, page_size);
+  REQUIRE(!sel_pages || sel_stride >= min_sel_stride(flags), "%s: sel_stride %u < %u", fn,
+          sel_stride, min_sel_stride(flags));
+  REQUIRE(aligned16(q) && aligned16(kv_data), "%s: q or kv_data not aligned to 16 bytes", fn);
+  const uint32_t max_sel = max_selected(sel_pages, sel_stride, token_budget, token_budgets,
+                                        max_pages, page_size, flags);
+  const uint64_t chunks = aoakv::decode_chunks(max_sel);
+  // (a dispatch's work-items are counted in 32 bits: 2^24 workgroups of 256)
+  REQUIRE((sel_pages ? chunks * batch_size : batch_size + 513ull) * num_kv_heads < (1ull << 24),
+          "%s: batch_size %u too large", fn, batch_size);
+  Workspace w{};
+  const size_t need =
+      ws_layout(batch_size, num_qo_heads, num_kv_heads, max_sel, head_dim, workspace, &w);
+  REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes < %zu needed", fn, workspace_bytes,
+          need);
+  aoakv::DecodeFp8Args a{};
+  a.q = static_cast<const aoakv::f16*>(q);
+  a.o = static_cast<aoakv::f16*>(o);
+  a.kv = static_cast<const uint8_t*>(kv_data);
+  a.kv_exp = kv_exp;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.sel = sel_pages;
+  a.sel_stride = sel_stride;
+  a.token_budget = token_budget;
+  a.token_budgets = token_budgets;
+  a.partial = w.partial;
+  a.counters = w.dec_counters;
+  a.Hq = num_qo_heads;
+  a.Hkv = num_kv_heads;
+  a.S = page_size;
+  a.max_chunks = (uint32_t)chunks;
+  a.max_pages = max_pages;
+  a.batch = batch_size;
+  a.flags = flags;
+  a.scale = 1.4426950408889634f / std::sqrt((float)head_dim);
+  a.g = aoakv::make_geom(layout, num_kv_heads, page_size, head_dim);
+  a.error = w.ctl + aoakv::kErrWord;
+  return hip_status(aoakv::launch_decode_fp8(a, head_dim, static_cast<hipStream_t>(stream)), fn);
 }
 
 size_t aoakv_attn_weights_workspace_size(void) { return aoakv::attn_weights_workspace(); }

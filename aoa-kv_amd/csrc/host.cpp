@@ -37,7 +37,8 @@ struct PyErr {};
   X(topk_filtering) X(decode_sparse_attn) X(sparse_decode_layer)                       \
   X(prefill_workspace_size) X(prefill_with_workspace)                                  \
   X(chunk_attn_call_workspace_size) X(chunk_attn) X(attn_weights_workspace_size) X(attn_weights) X(keep_tokens)          \
-  X(compact_kv_cache) X(last_error)
+  X(compact_kv_cache) X(append_kv_cache_fp8) X(rope_append_kv_cache_fp8)               \
+  X(read_kv_cache_fp8) X(chunk_attn_fp8) X(decode_sparse_attn_fp8) X(last_error)
 
 struct Lib {
 #define X(n) decltype(&aoakv_##n) n = nullptr;
@@ -62,7 +63,8 @@ std::string shape_str(const Tensor& t) {
 
 const char* dtype_name(at::ScalarType t) {
   return t == at::kHalf ? "torch.float16" : t == at::kFloat ? "torch.float32"
-         : t == at::kInt ? "torch.int32" : "torch.uint8";
+         : t == at::kInt ? "torch.int32" : t == at::kFloat8_e4m3fn ? "torch.float8_e4m3fn"
+         : t == at::kChar ? "torch.int8" : "torch.uint8";
 }
 
 // A contiguous device tensor of this dtype.
@@ -524,8 +526,10 @@ struct Chunks {
 };
 // q, q_indptr; t: kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages,
 // layout, causal, window, soft_cap, slopes, prefix_len
-Chunks chunk_args(PyObject* q_, PyObject* q_indptr, PyObject* const* t) {
-  const Tensor &q = here(q_, "q", at::kHalf), &kv = here(t[0], "kv_data", at::kHalf);
+// (the cache's own type: fp16, or codes)
+Chunks chunk_args(PyObject* q_, PyObject* q_indptr, PyObject* const* t,
+                  at::ScalarType kind = at::kHalf) {
+  const Tensor &q = here(q_, "q", at::kHalf), &kv = here(t[0], "kv_data", kind);
   const Dims d = cache_dims(kv, t[5]);
   if (q.dim() != 3 || q.size(2) != d.D)
     raise(PyExc_ValueError, "q must be [T, Hq, " + std::to_string(d.D) + "], got " + shape_str(q));
@@ -543,16 +547,29 @@ Chunks chunk_args(PyObject* q_, PyObject* q_indptr, PyObject* const* t) {
                 u32(t[6]), size31(t[7], "window"), f32(t[8])};
 }
 
-// (q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages,
-//  layout, causal, window, soft_cap, slopes, prefix_len, o or None, return_lse,
-//  workspace) -> o or (o, lse)
-PyObject* chunk_attn(PyObject* const* a) {
-  const Chunks c = chunk_args(a[0], a[1], a + 2);
-  const Tensor* given = here_or_null(a[13], "o", at::kHalf);
+// the exponents of a cache of codes, [max_pages, 2, H]
+int8_t* exponents(PyObject* o, const Tensor& kv, const Dims& d) {
+  const Tensor& e = here(o, "kv_exp", at::kChar);
+  if (!is_shape(e, kv.size(0), 2, d.H))
+    raise(PyExc_ValueError, "kv_exp must be [" + std::to_string(kv.size(0)) + ", 2, " +
+                                std::to_string(d.H) + "], got " + shape_str(e));
+  return static_cast<int8_t*>(ptr(e));
+}
+PyObject* two(const Tensor& a, const Tensor& b) {
+  PyObject *x = THPVariable_Wrap(a), *y = THPVariable_Wrap(b);
+  PyObject* both = x != nullptr && y != nullptr ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return both;
+}
+
+// a: q, q_indptr, then the call's options from o or None on; exp: of codes, or nullptr
+PyObject* chunk_call(const Chunks& c, const int8_t* exp, PyObject* const* a, const char* name) {
+  const Tensor* given = here_or_null(a[0], "o", at::kHalf);
   if (given != nullptr && given->sizes() != c.q.sizes())
     raise(PyExc_ValueError, "o must have q's shape");
-  const bool want = u32(a[14]) != 0u;
-  uint32_t* err = error_word(a[15]);
+  const bool want = u32(a[1]) != 0u;
+  uint32_t* err = error_word(a[2]);
   const Tensor o = given != nullptr ? *given : at::empty_like(c.q);
   Tensor lse;
   if (want) lse = at::empty({c.q.size(0), c.q.size(1)}, c.q.options().dtype(at::kFloat));
@@ -567,19 +584,172 @@ PyObject* chunk_attn(PyObject* const* a) {
     }
   }
   void* s = stream();
-  call("aoakv_chunk_attn", [&] {
-    return g_lib.chunk_attn(ptr(c.q), ptr(o), want ? static_cast<float*>(ptr(lse)) : nullptr,
-                            c.q_indptr, c.T, ptr(c.kv), c.t.indptr, c.t.indices, c.t.last,
-                            c.prefix, c.slopes, (uint32_t)c.t.B, c.max_pages, c.Hq, c.d.H, c.d.D,
-                            c.d.S, c.d.layout, c.causal, c.window, c.cap,
-                            n != 0 ? ptr(ws) : nullptr, n, err, s);
+  float* l = want ? static_cast<float*>(ptr(lse)) : nullptr;
+  void* w = n != 0 ? ptr(ws) : nullptr;
+  call(name, [&] {
+    if (exp != nullptr)
+      return g_lib.chunk_attn_fp8(ptr(c.q), ptr(o), l, c.q_indptr, c.T, ptr(c.kv), exp, c.t.indptr,
+                                  c.t.indices, c.t.last, c.prefix, c.slopes, (uint32_t)c.t.B,
+                                  c.max_pages, c.Hq, c.d.H, c.d.D, c.d.S, c.d.layout, c.causal,
+                                  c.window, c.cap, w, n, err, s);
+    return g_lib.chunk_attn(ptr(c.q), ptr(o), l, c.q_indptr, c.T, ptr(c.kv), c.t.indptr,
+                            c.t.indices, c.t.last, c.prefix, c.slopes, (uint32_t)c.t.B,
+                            c.max_pages, c.Hq, c.d.H, c.d.D, c.d.S, c.d.layout, c.causal,
+                            c.window, c.cap, w, n, err, s);
   });
-  if (!want) return THPVariable_Wrap(o);
-  PyObject *x = THPVariable_Wrap(o), *y = THPVariable_Wrap(lse);
-  PyObject* both = x != nullptr && y != nullptr ? PyTuple_Pack(2, x, y) : nullptr;
-  Py_XDECREF(x);
-  Py_XDECREF(y);
-  return both;
+  return want ? two(o, lse) : THPVariable_Wrap(o);
+}
+
+// (q, q_indptr, kv_data, kv_indptr, kv_indices, kv_last_page_len, max_pages,
+//  layout, causal, window, soft_cap, slopes, prefix_len, o or None, return_lse,
+//  workspace) -> o or (o, lse)
+PyObject* chunk_attn(PyObject* const* a) {
+  return chunk_call(chunk_args(a[0], a[1], a + 2), nullptr, a + 13, "aoakv_chunk_attn");
+}
+
+// (..., kv_data, kv_indptr, ... as chunk_attn, kv_exp)
+PyObject* chunk_attn_fp8(PyObject* const* a) {
+  const Chunks c = chunk_args(a[0], a[1], a + 2, at::kFloat8_e4m3fn);
+  return chunk_call(c, exponents(a[16], c.kv, c.d), a + 13, "aoakv_chunk_attn_fp8");
+}
+
+// What the calls that append to and read a cache of codes have alike.
+struct Codes {
+  const Tensor& kv;
+  int8_t* exp;
+  Dims d;
+  PageTable t;
+  const int32_t* tok_indptr;
+};
+// t: token_indptr, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len, layout
+Codes codes(PyObject* const* t) {
+  const Tensor& kv = here(t[1], "kv_data", at::kFloat8_e4m3fn);
+  const Dims d = cache_dims(kv, t[6]);
+  int8_t* exp = exponents(t[2], kv, d);
+  const PageTable table = page_table(t + 3);
+  const Tensor& ip = here(t[0], "token_indptr", at::kInt);
+  if (ip.numel() != table.B + 1) raise(PyExc_ValueError, "token_indptr does not match the batch");
+  return Codes{kv, exp, d, table, static_cast<const int32_t*>(ptr(ip))};
+}
+const Tensor& token_rows(PyObject* o, const char* name, const Dims& d, int64_t T) {
+  const Tensor& x = here(o, name, at::kHalf);
+  if (T < 0 && x.dim() == 3) T = x.size(0);
+  if (!is_shape(x, T, d.H, d.D) || T > 0x7FFFFFFF)
+    raise(PyExc_ValueError, std::string(name) + " must be [T, " + std::to_string(d.H) + ", " +
+                                std::to_string(d.D) + "], got " + shape_str(x));
+  return x;
+}
+// metadata_data, metadata_indptr, metadata_indices, v_log_norm, v_mean: tensors or None
+struct Statistics {
+  void* meta = nullptr;
+  const int32_t *indptr = nullptr, *indices = nullptr;
+  void *log_norm = nullptr, *mean = nullptr;
+};
+Statistics statistics(PyObject* const* a, const Codes& c, PyObject* layout) {
+  int none = 0;
+  for (int i = 0; i < 5; ++i) none += a[i] == Py_None;
+  if (none == 5) return Statistics{};
+  if (none != 0)
+    raise(PyExc_ValueError, "the page statistics' arguments are all given or all None");
+  const Tensor &meta = here(a[0], "metadata_data", at::kHalf),
+               &ip = here(a[1], "metadata_indptr", at::kInt),
+               &ix = here(a[2], "metadata_indices", at::kInt),
+               &log_norm = here(a[3], "v_log_norm", at::kHalf),
+               &mean = here(a[4], "v_mean", at::kHalf);
+  const Dims md = cache_dims(meta, layout);
+  if (md.S != c.d.S || md.H != c.d.H || md.D != c.d.D)
+    raise(PyExc_ValueError, "metadata_data's pages must be as kv_data's");
+  if (log_norm.numel() != c.kv.size(0) * c.d.H || mean.numel() != c.kv.size(0) * c.d.H * c.d.D)
+    raise(PyExc_ValueError, "v_log_norm must be [max_pages, H] and v_mean [max_pages, H, D]");
+  if (ip.numel() != c.t.B + 1)
+    raise(PyExc_ValueError, "metadata_indptr does not match the batch");
+  return Statistics{ptr(meta), static_cast<const int32_t*>(ptr(ip)),
+                    static_cast<const int32_t*>(ptr(ix)), ptr(log_norm), ptr(mean)};
+}
+
+// (k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len, layout,
+//  metadata_data, metadata_indptr, metadata_indices, v_log_norm, v_mean)
+void append_kv_cache_fp8(PyObject* const* a) {
+  const Codes c = codes(a + 2);
+  const Tensor &k = token_rows(a[0], "k", c.d, -1), &v = token_rows(a[1], "v", c.d, k.size(0));
+  const Statistics m = statistics(a + 9, c, a[8]);
+  void* s = stream();
+  call("aoakv_append_kv_cache_fp8", [&] {
+    return g_lib.append_kv_cache_fp8(ptr(k), ptr(v), c.tok_indptr, (uint32_t)k.size(0), ptr(c.kv),
+                                     c.exp, c.t.indptr, c.t.indices, c.t.last, m.meta, m.indptr,
+                                     m.indices, m.log_norm, m.mean, (uint32_t)c.t.B, c.d.H, c.d.D,
+                                     c.d.S, c.d.layout, s);
+  });
+}
+
+// (q, k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len, layout,
+//  rope_scale, rope_theta, metadata_data, metadata_indptr, metadata_indices, v_log_norm,
+//  v_mean)
+void rope_append_kv_cache_fp8(PyObject* const* a) {
+  const Codes c = codes(a + 3);
+  const Tensor &k = token_rows(a[1], "k", c.d, -1), &v = token_rows(a[2], "v", c.d, k.size(0)),
+               &q = here(a[0], "q", at::kHalf);
+  if (q.dim() != 3 || q.size(0) != k.size(0) || q.size(2) != c.d.D)
+    raise(PyExc_ValueError, "q must be [" + std::to_string(k.size(0)) + ", Hq, " +
+                                std::to_string(c.d.D) + "], got " + shape_str(q));
+  const Statistics m = statistics(a + 12, c, a[9]);
+  const float scale = f32(a[10]), theta = f32(a[11]);
+  void* s = stream();
+  call("aoakv_rope_append_kv_cache_fp8", [&] {
+    return g_lib.rope_append_kv_cache_fp8(
+        ptr(q), ptr(k), ptr(v), c.tok_indptr, (uint32_t)k.size(0), (uint32_t)q.size(1), ptr(c.kv),
+        c.exp, c.t.indptr, c.t.indices, c.t.last, m.meta, m.indptr, m.indices, m.log_norm, m.mean,
+        (uint32_t)c.t.B, c.d.H, c.d.D, c.d.S, c.d.layout, scale, theta, s);
+  });
+}
+
+// (num_tokens, token_indptr, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len,
+//  layout, k or None, v or None) -> (k, v)
+PyObject* read_kv_cache_fp8(PyObject* const* a) {
+  const Codes c = codes(a + 1);
+  const int64_t T = size31(a[0], "num_tokens");
+  auto rows = [&](PyObject* o, const char* name) {
+    if (o != Py_None) return token_rows(o, name, c.d, T);
+    return at::empty({T, c.d.H, c.d.D}, c.kv.options().dtype(at::kHalf));
+  };
+  const Tensor k = rows(a[8], "k"), v = rows(a[9], "v");
+  void* s = stream();
+  call("aoakv_read_kv_cache_fp8", [&] {
+    return g_lib.read_kv_cache_fp8(ptr(k), ptr(v), c.tok_indptr, (uint32_t)T, ptr(c.kv), c.exp,
+                                   c.t.indptr, c.t.indices, c.t.last, (uint32_t)c.t.B, c.d.H,
+                                   c.d.D, c.d.S, c.d.layout, s);
+  });
+  return two(k, v);
+}
+
+// (q, o, kv_data, kv_exp, kv_indptr, kv_indices, kv_last_page_len, sel_pages, token_budget,
+//  workspace, max_pages, layout, token_budgets, flags)
+void decode_sparse_attn_fp8(PyObject* const* a) {
+  const Tensor &q = here(a[0], "q", at::kHalf), &o = here(a[1], "o", at::kHalf),
+               &kv = here(a[2], "kv_data", at::kFloat8_e4m3fn),
+               &ws = here(a[9], "workspace", at::kByte);
+  const Dims d = cache_dims(kv, a[11]);
+  const int8_t* exp = exponents(a[3], kv, d);
+  const PageTable t = page_table(a + 4);
+  if (q.dim() != 3 || q.size(0) != t.B || q.size(2) != d.D)
+    raise(PyExc_ValueError, "q must be [" + std::to_string(t.B) + ", Hq, " + std::to_string(d.D) +
+                                "], got " + shape_str(q));
+  if (q.sizes() != o.sizes()) raise(PyExc_ValueError, "o must have q's shape");
+  const Tensor* sel = here_or_null(a[7], "sel_pages", at::kInt);
+  if (sel != nullptr && (sel->dim() != 3 || sel->size(0) != t.B || sel->size(1) != d.H))
+    raise(PyExc_ValueError, "sel_pages must be [" + std::to_string(t.B) + ", " +
+                                std::to_string(d.H) + ", n], got " + shape_str(*sel));
+  const int32_t* budgets = per_sequence(a[12], "token_budgets", t.B);
+  const uint32_t budget = size31(a[8], "token_budget"), pages = size31(a[10], "max_pages"),
+                 flags = u32(a[13]);
+  void* s = stream();
+  call("aoakv_decode_sparse_attn_fp8", [&] {
+    return g_lib.decode_sparse_attn_fp8(
+        ptr(q), ptr(o), ptr(kv), exp, t.indptr, t.indices, t.last,
+        data_or_null<const int32_t>(sel), sel != nullptr ? (uint32_t)sel->size(2) : 0u, budget,
+        budgets, ptr(ws), (size_t)ws.numel(), (uint32_t)t.B, pages, (uint32_t)q.size(1), d.H, d.D,
+        d.S, d.layout, flags, s);
+  });
 }
 
 // (q, lse, q_indptr, weights, kv_data, kv_indptr, kv_indices, kv_last_page_len,
@@ -736,6 +906,11 @@ PyMethodDef g_methods[] = {
     ENTRY(attn_weights, 17),
     ENTRY(keep_tokens, 10),
     ENTRY(compact_kv_cache, 17),
+    ENTRY(append_kv_cache_fp8, 14),
+    ENTRY(rope_append_kv_cache_fp8, 17),
+    ENTRY(read_kv_cache_fp8, 10),
+    ENTRY(chunk_attn_fp8, 17),
+    ENTRY(decode_sparse_attn_fp8, 14),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

@@ -295,6 +295,8 @@ struct ChunkArgs {
   float sm_scale, soft_cap;   // soft_cap 0: none
   PageGeom g;
   uint32_t* error;            // receives kErrTruncated, or nullptr
+  const uint8_t* kv8;         // the cache, where it holds codes (kv is then nullptr)
+  const int8_t* kv_exp;       // [pages, 2, H]
   void* cuts;                 // the workspace
   uint32_t whole;             // items are not cut (the attention: without a workspace;
                               // the weights: set by the launch)
@@ -317,6 +319,65 @@ size_t chunk_attn_workspace(uint32_t T, uint32_t B, uint32_t Hq, uint32_t H, uin
 size_t attn_weights_workspace();
 hipError_t launch_chunk_attn(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
 hipError_t launch_attn_weights(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
+hipError_t launch_chunk_attn_fp8(const ChunkArgs& a, uint32_t head_dim, hipStream_t s);
+
+// A paged cache of 8-bit codes (append_fp8.hip): new tokens of a ragged batch, and
+// tokens back as rows.  Sequence b's rows are tok_indptr[b] .. tok_indptr[b + 1] of k,
+// v and q (read: of k_out and v_out), the last of its cached tokens.
+//
+// Frequencies f_i / 2 pi, i < D / 2, as 64-bit fractions of a turn (the integer part
+// of what a position makes of them does not matter).
+struct RopeTurns {
+  uint64_t turns[kMaxHeadDim / 2];
+};
+struct AppendFp8Args {
+  const f16* k;           // [T, H, D]
+  const f16* v;           // [T, H, D]
+  f16* q;                 // [T, Hq, D] turned in place, or nullptr: neither q nor k turns
+  const int32_t* tok_indptr;
+  uint8_t* kv;            // codes
+  int8_t* kv_exp;         // [pages, 2, H]
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  f16* meta;              // or nullptr: no statistics
+  const int32_t* meta_indptr;
+  const int32_t* meta_indices;
+  f16* v_log_norm;
+  f16* v_mean;
+  f16* k_out;             // [T, H, D] (read)
+  f16* v_out;
+  uint32_t T, B, H, Hq, S;
+  PageGeom g;
+  RopeTurns rope;
+};
+hipError_t launch_append_fp8(const AppendFp8Args& a, uint32_t head_dim, hipStream_t s);
+hipError_t launch_read_fp8(const AppendFp8Args& a, uint32_t head_dim, hipStream_t s);
+
+// One token per sequence over a paged cache of codes (decode_fp8.hip): every page, or
+// the pages of a selection.
+struct DecodeFp8Args {
+  const f16* q;  // [B, Hq, D]
+  f16* o;        // [B, Hq, D]
+  const uint8_t* kv;
+  const int8_t* kv_exp;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  const int32_t* sel;  // [B, Hkv, sel_stride] physical ids, or nullptr (every page)
+  uint32_t sel_stride;
+  uint32_t token_budget;
+  const int32_t* token_budgets;
+  float* partial;      // [B * Hq, max_chunks, D + 4]
+  uint32_t* counters;  // a line per (sequence, query head)
+  uint32_t Hq, Hkv, S, max_chunks, max_pages, batch, flags;
+  float scale;         // log2(e) / sqrt(D)
+  PageGeom g;
+  uint32_t* error;
+  // set by the launch
+  uint32_t page_rcp, split, split_rcp;
+};
+hipError_t launch_decode_fp8(const DecodeFp8Args& a, uint32_t head_dim, hipStream_t s);
 
 // Eviction (evict.hip): the tokens a kv head keeps, and the cache packed down
 // to them.

@@ -21,7 +21,10 @@
  * sparse decode for one layer), aoakv_estimate_topk, and
  * aoakv_rope_append_kv_cache_decode (RoPE + decode append); and, beyond the
  * reference, aoakv_chunk_attn (attention of a ragged batch of chunks),
- * aoakv_attn_weights, aoakv_keep_tokens and aoakv_compact_kv_cache (eviction).
+ * aoakv_attn_weights, aoakv_keep_tokens and aoakv_compact_kv_cache (eviction),
+ * and a cache held in 8 bits: aoakv_append_kv_cache_fp8,
+ * aoakv_rope_append_kv_cache_fp8, aoakv_chunk_attn_fp8,
+ * aoakv_decode_sparse_attn_fp8 and aoakv_read_kv_cache_fp8.
  *
  * Conventions
  *   - All tensor arguments are device pointers (plain pointers, no torch
@@ -581,6 +584,101 @@ int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t k
                            uint32_t max_pages, uint32_t num_heads, uint32_t head_dim,
                            uint32_t page_size, uint32_t layout, uint32_t* error_word,
                            void* stream);
+
+/*
+ * A paged cache held in 8 bits.  No counterpart in the reference.
+ *
+ * kv_data: the layouts above with OCP e4m3 codes for elements (a byte each).
+ * kv_exp: int8 [max_pages, 2, num_kv_heads], for K (0) and V (1) of each page and
+ * kv head (a block) the exponent of its scale: an element is code * 2^exp.  The
+ * exponent of a block is the smallest e with max |x| <= 448 * 2^e over its tokens'
+ * finite values, held to [-15, 8]: every element is then an fp16 number, off by at
+ * most 2^-4 of itself, or by 2^(e - 10) where that is more.  At e = 8 elements end at
+ * 61440; inf and NaN are held as NaN.  Exponents outside [-15, 8] are read as the
+ * nearest.
+ *
+ * aoakv_append_kv_cache_fp8: new tokens of EVERY sequence of a batch (chunks of
+ * prompts, single tokens, mixed).  k, v: [num_tokens, num_heads, head_dim] fp16;
+ * sequence b's rows are token_indptr[b] .. token_indptr[b + 1] - 1 (int32,
+ * device, ascending; none is allowed), the last of its L_b cached tokens, which
+ * the page table already counts; rows of no sequence are not read.  A block that
+ * holds older tokens keeps their exponent or gets a larger one, to which their
+ * codes move (one rounding of those that become subnormal).  A page that begins
+ * with the chunk forgets what it held.  Sequences may share a page only if
+ * none of them appends to it.  The page statistics (metadata_data, metadata_indptr,
+ * metadata_indices, v_log_norm, v_mean: all given, or all NULL) become those of
+ * aoakv_append_kv_cache_prefill for the same fp16 rows, bit for bit: from the values
+ * before they were rounded to codes, so a selection is that of an fp16 cache.
+ *
+ * aoakv_rope_append_kv_cache_fp8: q [num_tokens, num_qo_heads, head_dim] and k turned
+ * on the way, row i of n_b at position L_b - n_b + i, as in
+ * aoakv_apply_rope_in_place but for the angle, which is exact to 2^-26 of a turn
+ * at every position (that call's is rounded to fp32).  q is turned in place; k
+ * is not written.  q may not share memory with k or v.
+ *
+ * k, v, q, kv_data, metadata_data and v_mean are aligned to 16 bytes.
+ */
+int aoakv_append_kv_cache_fp8(const void* k, const void* v, const int32_t* token_indptr,
+                              uint32_t num_tokens, void* kv_data, int8_t* kv_exp,
+                              const int32_t* kv_indptr, const int32_t* kv_indices,
+                              const int32_t* kv_last_page_len, void* metadata_data,
+                              const int32_t* metadata_indptr, const int32_t* metadata_indices,
+                              void* v_log_norm, void* v_mean, uint32_t batch_size,
+                              uint32_t num_heads, uint32_t head_dim, uint32_t page_size,
+                              uint32_t layout, void* stream);
+int aoakv_rope_append_kv_cache_fp8(void* q, const void* k, const void* v,
+                                   const int32_t* token_indptr, uint32_t num_tokens,
+                                   uint32_t num_qo_heads, void* kv_data, int8_t* kv_exp,
+                                   const int32_t* kv_indptr, const int32_t* kv_indices,
+                                   const int32_t* kv_last_page_len, void* metadata_data,
+                                   const int32_t* metadata_indptr,
+                                   const int32_t* metadata_indices, void* v_log_norm,
+                                   void* v_mean, uint32_t batch_size, uint32_t num_heads,
+                                   uint32_t head_dim, uint32_t page_size, uint32_t layout,
+                                   float rope_scale, float rope_theta, void* stream);
+
+/*
+ * The last n_b tokens of every sequence back as fp16 rows: k, v [num_tokens, num_heads,
+ * head_dim], rows by token_indptr as above, the elements' exact values.  Rows of no
+ * token are not written.  k and v are aligned to 16 bytes.
+ */
+int aoakv_read_kv_cache_fp8(void* k, void* v, const int32_t* token_indptr, uint32_t num_tokens,
+                            const void* kv_data, const int8_t* kv_exp, const int32_t* kv_indptr,
+                            const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                            uint32_t batch_size, uint32_t num_heads, uint32_t head_dim,
+                            uint32_t page_size, uint32_t layout, void* stream);
+
+/*
+ * aoakv_chunk_attn over a cache held in 8 bits: the same arguments, limits, options
+ * and workspace, with kv_exp.  Products are of fp16 operands (the elements' exact
+ * values), so the result is that of aoakv_chunk_attn over a cache of these.
+ */
+int aoakv_chunk_attn_fp8(const void* q, void* o, float* lse, const int32_t* q_indptr,
+                         uint32_t num_q_tokens, const void* kv_data, const int8_t* kv_exp,
+                         const int32_t* kv_indptr, const int32_t* kv_indices,
+                         const int32_t* kv_last_page_len, const int32_t* prefix_len,
+                         const float* slopes, uint32_t batch_size, uint32_t max_pages,
+                         uint32_t num_qo_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                         uint32_t page_size, uint32_t layout, uint32_t causal, uint32_t window,
+                         float soft_cap, void* workspace, size_t workspace_bytes,
+                         uint32_t* error_word, void* stream);
+
+/*
+ * aoakv_decode_sparse_attn over a cache held in 8 bits: the same arguments and
+ * workspace, with kv_exp; flags: AOAKV_FLAG_QUEST_KERNEL or 0.  The pages come from
+ * the statistics as before (aoakv_estimate_topk).  Scores are not rounded to fp16
+ * on the way to the softmax.  A sequence without a page gets zeros.  q and kv_data are
+ * aligned to 16 bytes.
+ */
+int aoakv_decode_sparse_attn_fp8(const void* q, void* o, const void* kv_data,
+                                 const int8_t* kv_exp, const int32_t* kv_indptr,
+                                 const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                 const int32_t* sel_pages, uint32_t sel_stride,
+                                 uint32_t token_budget, const int32_t* token_budgets,
+                                 void* workspace, size_t workspace_bytes, uint32_t batch_size,
+                                 uint32_t max_pages, uint32_t num_qo_heads, uint32_t num_kv_heads,
+                                 uint32_t head_dim, uint32_t page_size, uint32_t layout,
+                                 uint32_t flags, void* stream);
 
 #ifdef __cplusplus
 }
