@@ -1204,7 +1204,7 @@ static int fill_fp8(aoakv::AppendFp8Args& a, const int32_t* token_indptr, uint32
   REQUIRE(aligned16(kv_data), "%s: kv_data not aligned to 16 bytes", fn);
   // (a dispatch's work-items are counted in 32 bits: 2^24 workgroups of 256)
   const uint64_t heads = 2048u / head_dim;
-  const uint64_t groups = (num_heads + heads - 1u) / heads + (num_qo_heads + heads - 1u) / heads;
+  const uint64_t groups = (2u * num_heads + num_qo_heads + heads - 1u) / heads;
   REQUIRE((num_tokens / page_size + 2ull * batch_size) * groups < (1ull << 24),
           "%s: too many tokens (%u) in one call", fn, num_tokens);
   a.tok_indptr = token_indptr;

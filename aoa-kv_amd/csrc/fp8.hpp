@@ -68,6 +68,17 @@ __device__ inline uint2 encode8(const H8& v, int e) {
   return uint2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
+// The larger of two pairs of |x| (fp16 bits order as whole numbers do), over 8 values.
+__device__ inline uint32_t pair_top(const H8& v, uint32_t top) {
+  typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+  const uint4 u = __builtin_bit_cast(uint4, v);
+  ushort2v t = __builtin_bit_cast(ushort2v, top);
+  t = __builtin_elementwise_max(t, __builtin_bit_cast(ushort2v, u.x & 0x7FFF7FFFu));
+  t = __builtin_elementwise_max(t, __builtin_bit_cast(ushort2v, u.y & 0x7FFF7FFFu));
+  t = __builtin_elementwise_max(t, __builtin_bit_cast(ushort2v, u.z & 0x7FFF7FFFu));
+  t = __builtin_elementwise_max(t, __builtin_bit_cast(ushort2v, u.w & 0x7FFF7FFFu));
+  return __builtin_bit_cast(uint32_t, t);
+}
 // The largest |x| among 8 values and `top` (fp16 bits): what is not finite counts 0.
 __device__ inline uint32_t finite_top(const H8& v, uint32_t top) {
 #pragma unroll

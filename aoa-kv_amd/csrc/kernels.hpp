@@ -349,6 +349,7 @@ struct AppendFp8Args {
   f16* v_out;
   uint32_t T, B, H, Hq, S;
   PageGeom g;
+  uint32_t stream;        // (set by the launch) rows pass the caches by
   RopeTurns rope;
 };
 hipError_t launch_append_fp8(const AppendFp8Args& a, uint32_t head_dim, hipStream_t s);

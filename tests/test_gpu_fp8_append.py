@@ -327,3 +327,23 @@ def test_graph_and_streams():
             assert torch.equal(x[rowsof].view(torch.int16), y[rowsof].view(torch.int16))
         assert torch.equal(qa, qb) and torch.equal(a.exp, b.exp)
         (torch.randn(1000, device=DEV) * 2).sum().item()
+
+
+def test_large_calls():
+    """A call whose rows pass the caches by gives the bits of smaller ones."""
+    from aoakv import ops
+    _say("[append fp8] large")
+    H, G, D, S, n = 32, 1, 64, 16, [3001, 2999]
+    one, two = (Coded(n, n, D, S, H, G, seed=13, margin=0) for _ in range(2))
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, v = (torch.randn((sum(n), H, D), generator=g, device=DEV).half() for _ in range(3))
+    q2 = q.clone()
+    assert q.numel() * 2 * 3 >= 64 << 20
+    ops.rope_append_kv_cache_fp8(q, k, v, one.q_indptr, *one.table(), HND)
+    for b in range(2):
+        a = slice(two.q0[b], two.q0[b + 1])
+        ops.rope_append_kv_cache_fp8(q2[a], k[a], v[a], i32(0, n[b]), two.kv, two.exp,
+                                     two.indptr[b:b + 2].contiguous(), two.indices,
+                                     two.last[b:b + 1].contiguous(), HND)
+    assert torch.equal(q, q2) and torch.equal(one.exp, two.exp)
+    assert torch.equal(one.bytes(), two.bytes())
