@@ -15,11 +15,10 @@
 //               (dims D / 16 m + t of lane m) is a shuffle within its own registers.
 // Neither operand passes through LDS.  Chunks are joined through the workspace by the
 // last one to arrive.
-#include <type_traits>
-
 #include "fp8.hpp"
 #include "kernels.hpp"
 #include "mfma_tile.hpp"
+#include "topk.hpp"
 
 namespace aoakv {
 namespace {
@@ -43,49 +42,102 @@ __device__ inline float quarters(float x, F&& f) {
 __device__ inline float max2(float x, float y) { return fmaxf(x, y); }
 __device__ inline float add2(float x, float y) { return x + y; }
 
-// n / d, rounded up, for 1 <= n, rcp = floor(2^32 / d) + 1 (0: d = 1); from n * d = 2^32
-// on it may be more
-__device__ inline uint32_t div_up(uint32_t n, uint32_t rcp) {
-  return rcp == 0u ? n : (uint32_t)(((uint64_t)(n - 1u) * rcp) >> 32) + 1u;
-}
-
-// Chunk `chunk` of `per` pages of sequence b.
+// Chunk `chunk` of `per` pages of sequence b, whose table begins at `beg` and has `held`
+// pages, the last of `last` tokens.
 struct Place {
-  uint32_t b, chunk, per;
+  uint32_t b, chunk, per, beg;
+  int32_t held;
+  uint32_t last;
 };
-// The item-th of a call over every page: the pages of all sequences are cut into
-// a.split chunks per kv head, at least kGenChunkPages pages each; sequence b's items
-// begin at floor(pages before it / per) + b, room for its chunks, and for one where it
-// has no page.
+__device__ inline Place place_of(const DecodeFp8Args& a, uint32_t b, uint32_t chunk, uint32_t per) {
+  const uint32_t beg = (uint32_t)a.kv_indptr[b];
+  return Place{b, chunk, per, beg, a.kv_indptr[b + 1u] - (int32_t)beg,
+               (uint32_t)a.kv_last_page_len[b]};
+}
+// The item-th of a call over every page.  The pages of all sequences are cut into chunks of
+// as few pages (at least kGenChunkPages) as leaves a.split of them per kv head, so that all
+// are at work at once and end together.  (Cut into chunks of a.split-ths, 16 sequences made
+// some more than the GPU holds at once: 76 us, now XX.)  A sequence without a page has one.
 __device__ inline Place find_chunk(const DecodeFp8Args& a, uint32_t item) {
+  const uint32_t lane = __lane_id();
+  auto of = [](uint32_t x, uint32_t j) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)j);
+  };
+  if (a.batch <= (uint32_t)kWave) {  // a lane per sequence
+    const uint32_t i = lane < a.batch ? lane : a.batch - 1u;
+    const uint32_t beg = (uint32_t)a.kv_indptr[i];
+    const int32_t held = a.kv_indptr[i + 1u] - (int32_t)beg;
+    const uint32_t last = (uint32_t)a.kv_last_page_len[i];
+    uint32_t P = held > 0 ? (uint32_t)held : 0u;
+    if (P > a.max_pages) P = a.max_pages;
+    if (lane >= a.batch) P = 0u;
+    const uint32_t total = of(wave_incl_scan(P), kWave - 1u);
+    // chunks of `per` pages; the smallest per that leaves few enough lies between total /
+    // split and total / (split - batch) (many sequences: an equal share)
+    uint32_t n = 0u;
+    auto chunks = [&](uint32_t per) {
+      n = lane < a.batch ? (P + per - 1u) / per : 0u;
+      if (lane < a.batch && n == 0u) n = 1u;
+      return of(wave_incl_scan(n), kWave - 1u);
+    };
+    uint32_t lo = total / a.split + 1u, hi = lo;
+    if (a.split >= 2u * a.batch) {
+      hi = total / (a.split - a.batch) + 1u;
+      --lo;
+    }
+    if (lo < kGenChunkPages) lo = kGenChunkPages;
+    while (lo < hi) {  // (uniform)
+      const uint32_t mid = (lo + hi) / 2u;
+      if (chunks(mid) <= a.split) hi = mid;
+      else lo = mid + 1u;
+    }
+    chunks(lo);
+    const uint32_t upto = wave_incl_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(item < upto);
+    if (past == 0u) return Place{0u, ~0u, lo, 0u, 0, 0u};
+    const uint32_t j = (uint32_t)__builtin_ctzll(past);
+    return Place{j, item - (of(upto, j) - of(n, j)), lo, of(beg, j), (int32_t)of((uint32_t)held, j),
+                 of(last, j)};
+  }
+  // more: sequence b's items begin at floor(pages before it / per) + b, room for its chunks
+  // (and one where it has no page) whatever the lengths; 64 sequences are tried at a time
   const uint32_t first = (uint32_t)a.kv_indptr[0];
   const uint32_t total = (uint32_t)a.kv_indptr[a.batch] - first;
-  uint32_t per = total != 0u ? div_up(total, a.split_rcp) : 1u;
+  uint32_t per = total / a.split + 1u, lo = 0u, n = a.batch;
   if (per < kGenChunkPages) per = kGenChunkPages;
-  if (a.batch == 1u) return Place{0u, item, per};
-  const uint32_t lane = __lane_id();
-  uint32_t lo = 0u, n = a.batch;
-  for (;;) {  // 64 sequences are tried at a time
+  for (;;) {
     const uint32_t stride = (n + kWave - 1u) / kWave;
     const bool in = lane * stride < n;
     const uint32_t i = lo + (in ? lane * stride : 0u);
     const uint32_t off = ((uint32_t)a.kv_indptr[i] - first) / per + i;
     const uint64_t le = __builtin_amdgcn_ballot_w64(in && off <= item);
-    if (le == 0u) return Place{0u, ~0u, per};  // malformed page table
+    if (le == 0u) return Place{0u, ~0u, per, 0u, 0, 0u};  // malformed page table
     const uint32_t j = 63u - (uint32_t)__builtin_clzll(le);
     lo += j * stride;
     if (stride == 1u)
-      return Place{(uint32_t)__builtin_amdgcn_readfirstlane((int)lo),
-                   item - (uint32_t)__builtin_amdgcn_readlane((int)off, (int)j), per};
+      return place_of(a, (uint32_t)__builtin_amdgcn_readfirstlane((int)lo), item - of(off, j), per);
     const uint32_t left = n - j * stride;
     n = left < stride ? left : stride;
   }
 }
 
+constexpr uint32_t kJoin = 8u;  // parts whose loads go out together
+
+// two floats of a part (agent-coherent, as st_agent and ld_agent)
+__device__ inline void st_pair(float* p, const float2& x) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, x),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float2 ld_pair(const float* p) {
+  return __builtin_bit_cast(
+      float2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(p)),
+                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 // Codes of a lane: 16 of K per load, D / 16 of V.
 template <int D>
 struct DeShape {
-  static constexpr int kUnits = D == 256 ? 2 : 4;  // of 16 tokens per batch
+  static constexpr int kUnits = D == 256 ? 1 : 2;  // of 16 tokens per batch
   static constexpr int kKL = D / 64;               // 16-byte loads of K per unit
   static constexpr int kVW = D / 64;               // 32-bit words of V per token
   static constexpr int kFr = D / 16;               // fragments of V
@@ -97,10 +149,13 @@ __device__ inline float k_scale(uint32_t w) { return exp_scale((int)(int8_t)w); 
 __device__ inline float v_scale(uint32_t w) { return exp_scale((int)(int8_t)(w >> 8)); }
 __device__ inline uint32_t tokens(uint32_t w) { return w >> 16; }
 
-// S16: pages are of 16 or 32 tokens, so that 16 tokens lie in one.
-template <int D, bool S16>
+// RUN: tokens that lie in one page, from a multiple of RUN on: 16 (pages of 16 or 32), 4
+// (of a multiple of 4) or 1.
+template <int D, int RUN>
 __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args a) {
   using Sh = DeShape<D>;
+  constexpr bool S16 = RUN == 16;
+  constexpr int kVP = RUN == 1 ? 4 : 1;  // pages of a lane's four tokens
   constexpr int kU = Sh::kUnits;
   constexpr uint32_t kBatch = 16u * kU;
   constexpr uint32_t kStride = (uint32_t)D + 4u;  // partial: o[D], m, l, pad
@@ -120,13 +175,19 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
     at = find_chunk(a, blockIdx.y + gridDim.y * blockIdx.z);
   } else {
     hkv = blockIdx.y;
-    at = Place{blockIdx.z, blockIdx.x, kGenChunkPages};
+    at = place_of(a, blockIdx.z, blockIdx.x, a.split);
   }
-  const uint32_t b = at.b, per = at.per;
-  const uint32_t pbeg = (uint32_t)a.kv_indptr[b];
-  const int32_t held = a.kv_indptr[b + 1u] - (int32_t)pbeg;
+  // (of a selection the ids are fetched beside the page table)
+  const int32_t* const row =
+      a.sel != nullptr ? a.sel + ((size_t)at.b * a.Hkv + hkv) * a.sel_stride : nullptr;
+  uint32_t early = 0u;
+  if (row != nullptr && threadIdx.x < at.per && at.chunk * at.per + threadIdx.x < a.sel_stride)
+    early = (uint32_t)row[at.chunk * at.per + threadIdx.x];
+  if (at.chunk == ~0u) return;  // (uniform)
+  const uint32_t b = at.b, per = at.per, pbeg = at.beg;
+  const int32_t held = at.held;
   uint32_t P = held > 0 ? (uint32_t)held : 0u;
-  const uint32_t last = (uint32_t)a.kv_last_page_len[b];  // tokens of the table's last page
+  const uint32_t last = at.last;  // tokens of the table's last page
   if (last == 0u || last > S) P = 0u;  // malformed page table
   uint32_t L = P != 0u ? (P - 1u) * S + last : 0u;
   if (P > a.max_pages) {
@@ -144,8 +205,8 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
   if (a.sel != nullptr) {
     const uint32_t budget = a.token_budgets ? (uint32_t)a.token_budgets[b] : a.token_budget;
     npages = num_selected_pages(L, budget, S, P, quest ? kFlagQuestKernel : 0u);
-    const uint32_t row = a.sel_stride + (quest ? 1u : 0u);
-    if (npages > row) npages = row;
+    const uint32_t most = a.sel_stride + (quest ? 1u : 0u);
+    if (npages > most) npages = most;
   }
   if (npages > a.max_chunks * kGenChunkPages) {  // the workspace's chunks
     npages = a.max_chunks * kGenChunkPages;
@@ -153,8 +214,7 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
   }
   if ((uint64_t)at.chunk * per >= npages) return;  // uniform
   const uint32_t nsel = quest ? npages - 1u : npages;
-  const int32_t* list = a.sel != nullptr ? a.sel + ((size_t)b * a.Hkv + hkv) * a.sel_stride
-                                         : a.kv_indices + pbeg;
+  const int32_t* list = row != nullptr ? row : a.kv_indices + pbeg;
   const uint32_t last_page = (uint32_t)a.kv_indices[pbeg + (uint32_t)held - 1u];
 
   // q of head `col` of the group, the dims of K's loads
@@ -175,79 +235,91 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
   const size_t head = (size_t)hkv * a.g.head;
   for (uint32_t ib = i0; ib < i1; ib += kDeList) {
     const uint32_t np = i1 - ib < kDeList ? i1 - ib : kDeList;
-    __syncthreads();  // the ids before were read
+    if (ib != i0) __syncthreads();  // the ids before were read
     for (uint32_t i = threadIdx.x; i < np; i += kDeThreads) {
-      const uint32_t page = ib + i < nsel ? (uint32_t)list[ib + i] : last_page;
-      const int8_t* e = a.kv_exp + (size_t)page * 2u * a.Hkv + hkv;
-      s_page[i] = page;
-      s_word[i] = (uint32_t)(uint8_t)e[0] | (uint32_t)(uint8_t)e[a.Hkv] << 8 |
-                  (page == last_page ? last : S) << 16;
+      const bool fetched = row != nullptr && ib == i0 && i == threadIdx.x && i < per;
+      s_page[i] = ib + i >= nsel ? last_page : fetched ? early : (uint32_t)list[ib + i];
     }
     __syncthreads();
     const uint32_t T = np * S, nb = (T + kBatch - 1u) / kBatch;  // token slots, batches
-    // slot t of the list: entry and slot in its page (a slot past the end: the last)
-    auto entry = [&](uint32_t t) {
-      return a.page_rcp != 0u ? (uint32_t)(((uint64_t)t * a.page_rcp) >> 32) : t;
+    // slot t of the list (past the end: one of the last): entry and slot in its page
+    auto entry = [&](uint32_t t, uint32_t& slot) {
+      const uint32_t e = a.page_rcp != 0u ? (uint32_t)(((uint64_t)t * a.page_rcp) >> 32) : t;
+      slot = t - e * S;
+      return e;
     };
-    for (uint32_t i = wave; i < nb; i += kDeWaves) {
-      u32x4 kr[kU][Sh::kKL];
-      uint32_t vr[kU][4][Sh::kVW], kw[kU], vw[kU][S16 ? 1 : 4];
-      bool whole = true;  // every slot of the batch holds a token
-      const uint32_t t0 = i * kBatch;
+    auto unit = [&](uint32_t t) { return t < T ? t : T - 16u; };   // (S16)
+    auto token = [&](uint32_t t) { return t < T ? t : T - 1u; };
+    // batches in registers: one computed, one on its way
+    u32x4 kr[2][kU][Sh::kKL];
+    uint32_t vr[2][kU][4][Sh::kVW];
+    auto load = [&](uint32_t i, int s) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
+        const uint32_t t0 = i * kBatch + 16u * u;
         auto load_k = [&](uint32_t page, uint32_t slot) {
           const uint8_t* p = a.kv + (size_t)page * a.g.page + head + slot * a.g.tok + 16u * quarter;
 #pragma unroll
           for (int j = 0; j < Sh::kKL; ++j)
-            kr[u][j] = *reinterpret_cast<const u32x4*>(p + 64 * j);
+            kr[s][u][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * j));
         };
         auto load_v = [&](int r, uint32_t page, uint32_t slot) {
+          typedef uint32_t words __attribute__((ext_vector_type(Sh::kVW)));
           const uint8_t* p = a.kv + (size_t)page * a.g.page + a.g.kv + head + slot * a.g.tok +
                              (D / 16) * col;
+          const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
 #pragma unroll
-          for (int w = 0; w < Sh::kVW; ++w) vr[u][r][w] = reinterpret_cast<const uint32_t*>(p)[w];
+          for (int w = 0; w < Sh::kVW; ++w) vr[s][u][r][w] = x[w];
         };
+        uint32_t slot;
         if constexpr (S16) {
-          const uint32_t t = t0 + 16u * u < T ? t0 + 16u * u : T - 16u;
-          const uint32_t e = entry(t), slot = t - e * S;
+          const uint32_t e = entry(unit(t0), slot);
           const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_page[e]);
-          kw[u] = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_word[e]);
-          if (t0 + 16u * u >= T) kw[u] &= 0xFFFFu;  // (no token)
-          whole &= slot + 16u <= tokens(kw[u]);
           load_k(page, slot + col);
 #pragma unroll
           for (int r = 0; r < 4; ++r) load_v(r, page, slot + 4u * quarter + r);
         } else {
-          auto place = [&](uint32_t t, uint32_t& e, uint32_t& slot, uint32_t& word) {
-            const uint32_t c = t < T ? t : T - 1u;
-            e = entry(c);
-            slot = c - e * S;
-            word = s_word[e];
-            if (t >= T || slot >= tokens(word)) word &= 0xFFFFu;  // (no token)
-          };
-          uint32_t e, slot;
-          place(t0 + 16u * u + col, e, slot, kw[u]);
-          load_k(s_page[e], slot);
+          uint32_t e = entry(token(t0 + col), slot), page = s_page[e];
+          load_k(page, slot);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            place(t0 + 16u * u + 4u * quarter + r, e, slot, vw[u][r]);
-            whole &= tokens(vw[u][r]) != 0u;
-            load_v(r, s_page[e], slot);
+            if (r < kVP) {
+              // (T is a multiple of 4 where RUN is)
+              const uint32_t t = t0 + 4u * quarter + r;
+              e = entry(t < T ? t : T - RUN, slot);
+              page = s_page[e];
+            }
+            load_v(r, page, slot + (kVP == 1 ? r : 0u));
           }
         }
       }
-      whole = __builtin_amdgcn_ballot_w64(!whole) == 0u;
-      // whether slot 4 quarter + r of unit u holds a token
-      auto there = [&](int u, int r) {
+    };
+    auto attend = [&](uint32_t i, int b2) {
+      // the words of K's token, and of the four tokens of the lane's scores and V
+      uint32_t kw[kU], vw[kU][kVP];
+      bool there[kU][4], whole = true;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const uint32_t t0 = i * kBatch + 16u * u;
+        uint32_t slot;
         if constexpr (S16) {
-          const uint32_t t = t0 + 16u * u < T ? t0 + 16u * u : T - 16u;
-          return t - entry(t) * S + 4u * quarter + r < tokens(kw[u]);
+          const uint32_t e = entry(unit(t0), slot);
+          kw[u] = vw[u][0] = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_word[e]);
+          const uint32_t n = t0 < T ? tokens(kw[u]) : 0u;
+          whole &= slot + 16u <= n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) there[u][r] = slot + 4u * quarter + r < n;
         } else {
-          return tokens(vw[u][r]) != 0u;
+          kw[u] = s_word[entry(token(t0 + col), slot)];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t t = t0 + 4u * quarter + r;
+            if (r < kVP) vw[u][r % kVP] = s_word[entry(t < T ? t : T - RUN, slot)];
+            there[u][r] = t < T && slot + (kVP == 1 ? r : 0u) < tokens(vw[u][r % kVP]);
+            whole &= there[u][r];
+          }
         }
-      };
-
+      }
       floatx4 s[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
@@ -255,7 +327,7 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
         s[u] = floatx4{};
 #pragma unroll
         for (int j = 0; j < Sh::kKL; ++j) {
-          const u32x4 x = kr[u][j];
+          const u32x4 x = kr[b2][u][j];
           s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               __builtin_bit_cast(half8, decode8(uint2{x[0], x[1]}, f)), q[2 * j], s[u], 0, 0, 0);
           s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
@@ -263,15 +335,15 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
               0);
         }
       }
-      if (!whole) {
+      if (__builtin_amdgcn_ballot_w64(!whole) != 0u) {
 #pragma unroll
         for (int u = 0; u < kU; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (!there(u, r)) {
+            if (!there[u][r]) {
               s[u][r] = -INFINITY;
 #pragma unroll
-              for (int w = 0; w < Sh::kVW; ++w) vr[u][r][w] = 0u;  // (0 * NaN is NaN)
+              for (int w = 0; w < Sh::kVW; ++w) vr[b2][u][r][w] = 0u;  // (0 * NaN is NaN)
             }
       }
       float top = s[0][0];
@@ -305,7 +377,7 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
           half2v x[4][2];
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            decode4(vr[u][r][w], v_scale(S16 ? kw[u] : vw[u][S16 ? 0 : r]), x[r]);
+            decode4(vr[b2][u][r][w], v_scale(vw[u][r % kVP]), x[r]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const half4 f = {x[0][e / 2][e % 2], x[1][e / 2][e % 2], x[2][e / 2][e % 2],
@@ -314,6 +386,23 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
           }
         }
       }
+    };
+    uint32_t i = wave;
+    if (i < nb) load(i, 0);
+    // (beside the first loads; they are needed no earlier)
+    for (uint32_t j = threadIdx.x; j < np; j += kDeThreads) {
+      const uint32_t page = s_page[j];
+      const int8_t* e = a.kv_exp + (size_t)page * 2u * a.Hkv + hkv;
+      s_word[j] = (uint32_t)(uint8_t)e[0] | (uint32_t)(uint8_t)e[a.Hkv] << 8 |
+                  (page == last_page ? last : S) << 16;
+    }
+    __syncthreads();
+    for (; i < nb; i += 2u * kDeWaves) {
+      if (i + kDeWaves < nb) load(i + kDeWaves, 1);
+      attend(i, 0);
+      if (i + kDeWaves >= nb) break;
+      if (i + 2u * kDeWaves < nb) load(i + 2u * kDeWaves, 0);
+      attend(i + kDeWaves, 1);
     }
   }
   const uint32_t nch = (npages + per - 1u) / per;
@@ -333,71 +422,108 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
     }
   }
   __syncthreads();
-  for (uint32_t x = threadIdx.x; x < G * D; x += kDeThreads) {
+  float* const parts = a.partial + bh0 * a.max_chunks * kStride;  // [G][max_chunks][kStride]
+  auto part = [&](uint32_t g, uint32_t c) { return parts + ((size_t)g * a.max_chunks + c) * kStride; };
+  for (uint32_t x = 2u * threadIdx.x; x < G * D; x += 2u * kDeThreads) {  // (two dims a thread)
     const uint32_t g = x / D, d = x % D;
     float M = s_ml[0][g][0];
 #pragma unroll
     for (uint32_t w = 1; w < kDeWaves; ++w) M = fmaxf(M, s_ml[w][g][0]);
-    float acc = 0.f, sum = 0.f;
+    float2 acc = {0.f, 0.f};
+    float sum = 0.f;
 #pragma unroll
     for (uint32_t w = 0; w < kDeWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(s_ml[w][g][0] - M);
-      acc += f * s_o[w][g][d];
+      acc.x += f * s_o[w][g][d];
+      acc.y += f * s_o[w][g][d + 1u];
       sum += f * s_ml[w][g][1];
     }
     if (nch == 1u) {
-      a.o[(bh0 + g) * D + d] = r16(acc / sum);
+      *reinterpret_cast<half2v*>(a.o + (bh0 + g) * D + d) = half2v{r16(acc.x / sum), r16(acc.y / sum)};
     } else {
-      float* part = a.partial + ((bh0 + g) * a.max_chunks + at.chunk) * kStride;
-      st_agent(part + d, acc);
-      if (d == 0u) {
-        st_agent(part + D, M);
-        st_agent(part + D + 1u, sum);
-      }
+      st_pair(part(g, at.chunk) + d, acc);
+      if (d == 0u) st_pair(part(g, at.chunk) + D, float2{M, sum});
     }
   }
   if (nch == 1u) return;
-  if (!arrive_last(&a.counters[bh0 * kCounterStride], nch, &s_last)) return;
-  // the last chunk to arrive joins them: the loads of 8 or 16 chunks together, in order
-  auto join = [&](auto group) {
-    constexpr uint32_t kC = decltype(group)::value;
-    for (uint32_t x = threadIdx.x; x < G * D; x += kDeThreads) {
-      const uint32_t g = x / D, d = x % D;
-      const float* base = a.partial + (bh0 + g) * a.max_chunks * kStride;
-      float M = kPfNoMax, sum = 0.f, acc = 0.f;
-      for (uint32_t c0 = 0; c0 < nch; c0 += kC) {
-        float mc[kC], lc[kC], oc[kC];
+
+  // ---- the chunks: joined by the last of each kJoin to arrive, and these by the last of all
+  // (one workgroup for all chunks of a kv head took 50 of 60 us at 32768 tokens of 4 kv
+  // heads with 8 query heads each)
+  uint32_t* const counters = &a.counters[bh0 * kCounterStride];  // of all, then of each set
+  uint32_t each = G <= 2u ? 2u * kJoin : kJoin;
+  if (nch > each * (kCounterStride - 1u)) each = (nch + kCounterStride - 2u) / (kCounterStride - 1u);
+  const uint32_t sets = (nch + each - 1u) / each, set = at.chunk / each;
+  // joins n parts from chunk c0 on, `step` chunks apart: to the output, or to the first's place
+  auto join = [&](uint32_t c0, uint32_t n, uint32_t step, bool out) {
+    constexpr uint32_t kMost = 8 * D / (2 * kDeThreads) > 0 ? 8 * D / (2 * kDeThreads) : 1;
+    float2 acc[kMost], ml[kMost];
 #pragma unroll
-        for (uint32_t u = 0; u < kC; ++u) {
-          const float* part = base + (size_t)(c0 + u < nch ? c0 + u : nch - 1u) * kStride;
-          mc[u] = ld_agent(part + D);
-          lc[u] = ld_agent(part + D + 1u);
-          oc[u] = ld_agent(part + d);
+    for (uint32_t y = 0; y < kMost; ++y) {
+      const uint32_t x = 2u * (threadIdx.x + y * kDeThreads), g = x / D, d = x % D;
+      if (x >= G * D) break;
+      float2 s = {0.f, 0.f};
+      float M = kPfNoMax, sum = 0.f;
+      for (uint32_t i0 = 0; i0 < n; i0 += kJoin) {
+        float2 pm[kJoin], po[kJoin];
+#pragma unroll
+        for (uint32_t u = 0; u < kJoin; ++u) {
+          const float* p = part(g, c0 + (i0 + u < n ? i0 + u : n - 1u) * step);
+          pm[u] = ld_pair(p + D);
+          po[u] = ld_pair(p + d);
         }
         float next = M;
 #pragma unroll
-        for (uint32_t u = 0; u < kC; ++u) next = fmaxf(next, mc[u]);
+        for (uint32_t u = 0; u < kJoin; ++u) next = fmaxf(next, pm[u].x);
         const float keep = __builtin_amdgcn_exp2f(M - next);
         sum *= keep;
-        acc *= keep;
+        s.x *= keep;
+        s.y *= keep;
 #pragma unroll
-        for (uint32_t u = 0; u < kC; ++u) {
-          const float f = c0 + u < nch ? __builtin_amdgcn_exp2f(mc[u] - next) : 0.f;
-          sum += f * lc[u];
-          acc += f * oc[u];
+        for (uint32_t u = 0; u < kJoin; ++u) {
+          const float f = i0 + u < n ? __builtin_amdgcn_exp2f(pm[u].x - next) : 0.f;
+          sum += f * pm[u].y;
+          s.x += f * po[u].x;
+          s.y += f * po[u].y;
         }
         M = next;
       }
-      a.o[(bh0 + g) * D + d] = r16(acc / sum);
+      acc[y] = s;
+      ml[y] = float2{M, sum};
+    }
+    __syncthreads();  // every thread has read the parts
+#pragma unroll
+    for (uint32_t y = 0; y < kMost; ++y) {
+      const uint32_t x = 2u * (threadIdx.x + y * kDeThreads), g = x / D, d = x % D;
+      if (x >= G * D) break;
+      if (out) {
+        *reinterpret_cast<half2v*>(a.o + (bh0 + g) * D + d) =
+            half2v{r16(acc[y].x / ml[y].y), r16(acc[y].y / ml[y].y)};
+      } else {
+        st_pair(part(g, c0) + d, acc[y]);
+        if (d == 0u) st_pair(part(g, c0) + D, ml[y]);
+      }
     }
   };
-  if (nch <= 8u) join(std::integral_constant<uint32_t, 8u>{});
-  else join(std::integral_constant<uint32_t, 16u>{});
-  __syncthreads();  // every thread has read the partials
-  for (uint32_t g = 0; g < G; ++g) {  // (a workspace is left zeroed)
-    uint32_t* w = reinterpret_cast<uint32_t*>(a.partial + (bh0 + g) * a.max_chunks * kStride);
-    for (uint32_t i = threadIdx.x; i < nch * kStride; i += kDeThreads) st_agent_u32(w + i, 0u);
+  // a workspace is left zeroed (after the arrival, which would wait for these stores)
+  auto clear = [&](uint32_t c0, uint32_t n, uint32_t step) {
+    for (uint32_t i = wave; i < G * n; i += kDeWaves)
+      for (uint32_t j = 2u * lane; j < kStride; j += 2u * kWave)
+        st_pair(part(i / n, c0 + i % n * step) + j, float2{0.f, 0.f});
+  };
+  const uint32_t c0 = set * each, in_set = nch - c0 < each ? nch - c0 : each;
+  if (in_set > 1u && !arrive_last(&counters[1u + set], in_set, &s_last)) return;
+  if (sets == 1u) {
+    join(c0, in_set, 1u, true);
+    clear(c0, in_set, 1u);
+    return;
   }
+  if (in_set > 1u) join(c0, in_set, 1u, false);
+  const bool last_set = arrive_last(&counters[0], sets, &s_last);
+  if (in_set > 1u) clear(c0 + 1u, in_set - 1u, 1u);
+  if (!last_set) return;
+  join(0u, sets, each, true);
+  clear(0u, sets, each);
 }
 
 constexpr uint32_t kDeWorkgroups = 512;  // 2 per CU
@@ -409,20 +535,28 @@ hipError_t launch_decode_fp8(const DecodeFp8Args& args, uint32_t head_dim, hipSt
   auto rcp = [](uint32_t d) { return d > 1u ? (uint32_t)((1ull << 32) / d) + 1u : 0u; };
   a.page_rcp = rcp(a.S);
   a.split = kDeWorkgroups / a.Hkv > 1u ? kDeWorkgroups / a.Hkv : 1u;
-  a.split_rcp = rcp(a.split);
-  dim3 grid(a.max_chunks, a.Hkv, a.batch);
+  if (a.sel != nullptr) {  // pages per chunk
+    const uint64_t pages = (uint64_t)a.max_chunks * kGenChunkPages * a.Hkv * a.batch;
+    a.split = (uint32_t)((pages + kDeWorkgroups - 1u) / kDeWorkgroups);
+    if (a.split < kGenChunkPages) a.split = kGenChunkPages;
+    const uint32_t most = a.max_chunks * kGenChunkPages;
+    if (a.split > most) a.split = most;
+  }
+  dim3 grid((a.max_chunks * kGenChunkPages + a.split - 1u) / a.split, a.Hkv, a.batch);
   if (a.sel == nullptr) {
     const uint64_t most = (uint64_t)a.max_chunks * a.batch;
-    const uint32_t items =
-        a.batch > 1u ? a.split + a.batch : a.split < most ? a.split : (uint32_t)most;
+    const uint32_t room = a.batch <= (uint32_t)kWave && a.split >= 2u * a.batch
+                              ? a.split
+                              : a.split + a.batch;
+    const uint32_t items = room < most ? room : (uint32_t)most;
     constexpr uint32_t kRows = 32768u;
     grid = dim3(a.Hkv, items < kRows ? items : kRows, (items + kRows - 1u) / kRows);
   }
   const dim3 block(kDeThreads);
-  const bool whole = a.S % 16u == 0u;
-#define AOAKV_DE(D_)                                                                        \
-  if (whole) hipLaunchKernelGGL((decode_fp8_kernel<D_, true>), grid, block, 0, s, a);       \
-  else hipLaunchKernelGGL((decode_fp8_kernel<D_, false>), grid, block, 0, s, a)
+#define AOAKV_DE(D_)                                                                              \
+  if (a.S % 16u == 0u) hipLaunchKernelGGL((decode_fp8_kernel<D_, 16>), grid, block, 0, s, a);     \
+  else if (a.S % 4u == 0u) hipLaunchKernelGGL((decode_fp8_kernel<D_, 4>), grid, block, 0, s, a);  \
+  else hipLaunchKernelGGL((decode_fp8_kernel<D_, 1>), grid, block, 0, s, a)
   switch (head_dim) {
     case 64: AOAKV_DE(64); break;
     case 128: AOAKV_DE(128); break;

@@ -375,8 +375,9 @@ struct DecodeFp8Args {
   float scale;         // log2(e) / sqrt(D)
   PageGeom g;
   uint32_t* error;
-  // set by the launch
-  uint32_t page_rcp, split, split_rcp;
+  // set by the launch: the factor that divides by S (0: S = 1); the chunks that every page
+  // is cut into per kv head, or of a selection the pages per chunk
+  uint32_t page_rcp, split;
 };
 hipError_t launch_decode_fp8(const DecodeFp8Args& a, uint32_t head_dim, hipStream_t s);
 
