@@ -1343,8 +1343,8 @@ int aoakv_decode_sparse_attn_fp8(const void* q, void* o, const void* kv_data,
   const uint32_t max_sel = max_selected(sel_pages, sel_stride, token_budget, token_budgets,
                                         max_pages, page_size, flags);
   const uint64_t chunks = aoakv::decode_chunks(max_sel);
-  // (a dispatch's work-items are counted in 32 bits: 2^24 workgroups of 256)
-  REQUIRE((sel_pages ? chunks * batch_size : batch_size + 513ull) * num_kv_heads < (1ull << 24),
+  // (a dispatch's work-items are counted in 32 bits: 2^23 workgroups of 512)
+  REQUIRE((sel_pages ? chunks * batch_size : batch_size + 513ull) * num_kv_heads < (1ull << 23),
           "%s: batch_size %u too large", fn, batch_size);
   Workspace w{};
   const size_t need =

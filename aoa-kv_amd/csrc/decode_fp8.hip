@@ -25,7 +25,7 @@ namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kDeThreads = 256, kDeWaves = kDeThreads / kWave;
+constexpr uint32_t kDeThreads = 512, kDeWaves = kDeThreads / kWave;
 constexpr uint32_t kDeList = 512;  // pages whose ids are staged at a time
 // Probabilities of the second product are held 2^7 times as large, and the running
 // maximum moves where one would pass 2^8 (chunk_attn.hpp)
@@ -57,7 +57,7 @@ __device__ inline Place place_of(const DecodeFp8Args& a, uint32_t b, uint32_t ch
 // The item-th of a call over every page.  The pages of all sequences are cut into chunks of
 // as few pages (at least kGenChunkPages) as leaves a.split of them per kv head, so that all
 // are at work at once and end together.  (Cut into chunks of a.split-ths, 16 sequences made
-// some more than the GPU holds at once: 76 us, now XX.)  A sequence without a page has one.
+// some more than the GPU holds at once, 78 us and then 65.)  A sequence without a page has one.
 __device__ inline Place find_chunk(const DecodeFp8Args& a, uint32_t item) {
   const uint32_t lane = __lane_id();
   auto of = [](uint32_t x, uint32_t j) {
@@ -526,7 +526,16 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
   clear(0u, sets, each);
 }
 
-constexpr uint32_t kDeWorkgroups = 512;  // 2 per CU
+// One workgroup of 8 waves per CU, each with a batch on its way beside the one it computes
+// (16 KB).  Graphs of calls on three caches in turn, us, two workgroups of 4 waves / one of
+// 8 / two of 8 without a batch ahead: 2048 selected of 32768 tokens, 32 heads 10.2 / 9.3 /
+// 9.3; every page of 16384 29 / 28 / 29; 32768 tokens of 4 kv heads of 8 query heads 25 / 18
+// / 22; head dim 256 23 / 19 / 43; 16 sequences of 2000 to 16000 64 / 68 / 65.  Twice the
+// workgroups: 28 -> 33 and 18 -> 28.
+constexpr uint32_t kDeWorkgroups = 256;
+// Pages per chunk of a selection at least (of every page 8): with a call's two joins 16 are
+// 8.5 us at 2048 tokens of 8 kv heads, 8 9.9; of 1000 tokens on every page 8.5, and 8.1.
+constexpr uint32_t kDeListed = 16u;
 
 }  // namespace
 
@@ -538,9 +547,7 @@ hipError_t launch_decode_fp8(const DecodeFp8Args& args, uint32_t head_dim, hipSt
   if (a.sel != nullptr) {  // pages per chunk
     const uint64_t pages = (uint64_t)a.max_chunks * kGenChunkPages * a.Hkv * a.batch;
     a.split = (uint32_t)((pages + kDeWorkgroups - 1u) / kDeWorkgroups);
-    if (a.split < kGenChunkPages) a.split = kGenChunkPages;
-    const uint32_t most = a.max_chunks * kGenChunkPages;
-    if (a.split > most) a.split = most;
+    if (a.split < kDeListed) a.split = kDeListed;
   }
   dim3 grid((a.max_chunks * kGenChunkPages + a.split - 1u) / a.split, a.Hkv, a.batch);
   if (a.sel == nullptr) {
