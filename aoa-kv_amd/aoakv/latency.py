@@ -16,7 +16,8 @@ row.  ``--method`` is the older spelling of the same choice.  Both use the
 simulation's selection unless ``--semantics quest_kernel`` asks for the
 reference kernels' convention.  ``--graph`` replays each decode step's
 layers from a HIP graph (``QuestLlamaModel.decode_graphed``): at batch 1 the
-eager step is bound by its per-layer host dispatch.  Weights are random and
+eager step is bound by its per-layer host dispatch.  ``--kv_dtype fp8`` holds the
+cache in 8 bits (method suffix _fp8).  Weights are random and
 seeded (no checkpoint is loaded; latency does not depend on weight values),
 inputs are random
 embeddings as in the reference driver, and timing uses events with a
@@ -69,6 +70,9 @@ def parse_args(argv=None):
     p.add_argument("--graph", action="store_true",
                    help="replay each decode step's layers from a HIP graph (the host planner "
                         "runs eagerly before each replay; CSV method gets a _graph suffix)")
+    p.add_argument("--kv_dtype", choices=["fp16", "fp8"], default="fp16",
+                   help="what the cache holds: fp16 values, or 8-bit codes with a scale per page "
+                        "and kv head (CSV method gets a _fp8 suffix)")
     p.add_argument("--out", default=None, help="CSV to append to (optional)")
     args = p.parse_args(argv)
     if args.kernel and args.method and KERNELS[args.kernel] != args.method:
@@ -109,7 +113,8 @@ def main(argv=None):
     model.quest_init(page_size=args.page_size,
                      max_seq_len=args.context_len + args.decode_len + 512,
                      token_budget=args.token_budget, dtype=dtype, device=device,
-                     value_aware=args.method == "AOA_KV", semantics=args.semantics)
+                     value_aware=args.method == "AOA_KV", semantics=args.semantics,
+                     kv_dtype=torch.float8_e4m3fn if args.kv_dtype == "fp8" else None)
 
     prefill_ms, decode_ms = [], []
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -143,7 +148,7 @@ def main(argv=None):
 
     row = {
         "method": (args.method + ("" if args.semantics == "sim" else "_quest_kernel") +
-                   ("_graph" if args.graph else "")),
+                   ("_fp8" if args.kv_dtype == "fp8" else "") + ("_graph" if args.graph else "")),
         "kernel_md5": md5, "gpu": gpu, "model": args.model, "context_len": args.context_len,
         "token_budget": args.token_budget, "page_size": args.page_size,
         "decode_len": args.decode_len, "iteration": args.iteration,

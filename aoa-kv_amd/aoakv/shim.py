@@ -180,19 +180,22 @@ class QuestLlamaModel(nn.Module):
                    dtype=torch.float16, device="cuda:0", value_aware: bool = True,
                    semantics: str = "sim", layout: int = TensorLayout.HND,
                    evict_keep: Optional[int] = None, evict_sink: int = 4,
-                   evict_recent: int = 32):
+                   evict_recent: int = 32, kv_dtype: Optional[torch.dtype] = None):
         """Allocates the paged caches for max_seq_len tokens (llama.py:520-552).
         evict_keep: after each prompt, every layer's cache is cut down to that
         many tokens per kv head: the first evict_sink, the last evict_recent, and
-        those that the last queries of the prompts attend to most."""
+        those that the last queries of the prompts attend to most.
+        kv_dtype=torch.float8_e4m3fn: caches held in 8 bits (not with evict_keep)."""
         assert self.iController is None, "Can't init Quest Controller twice."
         cfg = self.cfg
+        if evict_keep is not None and kv_dtype == torch.float8_e4m3fn:
+            raise ValueError("evict_keep is for fp16 caches")
         self._page_budget = token_budget // page_size
         self.iController = InferenceController(
             cfg.num_hidden_layers, cfg.num_attention_heads,
             cfg.hidden_size // cfg.num_attention_heads, page_size, self._page_budget,
             max_seq_len, dtype, device, layout=layout, num_kv_heads=cfg.num_key_value_heads,
-            value_aware=value_aware, semantics=semantics)
+            value_aware=value_aware, semantics=semantics, kv_dtype=kv_dtype)
         self._evict = None
         if evict_keep is not None:
             if evict_sink + evict_recent > evict_keep:

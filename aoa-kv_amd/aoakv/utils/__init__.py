@@ -23,6 +23,9 @@ to::
     o, lse = chunk_forward(q, ctrl, layer, return_lse=True)   # N >= 1 new tokens
     observe(q, lse, ctrl, layer)                  # each token's weight is added up
     ctrl.evict(keep, sink, recent)                # between forward passes
+
+or held in 8 bits (``InferenceController(..., kv_dtype=torch.float8_e4m3fn)``): the calls
+above and their order stay, and ``read_kv`` gives cached tokens back as fp16 rows.
 """
 from __future__ import annotations
 
@@ -51,7 +54,20 @@ __all__ = [
     "decode_topk",
     "decode_sparse_attn",
     "decode_layer",
+    "read_kv",
 ]
+
+
+def _coded(c: InferenceController, layer_idx: int):
+    """The cache of a layer held in 8 bits, and the page table."""
+    return (c.kv_cache.buf_layer(layer_idx), c.kv_exp[layer_idx], c.kv_indptr_for_append,
+            c.kv_indices_with_last, c.kv_last_page_len_t)
+
+
+def _statistics(c: InferenceController, layer_idx: int):
+    return dict(metadata_data=c.metadata_cache.buf_layer(layer_idx),
+                metadata_indptr=c.metadata_indptr_for_append, metadata_indices=c.metadata_indices,
+                v_log_norm=c.v_log_norm_layer(layer_idx), v_mean=c.v_mean_layer(layer_idx))
 
 
 def apply_rope_in_place(q: torch.Tensor, k: torch.Tensor, past_kv_len: int,
@@ -78,12 +94,19 @@ def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """apply_rope_in_place(q, k, seqlen - N) then append_kv(k, v) -- the
     reference's two calls at QuestAttention.py:98-111 -- in one launch (a
     prompt at the shapes ops.rope_append_kv_cache_prefill names).  q and k are
-    left rotated, as the reference leaves them.  Call after begin_forward, like
+    left rotated, as the reference leaves them (with an 8-bit cache k is left as it
+    was: it is rotated on its way into the cache).  Call after begin_forward, like
     append_kv.  After an eviction, when a token's position is no longer its slot,
     these are the two calls."""
     c = iController
     scale = 1.0 if rope_scale is None else rope_scale
     theta = 1e4 if rope_theta is None else rope_theta
+    if c.kv_fp8:
+        n = k.size(0)
+        ops.rope_append_kv_cache_fp8(q.view(n, -1, c.head_dim), k, v, c.new_tokens(n),
+                                     *_coded(c, layer_idx), c.layout, scale, theta,
+                                     **_statistics(c, layer_idx))
+        return
     if c.evicted:
         ops.apply_rope_in_place(q.view(k.size(0), -1, c.head_dim), k,
                                 c.kv_cache.seqlen + c.evicted - k.size(0), scale, theta)
@@ -108,6 +131,10 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, iController: InferenceController
     """Append new k/v [N, H, D] to the layer's cache and metadata
     (reference __init__.py:69-131).  N > 1: bulk append; N == 1: decode append."""
     c = iController
+    if c.kv_fp8:
+        ops.append_kv_cache_fp8(k, v, c.new_tokens(k.size(0)), *_coded(c, layer_idx), c.layout,
+                                **_statistics(c, layer_idx))
+        return
     if k.size(0) > 1:
         ops.append_kv_cache_prefill(
             k, v, c.kv_cache.buf_layer(layer_idx), c.kv_indices_with_last,
@@ -129,6 +156,8 @@ def prefill_forward(q: torch.Tensor, iController: InferenceController, layer_idx
     """Causal attention of the new tokens over the cache (reference
     __init__.py:133-175).  RoPE is applied by the caller (rope_* unused)."""
     c = iController
+    if c.kv_fp8:
+        return chunk_forward(q, c, layer_idx)
     return ops.prefill_with_paged_kv_cache(
         q, c.kv_cache.buf_layer(layer_idx), c.kv_indices_with_last, len(c.kv_cache.indicies),
         c.kv_cache.last_page_len, c.layout, causal=True)
@@ -142,6 +171,11 @@ def chunk_forward(q: torch.Tensor, iController: InferenceController, layer_idx: 
     the options of ``ops.chunk_attn``; with ``return_lse`` (o, lse).  Distances
     and windows count cache slots, so after an eviction not positions."""
     c = iController
+    if c.kv_fp8:
+        return ops.chunk_attn_fp8(q, c.new_tokens(q.size(0)), *_coded(c, layer_idx),
+                                  c.decode_max_pages, c.layout, window=window, soft_cap=soft_cap,
+                                  slopes=slopes, prefix_len=prefix_len, return_lse=return_lse,
+                                  workspace=c.workspace)
     c._q_indptr[1].fill_(q.size(0))
     return ops.chunk_attn(q, c._q_indptr, c.kv_cache.buf_layer(layer_idx),
                           c.kv_indptr_for_append, c.kv_indices_with_last, c.kv_last_page_len_t,
@@ -221,6 +255,11 @@ def decode_sparse_attn(q: torch.Tensor, iController: InferenceController, layer_
             sel = torch.zeros((1, c.num_kv_heads, 1), dtype=torch.int32, device=c.device)
     q3 = q.view(1, c.num_heads, c.head_dim)
     o = torch.empty_like(q3)
+    if c.kv_fp8:
+        ops.decode_sparse_attn_fp8(q3, o, *_coded(c, layer_idx), sel, c.token_budget, c.workspace,
+                                   c.decode_max_pages, c.layout,
+                                   flags=c.flags & ops.FLAG_QUEST_KERNEL)
+        return o.view_as(q)
     ops.decode_sparse_attn(
         q3, o, c.kv_cache.buf_layer(layer_idx), c.kv_indptr_for_append, c.kv_indices_with_last,
         c.kv_last_page_len_t, sel, c.token_budget, c.workspace, c.decode_max_pages,
@@ -231,13 +270,26 @@ def decode_sparse_attn(q: torch.Tensor, iController: InferenceController, layer_
 def decode_layer(q: torch.Tensor, iController: InferenceController, layer_idx: int,
                  single_launch: bool = False) -> torch.Tensor:
     """estimate + top-k + sparse decode in two launches (or one, with
-    ``single_launch``).  A one-launch call whose wait gave up leaves NaN
+    ``single_launch``; an 8-bit cache's is two launches either way).  A one-launch
+    call whose wait gave up leaves NaN
     outputs from then on until the workspace is re-initialized;
     ``iController.check_errors()`` reports it (and re-initializes), and with
     ``iController.debug_checks`` it runs after every call."""
     c = iController
     q3 = q.view(1, c.num_heads, c.head_dim)
     o = torch.empty_like(q3)
+    if c.kv_fp8:
+        ops.estimate_topk(
+            q3, c.metadata_cache.buf_layer(layer_idx), c.metadata_indptr_for_append,
+            c.metadata_indices, c.kv_indptr_for_append, c.kv_indices_with_last,
+            c.kv_last_page_len_t, c.v_log_norm_layer(layer_idx), c.scores, c._sel, c.token_budget,
+            c.workspace, c.decode_max_pages, c.layout, c.flags)
+        ops.decode_sparse_attn_fp8(q3, o, *_coded(c, layer_idx), c._sel, c.token_budget,
+                                   c.workspace, c.decode_max_pages, c.layout,
+                                   flags=c.flags & ops.FLAG_QUEST_KERNEL)
+        if c.debug_checks:
+            c.check_errors()
+        return o.view_as(q)
     ops.sparse_decode_layer(
         q3, o, c.kv_cache.buf_layer(layer_idx), c.kv_indptr_for_append, c.kv_indices_with_last,
         c.kv_last_page_len_t, c.metadata_cache.buf_layer(layer_idx),
@@ -247,3 +299,14 @@ def decode_layer(q: torch.Tensor, iController: InferenceController, layer_idx: i
     if c.debug_checks:
         c.check_errors()
     return o.view_as(q)
+
+
+def read_kv(iController: InferenceController, layer_idx: int, last: Optional[int] = None):
+    """The sequence's cached tokens (``last``: its last ones) of a layer held in 8 bits as
+    fp16 rows k, v [n, Hkv, D], to hand them on: keys as they were rotated."""
+    c = iController
+    if not c.kv_fp8:
+        raise RuntimeError("read_kv is for caches held in 8 bits")
+    n = c.kv_cache.seqlen if last is None else max(0, min(last, c.kv_cache.seqlen))
+    c._q_indptr[1].fill_(n)
+    return ops.read_kv_cache_fp8(n, c._q_indptr, *_coded(c, layer_idx), c.layout)

@@ -16,7 +16,12 @@ switch trees.  Differences, by design:
   allocation; ``kv_indices_without_last`` is a broadcast view, not the
   reference's per-head copy (controller.py:130-131);
 * scores are fp32 and the per-page value statistic is written for every
-  page, with the page mean of V kept in ``v_mean`` for the running mean.
+  page, with the page mean of V kept in ``v_mean`` for the running mean;
+* ``kv_dtype=torch.float8_e4m3fn`` holds the cache in 8 bits, half its bytes, with
+  the exponents of its blocks' scales in ``kv_exp`` (aoakv.h): the same call order,
+  with prefill by the chunk attention and a decode layer of two launches.  Page
+  statistics, so the pages that are selected, are those of an fp16 cache.  Eviction is
+  for fp16 caches.
 
 ``semantics="quest_kernel"`` switches to the reference kernel's convention
 instead (controller.py:113-124, quest/utils/__init__.py:196-246): the last
@@ -40,9 +45,13 @@ class InferenceController:
                  dtype, device, layout: int = TensorLayout.HND,
                  num_kv_heads: Optional[int] = None, fixed: bool = True,
                  value_aware: bool = True, shuffle_seed: Optional[int] = None,
-                 semantics: str = "sim"):
+                 semantics: str = "sim", kv_dtype: Optional[torch.dtype] = None):
         if dtype != torch.float16:
             raise TypeError("only float16 caches are supported")
+        if kv_dtype not in (None, torch.float16, torch.float8_e4m3fn):
+            raise TypeError(f"kv_dtype must be torch.float16 or torch.float8_e4m3fn, got {kv_dtype}")
+        self.kv_dtype = kv_dtype or dtype
+        self.kv_fp8 = kv_dtype == torch.float8_e4m3fn
         if semantics not in ("sim", "quest_kernel"):
             raise ValueError(f"semantics must be 'sim' or 'quest_kernel', got {semantics!r}")
         self.semantics = semantics
@@ -60,7 +69,11 @@ class InferenceController:
         max_kv_pages = (max_seq_len + page_size - 1) // page_size
         self.max_kv_pages = max_kv_pages
         self.kv_cache = KvCache(num_layers, self.num_kv_heads, head_dim, max_seq_len, page_size,
-                                dtype, device, layout, shuffle_seed)
+                                self.kv_dtype, device, layout, shuffle_seed)
+        self.kv_exp = None
+        if self.kv_fp8:  # of the blocks of every layer (a view per layer, as the cache's)
+            self.kv_exp = torch.zeros((num_layers, max_kv_pages, 2, self.num_kv_heads),
+                                      dtype=torch.int8, device=device).unbind(0)
         self.metadata_cache = KvCache(num_layers, self.num_kv_heads, head_dim, max_kv_pages,
                                       page_size, dtype, device, layout,
                                       None if shuffle_seed is None else shuffle_seed + 1)
@@ -105,7 +118,9 @@ class InferenceController:
         # rows of a chunk and where its tokens begin (utils.chunk_forward, observe)
         self._q_indptr = torch.zeros(2, **i32)
         self._start = torch.zeros(1, **i32)
-        self._up = {"kv": 0, "md": 0, "P": 0, "Pm": 0, "lpl": 0}
+        # rows of the forward pass's new tokens (8-bit caches)
+        self._new_indptr = torch.zeros(2, **i32)
+        self._up = {"kv": 0, "md": 0, "P": 0, "Pm": 0, "lpl": 0, "new": 0}
 
         # fixed-size decode buffers (one layer at a time)
         self.scores = torch.empty((1, self.num_kv_heads, max_kv_pages), dtype=torch.float32,
@@ -182,6 +197,8 @@ class InferenceController:
                 if up[key] != val:
                     t.fill_(val)
                     up[key] = val
+            if self.kv_fp8 and seq_len > 0:
+                self.new_tokens(seq_len)
             self.kv_indices_with_last = self._kv_ids[:P]
             self.metadata_indices = self._md_ids[:Pm]
             self.kv_indptr_for_append = self._kv_indptr
@@ -199,6 +216,14 @@ class InferenceController:
 
     def end_forward(self):
         pass
+
+    def new_tokens(self, n: int) -> torch.Tensor:
+        """The device's [0, n], the rows of n new tokens (begin_forward writes it, so that
+        the layers launch nothing for it)."""
+        if self._up["new"] != n:
+            self._new_indptr[1].fill_(n)
+            self._up["new"] = n
+        return self._new_indptr
 
     @property
     def kv_indices_without_last(self) -> Optional[torch.Tensor]:
@@ -256,6 +281,8 @@ class InferenceController:
     def track_weights(self):
         """Allocate the sums of attention weight per layer, page, kv head and
         slot (fp32), which utils.observe adds to and evict goes by."""
+        if self.kv_fp8:
+            raise RuntimeError("eviction is for fp16 caches")
         if self._attn_weights is None:
             self._attn_weights = torch.zeros(
                 (self.num_layers, self.max_kv_pages, self.num_kv_heads, self.page_size),
