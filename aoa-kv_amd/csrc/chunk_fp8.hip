@@ -1,5 +1,18 @@
 // Attention of a ragged batch of chunks over a paged cache of 8-bit codes (gfx950):
 // chunk_attn.hpp with fragments made from codes.
+//
+//   o = softmax(mod(q k^T / sqrt(D)) + mask) v,  k = code * 2^exp,  v likewise (fp8.hpp)
+//
+// Tiles of K and V are codes in LDS too: half the bytes on every way but the last, where
+// one instruction makes two fp16 values of two codes and the power of two of their block,
+// exactly.  K's lanes read 16 codes of a row, two fragments; V's go through the transposing
+// read of 8-bit elements.  The four waves of a workgroup turn the same codes each for
+// itself, 128 instructions per wave and tile at head dim 128 beside 32 matrix instructions:
+// a prompt of 8192 tokens of 32 heads takes 616 to 632 us (890 TFLOP/s), 572 over fp16.
+// 5 drafted tokens of 8 sequences over up to 16384, 8 kv heads (165 MB), take 53 us: of a
+// workgroup's four waves one has rows, and its chain per tile bounds.  Tiles dealt to the
+// four waves took as long (a buffer per wave: it waits out its own loads), four buffers
+// filled three tiles ahead 55, and the prompt then 655.
 #include "chunk_attn.hpp"
 
 namespace aoakv {
