@@ -557,11 +557,14 @@ hipError_t launch_decode_fp8(const DecodeFp8Args& args, uint32_t head_dim, hipSt
   }
   dim3 grid((a.max_chunks * kGenChunkPages + a.split - 1u) / a.split, a.Hkv, a.batch);
   if (a.sel == nullptr) {
+    // (up to 64 sequences the items are counted, so no more than all chunks; else a sequence's
+    // begin behind room for those before it)
     const uint64_t most = (uint64_t)a.max_chunks * a.batch;
-    const uint32_t room = a.batch <= (uint32_t)kWave && a.split >= 2u * a.batch
-                              ? a.split
-                              : a.split + a.batch;
-    const uint32_t items = room < most ? room : (uint32_t)most;
+    uint32_t items = a.split + a.batch;
+    if (a.batch <= (uint32_t)kWave) {
+      if (a.split >= 2u * a.batch) items = a.split;
+      if (items > most) items = (uint32_t)most;
+    }
     constexpr uint32_t kRows = 32768u;
     grid = dim3(a.Hkv, items < kRows ? items : kRows, (items + kRows - 1u) / kRows);
   }

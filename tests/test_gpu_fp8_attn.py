@@ -258,6 +258,16 @@ def test_decode_many():
     assert not decode(Coded([0], [1], 64, 16, 2, 2, seed=5))[0].any()
 
 
+@pytest.mark.parametrize("n,L", [(65, 128), (100, 16), (200, 256), (64, 128)])
+def test_decode_many_short(n, L):
+    """Tables of a page or a few: the bound on their pages allows for no more chunks than
+    sequences, and each has its own all the same."""
+    _say(f"[decode fp8] {n} sequences of {L} tokens")
+    r = Coded([L] * n, [1] * n, 64, 16, 2, 2, seed=6)
+    ref, tol = expected(r, every(r))
+    within(decode(r, max_pages=L // 16)[0], ref, tol)
+
+
 @pytest.mark.parametrize("S,L", [(16, 70000), (1, 9000), (32, 40000)])
 def test_decode_long(S, L):
     """Chunks of more pages than are staged at a time."""
