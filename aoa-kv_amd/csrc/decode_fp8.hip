@@ -362,7 +362,9 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
       const float next = up ? top : m;
       const float neg = __builtin_fmaf(-next, a.scale, kDeLift);
       if (__builtin_amdgcn_ballot_w64(up) != 0u) {
-        const float keep = __builtin_amdgcn_exp2f((m - next) * a.scale);
+        // (between the offsets as exponentials have them: rounded apart from them, scores of
+        // 2^18 scaled units weighed what was summed before 2^-5 wrong)
+        const float keep = __builtin_amdgcn_exp2f(neg - __builtin_fmaf(-m, a.scale, kDeLift));
         l *= keep;
 #pragma unroll
         for (int t = 0; t < Sh::kFr; ++t) o[t] *= keep;
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
         *reinterpret_cast<float4*>(&s_o[wave][col][(D / 16) * (4 * quarter + r) + t]) =
             float4{o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
     if (quarter == 0u) {
-      s_ml[wave][col][0] = m * a.scale;
+      s_ml[wave][col][0] = -__builtin_fmaf(-m, a.scale, kDeLift);  // (the offset itself)
       s_ml[wave][col][1] = l;
     }
   }
