@@ -399,7 +399,7 @@ __device__ inline void store_row(const ChunkArgs& a, const Seq& s, const Row& r,
       *reinterpret_cast<half4*>(o + t * 32 + crow(i0, g)) = v;
     }
   if (a.lse != nullptr && g == 0)
-    a.lse[row] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l * kLiftInv)) * kLn2;
+    a.lse[row] = l == 0.f ? -INFINITY : (m2 + kLift + __builtin_amdgcn_logf(l * kLiftInv)) * kLn2;
 }
 
 // A call of many items: a launch before lists them (and the parts of those
@@ -1012,7 +1012,9 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         }
       if constexpr (!kHalves) lt = pair_sum(lt);
       if (move) {
-        const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * scale);
+        // (between the offsets as exponentials have them: rounded apart from them, scores of
+        // 2^18 scaled units weighed what was summed before 2^-5 wrong)
+        const float alpha = __builtin_amdgcn_exp2f(neg_m - __builtin_fmaf(-m_run, scale, kLift));
         l_run = l_run * alpha;
 #pragma unroll
         for (int t = 0; t < Sh::kDB; ++t)
@@ -1138,8 +1140,8 @@ __global__ __launch_bounds__(kChThreads, attn_per_cu<D>()) void chunk_attn_kerne
         }
       }
     if constexpr (kHalves) l_run = pair_sum(l_run);
-    // (in units of log 2, as the exponents had it)
-    const float m2 = kLift - __builtin_fmaf(-m_run, scale, kLift);
+    // (in units of log 2, as the exponents had it: less kLift, which adding would round)
+    const float m2 = -__builtin_fmaf(-m_run, scale, kLift);
     if (slot == kWhole) {
       if (live) store_row<D>(a, s, row, g, m2, l_run, acc_o);
     } else if (live) {  // a part: O lifted, l not
@@ -1240,7 +1242,7 @@ __global__ __launch_bounds__(kChThreads) void chunk_join_kernel(ChunkArgs a) {
     *reinterpret_cast<half4*>(o + 4 * v) = half4{(f16)(acc[v].x * inv), (f16)(acc[v].y * inv),
                                                  (f16)(acc[v].z * inv), (f16)(acc[v].w * inv)};
   if (a.lse != nullptr && j0 == 0u)
-    a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    a.lse[at] = l == 0.f ? -INFINITY : (m + kLift + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Workgroups of a call: those that fit on the chip at once, fewer where the

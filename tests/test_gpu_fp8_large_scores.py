@@ -1,4 +1,5 @@
-"""Decode over a cache held in 8 bits where scores are large (whole numbers, so exact in
+"""Attention over a cache held in 8 bits (decode, and of chunks, where an fp16 cache of the
+same values goes through the same kernel) where scores are large (whole numbers, so exact in
 fp32): a key's weight is that of its score to the roundings of probabilities, whether the
 running maximum moved after it and wherever its part was joined.  An offset rounded apart
 from the one that exponentials were taken with would weigh parts by up to a step of the
@@ -9,7 +10,7 @@ import sys
 import pytest
 import torch
 
-from codes import DEV, Coded, within
+from codes import DEV, HND, Coded, values, within
 
 pytestmark = pytest.mark.gpu
 
@@ -44,17 +45,34 @@ def batch(D, S, H, G, L, heads, steps, values=None):
     return r
 
 
-def check(r):
-    """One token's attention against fp64.  Probabilities and the result are rounded to fp16
-    (half a step, 2^-11, each), an exponent below 64 and the exponential are off by 2^-19 at
-    most, sums of L terms by L 2^-24; scores are exact."""
+def decode(r):
     from aoakv import ops
-    q, L = r.q[:1].contiguous(), r.lens[0]
+    q = r.q[:1].contiguous()
     o = torch.zeros_like(q)
     ws = ops.decode_workspace(1, r.H * r.G, r.H, r.max_pages, DEV, head_dim=r.D)
     ops.decode_sparse_attn_fp8(q, o, *r.table(), None, 0, ws, r.max_pages, r.layout)
+    return o
+
+
+def chunk(r):
+    from aoakv import ops
+    return ops.chunk_attn_fp8(r.q, r.q_indptr, *r.table(), r.max_pages, r.layout)
+
+
+def chunk_fp16(r):
+    from aoakv import ops
+    kv = values(r.bytes(), r.exp).half().contiguous()
+    return ops.chunk_attn(r.q, r.q_indptr, kv, r.indptr, r.indices, r.last, r.max_pages, HND)
+
+
+def check(r, call):
+    """One token's attention against fp64.  Probabilities and the result are rounded to fp16
+    (half a step, 2^-11, each), an exponent below 64 and the exponential are off by 2^-19 at
+    most, sums of L terms by L 2^-24; scores are exact."""
+    q, o, L = r.q[:1], call(r), r.lens[0]
+    K, V = r.cached(0, 0), r.cached(0, 1)
     for h in range(r.H):
-        k, v = r.cached(0, 0)[h], r.cached(0, 1)[h]
+        k, v = K[h], V[h]
         a = slice(h * r.G, (h + 1) * r.G)
         t = q[0, a].double() @ k.t()
         assert bool((t == t.round()).all()) and float(t.abs().max()) < 2 ** 24
@@ -68,10 +86,11 @@ def check(r):
 @pytest.mark.parametrize("D,S,H,G,L", [(128, 16, 2, 4, 3000), (128, 7, 2, 8, 3000),
                                        (64, 16, 4, 1, 9000), (256, 16, 2, 2, 3000),
                                        (128, 16, 2, 4, 700)])
-def test_near_equal_maxima(D, S, H, G, L):
+@pytest.mark.parametrize("call", [decode, chunk, chunk_fp16])
+def test_near_equal_maxima(call, D, S, H, G, L):
     """A key in 97 scores 1024 more than the others, and up to 14 more than each other, just
     past 2^18 in scaled units, where the step of fp32 doubles."""
-    _say(f"[large scores fp8] {H} x {G} x {D}, pages of {S}, {L} tokens")
+    _say(f"[large scores fp8] {call.__name__}, {H} x {G} x {D}, pages of {S}, {L} tokens")
     i = torch.arange(L, device=DEV)
     top = (i % 97 == 5).double()
     border = math.log(2) * math.sqrt(D) * 2 ** 18
@@ -81,16 +100,18 @@ def test_near_equal_maxima(D, S, H, G, L):
         first = left // 2 ** 15
         return first, math.ceil((left - first * 2 ** 15) / 2 ** 8 * 16) / 16, 4.0, 8.0
 
-    check(batch(D, S, H, G, L, heads, torch.stack([256 * top, 0.25 * top * (i // 97 * 5 % 8)], 1)))
+    check(batch(D, S, H, G, L, heads, torch.stack([256 * top, 0.25 * top * (i // 97 * 5 % 8)], 1)),
+          call)
 
 
 @pytest.mark.parametrize("D,S,L,step", [(128, 16, 4096, 4.0), (64, 16, 4096, 3.0),
                                         (256, 16, 2048, 6.0), (128, 5, 2055, 4.0)])
-def test_a_maximum_that_moves(D, S, L, step):
+@pytest.mark.parametrize("call", [decode, chunk, chunk_fp16])
+def test_a_maximum_that_moves(call, D, S, L, step):
     """Eight of the last keys have some 2^8 times the weight of each other one: what was summed
     before them is as much as they are."""
-    _say(f"[large scores fp8] a maximum that moves, head dim {D}, pages of {S}, {L} tokens")
+    _say(f"[large scores fp8] a maximum that moves, {call.__name__}, head dim {D}, {L} tokens")
     j = torch.arange(L, device=DEV)
     few = ((j >= L - 256) & (j % 32 == 11)).double()
     check(batch(D, S, 256, 1, L, lambda h: (63.0 - h % 32, 1.0 + h % 7, 16.0, 0.0),
-                torch.stack([step * few, 0 * few], 1), 1 - 2 * few))
+                torch.stack([step * few, 0 * few], 1), 1 - 2 * few), call)
