@@ -368,7 +368,9 @@ def append_kv_cache_fp8(k, v, token_indptr, kv_data, kv_exp, kv_indptr, kv_indic
     k, v [T, Hkv, D] fp16 hold the sequences' new tokens one after the other, rows
     token_indptr[b] .. token_indptr[b + 1] - 1 (int32, device) those of sequence b, the last
     of its cached ones (the page table counts them).  An element becomes a code and its
-    block's exponent in ``kv_exp``, off by at most 2^-4 of itself.  With the five arguments
+    block's exponent e in ``kv_exp``, off by at most 2^-4 of itself and 2^(e - 9) together
+    (small elements of a block are rounded each time that its exponent grows; of one whose
+    exponent does not, 2^-4 or 2^(e - 10), the larger).  With the five arguments
     of the page statistics these are written as append_kv_cache_prefill writes them, from
     the fp16 rows, so that estimate_topk selects the pages it would select of an fp16
     cache."""

@@ -592,10 +592,12 @@ int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t k
  * kv_exp: int8 [max_pages, 2, num_kv_heads], for K (0) and V (1) of each page and
  * kv head (a block) the exponent of its scale: an element is code * 2^exp.  The
  * exponent of a block is the smallest e with max |x| <= 448 * 2^e over its tokens'
- * finite values, held to [-15, 8]: every element is then an fp16 number, off by at
- * most 2^-4 of itself, or by 2^(e - 10) where that is more.  At e = 8 elements end at
- * 61440; inf and NaN are held as NaN.  Exponents outside [-15, 8] are read as the
- * nearest.
+ * finite values, held to [-15, 8]: every element is then an fp16 number.  On the way in
+ * it is rounded by at most 2^-4 of itself, or 2^(e - 10) where that is more; each time
+ * that its block's exponent grows to e', elements below 2^(e' - 6) are rounded again, by
+ * at most 2^(e' - 10).  So an element is off by at most 2^-4 of itself and 2^(e - 9)
+ * together, e its block's exponent now.  At e = 8 elements end at 61440; inf and NaN are
+ * held as NaN.  Exponents outside [-15, 8] are read as the nearest.
  *
  * aoakv_append_kv_cache_fp8: new tokens of EVERY sequence of a batch (chunks of
  * prompts, single tokens, mixed).  k, v: [num_tokens, num_heads, head_dim] fp16;
@@ -603,7 +605,7 @@ int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t k
  * device, ascending; none is allowed), the last of its L_b cached tokens, which
  * the page table already counts; rows of no sequence are not read.  A block that
  * holds older tokens keeps their exponent or gets a larger one, to which their
- * codes move (one rounding of those that become subnormal).  A page that begins
+ * codes move (each time one rounding of those that become subnormal).  A page that begins
  * with the chunk forgets what it held.  Sequences may share a page only if
  * none of them appends to it.  The page statistics (metadata_data, metadata_indptr,
  * metadata_indices, v_log_norm, v_mean: all given, or all NULL) become those of
