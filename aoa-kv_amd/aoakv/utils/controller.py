@@ -20,8 +20,10 @@ switch trees.  Differences, by design:
 * ``kv_dtype=torch.float8_e4m3fn`` holds the cache in 8 bits, half its bytes, with
   the exponents of its blocks' scales in ``kv_exp`` (aoakv.h): the same call order,
   with prefill by the chunk attention and a decode layer of two launches.  Page
-  statistics, so the pages that are selected, are those of an fp16 cache.  Eviction is
-  for fp16 caches.
+  statistics are taken from the fp16 rows, so of the same rows and queries the pages that
+  are selected are those of an fp16 cache (rope_append_kv turns them by more exact angles
+  than it does for an fp16 cache, so there scores differ by roundings, and pages whose
+  scores are that near).  Eviction is for fp16 caches.
 
 ``semantics="quest_kernel"`` switches to the reference kernel's convention
 instead (controller.py:113-124, quest/utils/__init__.py:196-246): the last

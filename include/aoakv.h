@@ -610,12 +610,15 @@ int aoakv_compact_kv_cache(const int32_t* kept, uint32_t kept_stride, uint32_t k
  * none of them appends to it.  The page statistics (metadata_data, metadata_indptr,
  * metadata_indices, v_log_norm, v_mean: all given, or all NULL) become those of
  * aoakv_append_kv_cache_prefill for the same fp16 rows, bit for bit: from the values
- * before they were rounded to codes, so a selection is that of an fp16 cache.
+ * before they were rounded to codes, so a selection by the same queries is that of an
+ * fp16 cache that was given the same rows.
  *
  * aoakv_rope_append_kv_cache_fp8: q [num_tokens, num_qo_heads, head_dim] and k turned
  * on the way, row i of n_b at position L_b - n_b + i, as in
  * aoakv_apply_rope_in_place but for the angle, which is exact to 2^-26 of a turn
- * at every position (that call's is rounded to fp32).  q is turned in place; k
+ * at every position where rope_theta >= 1 and rope_scale >= 2^-10 (that call's is
+ * rounded to fp32, some 1e-3 at position 16000: rows, statistics and a selection near
+ * its cut can differ from those of the fp16 cache's calls).  q is turned in place; k
  * is not written.  q may not share memory with k or v.
  *
  * k, v, q, kv_data, metadata_data and v_mean are aligned to 16 bytes.
