@@ -21,12 +21,18 @@
 // whatever the lengths.
 //
 // Bounds.  K and V are read as fp16 and written as codes, q is read and written; a page's
-// rows stay in registers from the load to the store, so each byte passes once.  8192 tokens of 32 heads, rotated, with statistics: 65 us alone, 5.4
-// TB/s with the reading back of its codes (a large copy: 5.15).  16 chunks of 400 tokens
-// and less: 21 us, where angles, turning and loads of a page follow each other in a
-// workgroup.  One token of 16 sequences: 4.6 us, a launch and the chain of lengths, page
-// id, rows, exponent and codes.  (With the reading back 102 to 111, 27 and 10 us; 131, 45
-// and 12 when a workgroup took K, V and q of its heads in turn, stores between the loads.)
+// rows stay in registers from the load to the store, so each of their bytes passes once.
+// 8192 tokens of 32 heads, rotated, with statistics: 65 us alone, 5.4 TB/s with the reading
+// back of its codes (a large copy: 5.15).  16 chunks of 400 tokens and less: 21 us, where
+// angles, turning and loads of a page follow each other in a workgroup.  One token of 16
+// sequences: 4.6 us, a launch and the chain of lengths, page id, rows, exponent and codes.
+// (With the reading back 102 to 111, 27 and 10 us; 131, 45 and 12 when a workgroup took K, V
+// and q of its heads in turn, stores between the loads.)
+// A block whose exponent grows has its older codes read and written again, token after
+// token: a load does not pass the store before it, so the chain of one block's is what such a
+// step takes, however few grow.  A token each, 8 kv heads, caches restored before each call:
+// 16 sequences 6.4 us where no exponent grows, 10.8 where a tenth does, 12 where all do; 64
+// behind 14 tokens of a page 5.8, 13 and 14, behind 30 6.4, 22 and 23.
 #include "fp8.hpp"
 #include "kernels.hpp"
 

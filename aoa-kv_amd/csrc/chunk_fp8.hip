@@ -8,7 +8,9 @@
 // exactly.  K's lanes read 16 codes of a row, two fragments; V's go through the transposing
 // read of 8-bit elements.  The four waves of a workgroup turn the same codes each for
 // itself, 128 instructions per wave and tile at head dim 128 beside 32 matrix instructions:
-// a prompt of 8192 tokens of 32 heads takes 616 to 632 us (890 TFLOP/s), 572 over fp16.
+// a prompt of 8192 tokens of 32 heads takes 616 to 632 us (890 TFLOP/s), 572 to 590 over
+// fp16; with slopes 674 (fp16 619); 4096 tokens with a cap 228 (204), in pages of 12 232
+// (181), 16 heads of 256 239 (220); 8192 tokens of 32 heads of 64 366 (345).
 // 5 drafted tokens of 8 sequences over up to 16384, 8 kv heads (165 MB), take 53 us: of a
 // workgroup's four waves one has rows, and its chain per tile bounds.  Tiles dealt to the
 // four waves took as long (a buffer per wave: it waits out its own loads), four buffers

@@ -60,10 +60,17 @@ __device__ inline Place place_of(const DecodeFp8Args& a, uint32_t b, uint32_t ch
   return Place{b, chunk, per, beg, a.kv_indptr[b + 1u] - (int32_t)beg,
                (uint32_t)a.kv_last_page_len[b]};
 }
-// The item-th of a call over every page.  The pages of all sequences are cut into chunks of
-// as few pages (at least kGenChunkPages) as leaves a.split of them per kv head, so that all
-// are at work at once and end together.  (Each sequence cut into chunks of a fixed share,
-// 16 sequences made some more than the GPU holds at once: 78 us, then 65.)  A sequence without a page has one.
+// The item-th of a call over every page.  A sequence without a page has one.
+//
+// Up to a.split / 2 sequences: the pages of all are cut into chunks of as few pages (at
+// least kGenChunkPages) as leaves a.split chunks per kv head, which are all at work at once.
+// (Chunks of a fixed share of each sequence were some more than the GPU holds at once: 16
+// sequences 78 us where this way took 65.)
+// More sequences: chunks of an equal share of all pages, and the rest of each sequence as
+// one more, so up to a.split + batch: some begin when the first end, and most of the GPU
+// waits for these.  8000 tokens a sequence, us and TB/s, of 8 kv heads: 15 sequences 58,
+// 4.2; 16 60, 4.4; 17 92, 3.0; 24 123, 3.2; 32 (a chunk each) 102, 5.1; 33 156, 3.5; 64 205,
+// 5.1.  Of 32 kv heads: 4 sequences 54, 4.9; 5 86, 3.8; 8 103, 5.1; 9 155, 3.8.
 __device__ inline Place find_chunk(const DecodeFp8Args& a, uint32_t item) {
   const uint32_t lane = __lane_id();
   auto of = [](uint32_t x, uint32_t j) {
@@ -79,7 +86,7 @@ __device__ inline Place find_chunk(const DecodeFp8Args& a, uint32_t item) {
     if (lane >= a.batch) P = 0u;
     const uint32_t total = of(wave_incl_scan(P), kWave - 1u);
     // chunks of `per` pages; the smallest per that leaves few enough lies between total /
-    // split and total / (split - batch) (many sequences: an equal share)
+    // split and total / (split - batch), where there are not too many sequences for one
     uint32_t n = 0u;
     auto chunks = [&](uint32_t per) {
       n = lane < a.batch ? (P + per - 1u) / per : 0u;
@@ -539,10 +546,15 @@ __global__ __launch_bounds__(kDeThreads, 2) void decode_fp8_kernel(DecodeFp8Args
 // 8 / two of 8 without a batch ahead: 2048 selected of 32768 tokens, 32 heads 10.2 / 9.3 /
 // 9.3; every page of 16384 29 / 28 / 29; 32768 tokens of 4 kv heads of 8 query heads 25 / 18
 // / 22; head dim 256 23 / 19 / 43; 16 sequences of 2000 to 16000 64 / 68 / 65.  Twice the
-// workgroups: 28 -> 33 and 18 -> 28.
+// workgroups: 28 -> 33 and 18 -> 28.  At head dim 64 a CU holds two; 512 / 256 of them, 16000
+// tokens of 8 kv heads: 1 sequence 13.8 / 13.5, 4 22 / 20, 16 58 / 56, 17 68 / 89, 16 ragged
+// ones 40 / 43; 2000 tokens of 32 heads 10.5 / 9.6.
 constexpr uint32_t kDeWorkgroups = 256;
 // Pages per chunk of a selection at least (of every page 8): with a call's two joins 16 are
 // 8.5 us at 2048 tokens of 8 kv heads, 8 9.9; of 1000 tokens on every page 8.5, and 8.1.
+// Chunks are of one length for all sequences, so just past a fill of the GPU the rest waits
+// for a few: 4096 selected tokens of 8 kv heads, 16 sequences 35 us (3.8 TB/s), 17 55 (2.6),
+// 32 61 (4.4), 33 93 (3.0).
 constexpr uint32_t kDeListed = 16u;
 
 }  // namespace
